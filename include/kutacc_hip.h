@@ -422,6 +422,162 @@ typedef struct kutacc_hip_msa_attention_args {
 kutacc_export int64_t kutacc_hip_msa_attention_workspace(int64_t n_seq, int64_t n_res, int64_t nheads, int32_t column);
 kutacc_export int kutacc_hip_msa_attention(const kutacc_hip_msa_attention_args_t *args, void *stream);
 
+/* ---- the feed-forward half of a transformer block (no counterpart in the reference) ---- */
+
+/*
+ * RMS norm with the residual's addition, row by row:
+ *   s = x + residual,   y = s / sqrt(mean(s^2) + eps) * gamma
+ * `sum` receives s and `out` y in storage type (bf16 or fp32), `out8` y in 8 bits (e4m3, OCP: largest value 448) with one scale for
+ * each 128 channels of a row,
+ *   scales[row, g] = max(max |y| / 448, 2^-126),   out8 = e4m3(y / scale), to nearest even:
+ * the operand `a` of kutacc_hip_linear_fp8.  Each of residual, sum, gamma (ones), out and out8 with scales may be NULL, but not all
+ * results.  y is formed from s before its rounding to storage; sums are fp32.  `sum` may be x or residual, and `out` any of the three, with
+ * the same row stride.  A block with a NaN has a NaN for its scale, one with an infinity an infinity.  Any size up to 16384 (beyond:
+ * KUTACC_HIP_EUNSUPPORTED), row strides of at least `size` elements (scales: of at least ceil(size / 128)) and addresses; what lies between
+ * a row's end and the next row is neither read nor written.  rows == 0 is a call that does nothing.
+ */
+typedef struct kutacc_hip_rms_norm_args {
+    int64_t rows;
+    int64_t size;
+    int32_t dtype; /* of x, residual, sum and out: KUTACC_DTYPE_BF16 or KUTACC_DTYPE_FP32 */
+    float eps;     /* >= 0 */
+    const void *x;
+    int64_t x_ld;
+    const void *residual;
+    int64_t residual_ld;
+    const float *gamma; /* [size] */
+    void *sum;
+    int64_t sum_ld;
+    void *out;
+    int64_t out_ld;
+    void *out8;
+    int64_t out8_ld;
+    float *scales; /* [rows, ceil(size / 128)] */
+    int64_t scales_ld;
+} kutacc_hip_rms_norm_args_t;
+
+kutacc_export int kutacc_hip_rms_norm(const kutacc_hip_rms_norm_args_t *args, void *stream);
+
+/*
+ * Its backward pass, from what was normalised (x, or x + residual as `sum` keeps it) and the gradient of y:
+ *   r = 1 / sqrt(mean(x^2) + eps),  h = gamma grad_out
+ *   grad_x = grad_sum + r (h - x r^2 mean(h x)),   grad_gamma = sum over the rows of grad_out x r   (fp32)
+ * grad_sum: the gradient that reached x + residual by other ways than the norm; NULL: none.  grad_x is then the gradient of x and of
+ * residual alike; it may be grad_sum, grad_out or x, with the same row stride.  grad_x or grad_gamma may be NULL.  The sums over rows are
+ * taken in one order for a given number of rows and GPU: the same bits every time.  `workspace`, for grad_gamma alone: device memory,
+ * 256-byte aligned, of at least kutacc_hip_rms_norm_backward_workspace(rows, size) bytes.  rows > 0.
+ */
+typedef struct kutacc_hip_rms_norm_backward_args {
+    int64_t rows;
+    int64_t size;
+    int32_t dtype; /* of x, grad_out, grad_sum and grad_x */
+    float eps;
+    const void *x;
+    int64_t x_ld;
+    const float *gamma;
+    const void *grad_out;
+    int64_t grad_out_ld;
+    const void *grad_sum;
+    int64_t grad_sum_ld;
+    void *grad_x;
+    int64_t grad_x_ld;
+    float *grad_gamma; /* [size] */
+    void *workspace;
+    int64_t workspace_bytes;
+} kutacc_hip_rms_norm_backward_args_t;
+
+kutacc_export int64_t kutacc_hip_rms_norm_backward_workspace(int64_t rows, int64_t size);
+kutacc_export int kutacc_hip_rms_norm_backward(const kutacc_hip_rms_norm_backward_args_t *args, void *stream);
+
+/* x [rows, size] (bf16 or fp32) in 8 bits with scales as kutacc_hip_rms_norm writes them: one for each 128 channels of a row (block_rows 1,
+ * activations; scales [rows, ceil(size / 128)]) or of 128 rows (block_rows 128, weights; scales [ceil(rows / 128), ceil(size / 128)]). */
+kutacc_export int kutacc_hip_quantize_fp8(const void *x, int64_t x_ld, void *out, int64_t out_ld, float *scales, int64_t scales_ld,
+                                          int64_t rows, int64_t size, int32_t block_rows, int32_t dtype, void *stream);
+
+/*
+ * kutacc_hip_linear on 8-bit operands (e4m3) with a scale for each block of 128:
+ *   out[m, n] = sum_k a[m, k] a_scales[m, k / 128] w[n, k] w_scales[n / 128, k / 128] + bias[n]
+ * sums in fp32, rounded once to `dtype`.  Any m, n and k, row strides and addresses; operands whose rows start on multiples of 16 bytes
+ * are read in whole pieces.  m == 0 is a call that does nothing.
+ */
+typedef struct kutacc_hip_linear_fp8_args {
+    int64_t m;
+    int64_t n;
+    int64_t k;
+    int32_t dtype; /* of out: KUTACC_DTYPE_BF16 or KUTACC_DTYPE_FP32 */
+    int32_t reserved;
+    const void *a; /* [m, k] */
+    int64_t a_ld;
+    const float *a_scales; /* [m, ceil(k / 128)] */
+    int64_t a_scales_ld;
+    const void *w; /* [n, k], stored [out, in] */
+    int64_t w_ld;
+    const float *w_scales; /* [ceil(n / 128), ceil(k / 128)] */
+    int64_t w_scales_ld;
+    const float *bias; /* [n] or NULL */
+    void *out; /* [m, n] */
+    int64_t out_ld;
+} kutacc_hip_linear_fp8_args_t;
+
+kutacc_export int kutacc_hip_linear_fp8(const kutacc_hip_linear_fp8_args_t *args, void *stream);
+
+/*
+ * The transition with a gate in the place of its ReLU:
+ *   out = (act(x gate_w^T) * (x up_w^T)) down_w^T
+ * act: KUTACC_HIP_SILU, v / (1 + exp(-v)), or KUTACC_HIP_GELU in its tanh form, v / 2 (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))).  bf16,
+ * weights dense and stored [out, in], sums and the activation fp32; the hidden layer is rounded to bf16 once, as an operand.  Any number of
+ * rows, widths, row strides and addresses.  `out` must not overlap x.  `workspace`: device memory, 256-byte aligned, of at least
+ * kutacc_hip_gated_transition_workspace(rows, c_o, c_i) bytes (may be NULL where that is 0).  rows == 0 is a call that does nothing.
+ */
+#define KUTACC_HIP_SILU 0
+#define KUTACC_HIP_GELU 1
+
+typedef struct kutacc_hip_gated_transition_args {
+    int64_t rows;
+    int64_t c_o; /* channels of x and out */
+    int64_t c_i; /* hidden channels */
+    int32_t dtype; /* KUTACC_DTYPE_BF16 */
+    int32_t activation;
+    const void *x;
+    int64_t x_ld;
+    const void *gate_w, *up_w; /* [c_i, c_o] */
+    const void *down_w;        /* [c_o, c_i] */
+    void *out;
+    int64_t out_ld;
+    void *workspace;
+    int64_t workspace_bytes;
+} kutacc_hip_gated_transition_args_t;
+
+kutacc_export int64_t kutacc_hip_gated_transition_workspace(int64_t rows, int64_t c_o, int64_t c_i);
+kutacc_export int kutacc_hip_gated_transition(const kutacc_hip_gated_transition_args_t *args, void *stream);
+
+/*
+ * Its backward pass: the gradients of x and of the three weights, dense like them, in bf16, from x, the weights and the gradient of out.
+ * The hidden layer is formed again; nothing of the forward pass has to be kept.  Any of the four gradients may be NULL, but not all.
+ * Sums are taken in one order: the same bits every time.  No gradient may overlap another or an input.  rows > 0.
+ */
+typedef struct kutacc_hip_gated_transition_backward_args {
+    int64_t rows;
+    int64_t c_o;
+    int64_t c_i;
+    int32_t dtype; /* KUTACC_DTYPE_BF16 */
+    int32_t activation;
+    const void *x;
+    int64_t x_ld;
+    const void *gate_w, *up_w, *down_w;
+    const void *grad_out;
+    int64_t grad_out_ld;
+    void *grad_x;
+    int64_t grad_x_ld;
+    void *grad_gate_w, *grad_up_w; /* [c_i, c_o] */
+    void *grad_down_w;             /* [c_o, c_i] */
+    void *workspace;
+    int64_t workspace_bytes;
+} kutacc_hip_gated_transition_backward_args_t;
+
+kutacc_export int64_t kutacc_hip_gated_transition_backward_workspace(int64_t rows, int64_t c_o, int64_t c_i);
+kutacc_export int kutacc_hip_gated_transition_backward(const kutacc_hip_gated_transition_backward_args_t *args, void *stream);
+
 /* ---- runtime control (no counterpart in the reference; the CPU library has no device) ---- */
 
 /* Stream used when a `stream` argument is NULL and by the handle-based API of kutacc.h.

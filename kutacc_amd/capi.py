@@ -150,6 +150,49 @@ class HipMsaAttentionArgs(ctypes.Structure):
     ]
 
 
+class HipRmsNormArgs(ctypes.Structure):
+    """kutacc_hip_rms_norm_args_t"""
+    _fields_ = [
+        ("rows", _i64), ("size", _i64), ("dtype", _i32), ("eps", ctypes.c_float), ("x", _vp), ("x_ld", _i64), ("residual", _vp), ("residual_ld", _i64),
+        ("gamma", _vp), ("sum", _vp), ("sum_ld", _i64), ("out", _vp), ("out_ld", _i64), ("out8", _vp), ("out8_ld", _i64), ("scales", _vp),
+        ("scales_ld", _i64),
+    ]
+
+
+class HipRmsNormBackwardArgs(ctypes.Structure):
+    """kutacc_hip_rms_norm_backward_args_t"""
+    _fields_ = [
+        ("rows", _i64), ("size", _i64), ("dtype", _i32), ("eps", ctypes.c_float), ("x", _vp), ("x_ld", _i64), ("gamma", _vp),
+        ("grad_out", _vp), ("grad_out_ld", _i64), ("grad_sum", _vp), ("grad_sum_ld", _i64), ("grad_x", _vp), ("grad_x_ld", _i64),
+        ("grad_gamma", _vp), ("workspace", _vp), ("workspace_bytes", _i64),
+    ]
+
+
+class HipLinearFp8Args(ctypes.Structure):
+    """kutacc_hip_linear_fp8_args_t"""
+    _fields_ = [
+        ("m", _i64), ("n", _i64), ("k", _i64), ("dtype", _i32), ("reserved", _i32), ("a", _vp), ("a_ld", _i64), ("a_scales", _vp),
+        ("a_scales_ld", _i64), ("w", _vp), ("w_ld", _i64), ("w_scales", _vp), ("w_scales_ld", _i64), ("bias", _vp), ("out", _vp), ("out_ld", _i64),
+    ]
+
+
+class HipGatedTransitionArgs(ctypes.Structure):
+    """kutacc_hip_gated_transition_args_t"""
+    _fields_ = [
+        ("rows", _i64), ("c_o", _i64), ("c_i", _i64), ("dtype", _i32), ("activation", _i32), ("x", _vp), ("x_ld", _i64), ("gate_w", _vp),
+        ("up_w", _vp), ("down_w", _vp), ("out", _vp), ("out_ld", _i64), ("workspace", _vp), ("workspace_bytes", _i64),
+    ]
+
+
+class HipGatedTransitionBackwardArgs(ctypes.Structure):
+    """kutacc_hip_gated_transition_backward_args_t"""
+    _fields_ = [
+        ("rows", _i64), ("c_o", _i64), ("c_i", _i64), ("dtype", _i32), ("activation", _i32), ("x", _vp), ("x_ld", _i64), ("gate_w", _vp),
+        ("up_w", _vp), ("down_w", _vp), ("grad_out", _vp), ("grad_out_ld", _i64), ("grad_x", _vp), ("grad_x_ld", _i64), ("grad_gate_w", _vp),
+        ("grad_up_w", _vp), ("grad_down_w", _vp), ("workspace", _vp), ("workspace_bytes", _i64),
+    ]
+
+
 # every symbol the two public headers declare; tests check that the library exports all of them
 DECLARED_SYMBOLS = [
     "kutacc_get_version", "kutacc_af2_gating_attention", "kutacc_af2_global_attention", "kutacc_af2_layernorm",
@@ -168,7 +211,9 @@ DECLARED_SYMBOLS = [
     "kutacc_hip_pair_bias", "kutacc_hip_set_stream", "kutacc_hip_get_stream", "kutacc_hip_set_blocking",
     "kutacc_hip_error_flag", "kutacc_hip_clear_error", "kutacc_hip_tensor_create", "kutacc_hip_tensor_destroy",
     "kutacc_hip_profile_enable", "kutacc_hip_profile_read", "kutacc_hip_set_tuning",
-    "kutacc_hip_gating_attention_static", "kutacc_hip_release_staging",
+    "kutacc_hip_gating_attention_static", "kutacc_hip_release_staging", "kutacc_hip_rms_norm", "kutacc_hip_rms_norm_backward_workspace",
+    "kutacc_hip_rms_norm_backward", "kutacc_hip_quantize_fp8", "kutacc_hip_linear_fp8", "kutacc_hip_gated_transition_workspace",
+    "kutacc_hip_gated_transition", "kutacc_hip_gated_transition_backward_workspace", "kutacc_hip_gated_transition_backward",
 ]
 
 _lib = None
@@ -267,6 +312,20 @@ def lib() -> ctypes.CDLL:
     L.kutacc_hip_msa_attention_workspace.restype = _i64
     L.kutacc_hip_msa_attention.argtypes = [ctypes.POINTER(HipMsaAttentionArgs), _vp]
     L.kutacc_hip_msa_attention.restype = ctypes.c_int
+    L.kutacc_hip_rms_norm.argtypes = [ctypes.POINTER(HipRmsNormArgs), _vp]
+    L.kutacc_hip_rms_norm.restype = ctypes.c_int
+    L.kutacc_hip_rms_norm_backward_workspace.argtypes = [_i64, _i64]
+    L.kutacc_hip_rms_norm_backward_workspace.restype = _i64
+    L.kutacc_hip_rms_norm_backward.argtypes = [ctypes.POINTER(HipRmsNormBackwardArgs), _vp]
+    L.kutacc_hip_rms_norm_backward.restype = ctypes.c_int
+    L.kutacc_hip_quantize_fp8.argtypes = [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i32, _i32, _vp]
+    L.kutacc_hip_quantize_fp8.restype = ctypes.c_int
+    L.kutacc_hip_linear_fp8.argtypes = [ctypes.POINTER(HipLinearFp8Args), _vp]
+    L.kutacc_hip_linear_fp8.restype = ctypes.c_int
+    for name, args in (("gated_transition", HipGatedTransitionArgs), ("gated_transition_backward", HipGatedTransitionBackwardArgs)):
+        workspace, call = getattr(L, f"kutacc_hip_{name}_workspace"), getattr(L, f"kutacc_hip_{name}")
+        workspace.argtypes, workspace.restype = [_i64, _i64, _i64], _i64
+        call.argtypes, call.restype = [ctypes.POINTER(args), _vp], ctypes.c_int
     L.kutacc_hip_set_stream.argtypes = [_vp]
     L.kutacc_hip_get_stream.restype = _vp
     L.kutacc_hip_set_blocking.argtypes = [ctypes.c_int]
@@ -566,3 +625,178 @@ class MsaAttentionBlock:
 
     def run(self, stream_ptr=None) -> int:
         return lib().kutacc_hip_msa_attention(ctypes.byref(self.args), stream_ptr)
+
+
+# ---- the feed-forward half of a transformer block ------------------------------------------------------------
+ACTIVATIONS = {"silu": 0, "gelu": 1}  # KUTACC_HIP_SILU, KUTACC_HIP_GELU
+
+
+def _rows(t, shape, dtype, what):
+    """Address and row stride of a matrix of `shape` and `dtype` (one, or several to choose from) with contiguous rows; (None, 0) for None."""
+    if t is None:
+        return None, 0
+    if tuple(t.shape) != tuple(shape) or t.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
+        raise ValueError(f"{what}: {tuple(t.shape)} of {t.dtype}, wanted {tuple(shape)} of {dtype}")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{what}: its rows are not contiguous")
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+
+def _dense(t, shape, dtype, what):
+    if t is None:
+        return None
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous():
+        raise ValueError(f"{what}: {tuple(t.shape)} of {t.dtype} with strides {t.stride()}, wanted a dense {tuple(shape)} of {dtype}")
+    return t.data_ptr()
+
+
+def _one_device(*tensors):
+    """All on one device: the library's calls run on the current one."""
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) != 1:
+        raise ValueError(f"operands on {sorted(map(str, devices))}")
+
+
+def _workspace(nbytes, device):
+    import torch
+    if nbytes < 0:
+        raise ValueError(f"the library returned {nbytes} for its workspace")
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+class RmsNorm:
+    """One kutacc_hip_rms_norm call on device tensors: x, residual, sum and out [rows, size] in bf16 or fp32, gamma fp32 [size], out8
+    [rows, size] in torch.float8_e4m3fn with scales fp32 [rows, ceil(size / 128)].  Rows contiguous, any row stride.  Each but x may be None, not
+    all results.  `run()` returns the library's code."""
+
+    def __init__(self, x, gamma, eps=1e-6, residual=None, sum=None, out=None, out8=None, scales=None):
+        import torch
+        _one_device(x, gamma, residual, sum, out, out8, scales)
+        self.keep = (x, gamma, residual, sum, out, out8, scales)
+        a = HipRmsNormArgs()
+        a.rows, a.size = x.shape
+        a.dtype, a.eps = _torch_dtype_code(x), eps
+        a.x, a.x_ld = _rows(x, x.shape, (torch.bfloat16, torch.float32), "x")
+        a.residual, a.residual_ld = _rows(residual, x.shape, x.dtype, "residual")
+        a.gamma = _dense(gamma, (a.size,), torch.float32, "gamma")
+        a.sum, a.sum_ld = _rows(sum, x.shape, x.dtype, "sum")
+        a.out, a.out_ld = _rows(out, x.shape, x.dtype, "out")
+        a.out8, a.out8_ld = _rows(out8, x.shape, torch.float8_e4m3fn, "out8")
+        a.scales, a.scales_ld = _rows(scales, (a.rows, -(-a.size // 128)), torch.float32, "scales")
+        self.args = a
+
+    def run(self, stream_ptr=None) -> int:
+        return lib().kutacc_hip_rms_norm(ctypes.byref(self.args), stream_ptr)
+
+
+class RmsNormBackward:
+    """One kutacc_hip_rms_norm_backward call: x (what was normalised), grad_out, grad_sum and grad_x [rows, size], gamma and grad_gamma fp32
+    [size].  Owns the workspace."""
+
+    def __init__(self, x, gamma, grad_out, eps=1e-6, grad_sum=None, grad_x=None, grad_gamma=None):
+        import torch
+        _one_device(x, gamma, grad_out, grad_sum, grad_x, grad_gamma)
+        a = HipRmsNormBackwardArgs()
+        a.rows, a.size = x.shape
+        a.dtype, a.eps = _torch_dtype_code(x), eps
+        a.x, a.x_ld = _rows(x, x.shape, (torch.bfloat16, torch.float32), "x")
+        a.gamma = _dense(gamma, (a.size,), torch.float32, "gamma")
+        a.grad_out, a.grad_out_ld = _rows(grad_out, x.shape, x.dtype, "grad_out")
+        a.grad_sum, a.grad_sum_ld = _rows(grad_sum, x.shape, x.dtype, "grad_sum")
+        a.grad_x, a.grad_x_ld = _rows(grad_x, x.shape, x.dtype, "grad_x")
+        a.grad_gamma = _dense(grad_gamma, (a.size,), torch.float32, "grad_gamma")
+        self.workspace = _workspace(lib().kutacc_hip_rms_norm_backward_workspace(a.rows, a.size) if grad_gamma is not None else 0, x.device)
+        a.workspace, a.workspace_bytes = self.workspace.data_ptr(), self.workspace.numel()
+        self.keep = (x, gamma, grad_out, grad_sum, grad_x, grad_gamma)
+        self.args = a
+
+    def run(self, stream_ptr=None) -> int:
+        return lib().kutacc_hip_rms_norm_backward(ctypes.byref(self.args), stream_ptr)
+
+
+class QuantizeFp8:
+    """One kutacc_hip_quantize_fp8 call: x [rows, size] in bf16 or fp32 -> out in torch.float8_e4m3fn and fp32 scales for blocks of `block_rows` (1:
+    activations, 128: weights) by 128."""
+
+    def __init__(self, x, out, scales, block_rows=1):
+        import torch
+        _one_device(x, out, scales)
+        rows, size = x.shape
+        self.keep = (x, out, scales)
+        self.args = (*_rows(x, x.shape, (torch.bfloat16, torch.float32), "x"), *_rows(out, x.shape, torch.float8_e4m3fn, "out"),
+                     *_rows(scales, (-(-rows // block_rows), -(-size // 128)), torch.float32, "scales"), rows, size, block_rows, _torch_dtype_code(x))
+
+    def run(self, stream_ptr=None) -> int:
+        return lib().kutacc_hip_quantize_fp8(*self.args, stream_ptr)
+
+
+class LinearFp8:
+    """One kutacc_hip_linear_fp8 call: a [m, k] and w [n, k] in torch.float8_e4m3fn, a_scales [m, ceil(k / 128)] and w_scales [ceil(n / 128),
+    ceil(k / 128)], bias [n] fp32, out [m, n] in bf16 or fp32."""
+
+    def __init__(self, a, a_scales, w, w_scales, out, bias=None):
+        import torch
+        _one_device(a, a_scales, w, w_scales, out, bias)
+        self.keep = (a, a_scales, w, w_scales, out, bias)
+        g = HipLinearFp8Args()
+        (g.m, g.k), g.n, g.dtype = a.shape, w.shape[0], _torch_dtype_code(out)
+        blocks = -(-g.k // 128)
+        g.a, g.a_ld = _rows(a, a.shape, torch.float8_e4m3fn, "a")
+        g.a_scales, g.a_scales_ld = _rows(a_scales, (g.m, blocks), torch.float32, "a_scales")
+        g.w, g.w_ld = _rows(w, (g.n, g.k), torch.float8_e4m3fn, "w")
+        g.w_scales, g.w_scales_ld = _rows(w_scales, (-(-g.n // 128), blocks), torch.float32, "w_scales")
+        g.bias = _dense(bias, (g.n,), torch.float32, "bias")
+        g.out, g.out_ld = _rows(out, (g.m, g.n), (torch.bfloat16, torch.float32), "out")
+        self.args = g
+
+    def run(self, stream_ptr=None) -> int:
+        return lib().kutacc_hip_linear_fp8(ctypes.byref(self.args), stream_ptr)
+
+
+class GatedTransition:
+    """One kutacc_hip_gated_transition call: x and out [rows, c_o], gate_w and up_w [c_i, c_o], down_w [c_o, c_i], all bf16; activation "silu" or
+    "gelu".  Owns the workspace."""
+
+    def __init__(self, x, gate_w, up_w, down_w, out, activation="silu"):
+        import torch
+        _one_device(x, gate_w, up_w, down_w, out)
+        bf16 = torch.bfloat16
+        a = HipGatedTransitionArgs()
+        (a.rows, a.c_o), a.c_i, a.dtype, a.activation = x.shape, gate_w.shape[0], K_BF16, ACTIVATIONS[activation]
+        a.x, a.x_ld = _rows(x, x.shape, bf16, "x")
+        a.gate_w, a.up_w = _dense(gate_w, (a.c_i, a.c_o), bf16, "gate_w"), _dense(up_w, (a.c_i, a.c_o), bf16, "up_w")
+        a.down_w = _dense(down_w, (a.c_o, a.c_i), bf16, "down_w")
+        a.out, a.out_ld = _rows(out, x.shape, bf16, "out")
+        self.workspace = _workspace(lib().kutacc_hip_gated_transition_workspace(a.rows, a.c_o, a.c_i), x.device)
+        a.workspace, a.workspace_bytes = self.workspace.data_ptr(), self.workspace.numel()
+        self.keep = (x, gate_w, up_w, down_w, out)
+        self.args = a
+
+    def run(self, stream_ptr=None) -> int:
+        return lib().kutacc_hip_gated_transition(ctypes.byref(self.args), stream_ptr)
+
+
+class GatedTransitionBackward:
+    """One kutacc_hip_gated_transition_backward call: the gradients of x and of the three weights (each may be None, not all) from grad_out and
+    the forward pass's inputs.  Owns the workspace."""
+
+    def __init__(self, x, gate_w, up_w, down_w, grad_out, grad_x=None, grad_gate_w=None, grad_up_w=None, grad_down_w=None, activation="silu"):
+        import torch
+        _one_device(x, gate_w, up_w, down_w, grad_out, grad_x, grad_gate_w, grad_up_w, grad_down_w)
+        bf16 = torch.bfloat16
+        a = HipGatedTransitionBackwardArgs()
+        (a.rows, a.c_o), a.c_i, a.dtype, a.activation = x.shape, gate_w.shape[0], K_BF16, ACTIVATIONS[activation]
+        wide, tall = (a.c_i, a.c_o), (a.c_o, a.c_i)
+        a.x, a.x_ld = _rows(x, x.shape, bf16, "x")
+        a.gate_w, a.up_w, a.down_w = _dense(gate_w, wide, bf16, "gate_w"), _dense(up_w, wide, bf16, "up_w"), _dense(down_w, tall, bf16, "down_w")
+        a.grad_out, a.grad_out_ld = _rows(grad_out, x.shape, bf16, "grad_out")
+        a.grad_x, a.grad_x_ld = _rows(grad_x, x.shape, bf16, "grad_x")
+        a.grad_gate_w, a.grad_up_w = _dense(grad_gate_w, wide, bf16, "grad_gate_w"), _dense(grad_up_w, wide, bf16, "grad_up_w")
+        a.grad_down_w = _dense(grad_down_w, tall, bf16, "grad_down_w")
+        self.workspace = _workspace(lib().kutacc_hip_gated_transition_backward_workspace(a.rows, a.c_o, a.c_i), x.device)
+        a.workspace, a.workspace_bytes = self.workspace.data_ptr(), self.workspace.numel()
+        self.keep = (x, gate_w, up_w, down_w, grad_out, grad_x, grad_gate_w, grad_up_w, grad_down_w)
+        self.args = a
+
+    def run(self, stream_ptr=None) -> int:
+        return lib().kutacc_hip_gated_transition_backward(ctypes.byref(self.args), stream_ptr)

@@ -214,4 +214,21 @@ int pair_bias(const void *z, const float *gamma, const float *beta, const void *
 bool pair_bias_writes_fragments(const void *z, const void *w, const void *z_norm, int64_t rows_i, int64_t rows_j, int64_t c_z,
                                 int64_t nheads, int32_t dtype);
 
+// rms_norm.hip: arguments as checked by api_feed_forward.cpp, here and below
+bool rms_norm_supports(int64_t size);
+int rms_norm(const kutacc_hip_rms_norm_args_t &args, hipStream_t stream);
+int64_t rms_norm_backward_workspace(int64_t rows, int64_t size);
+int rms_norm_backward(const kutacc_hip_rms_norm_backward_args_t &args, hipStream_t stream);
+int quantize_fp8(const void *x, int64_t x_ld, void *out, int64_t out_ld, float *scales, int64_t scales_ld, int64_t rows, int64_t size,
+                 int32_t block_rows, int32_t dtype, hipStream_t stream);
+
+// fp8_linear.hip
+int linear_fp8(const kutacc_hip_linear_fp8_args_t &args, hipStream_t stream);
+
+// gated_transition.hip
+int64_t gated_transition_workspace(int64_t rows, int64_t c_o, int64_t c_i);
+int gated_transition(const kutacc_hip_gated_transition_args_t &args, hipStream_t stream);
+int64_t gated_transition_backward_workspace(int64_t rows, int64_t c_o, int64_t c_i);
+int gated_transition_backward(const kutacc_hip_gated_transition_backward_args_t &args, hipStream_t stream);
+
 } // namespace kutacc_launch

@@ -1,0 +1,432 @@
+// RMS norm with the residual's addition, into the storage type and / or 8 bits with a scale for 128 channels, its backward pass, and the
+// quantiser by itself.
+//
+//   s = x + residual,  r = 1 / sqrt(mean(s^2) + eps),  y = s r gamma
+//   scale = max(max |y| / 448, 2^-126) over a row's channels 128 g .. 128 g + 127,  q = e4m3(y / scale)
+// backward, with h = gamma dy:
+//   ds = d_sum + r (h - s r^2 mean(h s)),  dgamma = sum over the rows of dy s r
+//
+// All sums are fp32, and y is formed from s before its rounding to storage.  Memory bounds them: a row is read once, held in
+// registers (8 values a lane and chunk) over its reduction, and written once.  TPR threads share a row, each with NV chunks, chunk
+// TPR i + thread: whole lines a load, and the 16 lanes whose chunks make up a block of 128 are neighbours, so that a scale costs four DPP
+// steps.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "launch_internal.h"
+#include "profiler.h"
+#include "row_chunks.h"
+
+namespace {
+using namespace kutacc_dev;
+
+constexpr int MAX_SIZE = 16384; // of a row: what 1024 threads hold with two chunks each (with four the backward pass has no registers)
+
+// the sum over the TPR threads of a row, in all of them; `waves` for more than a wave a row: one float for each wave of the workgroup
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float *waves)
+{
+    if constexpr (TPR <= 64) {
+        return group_sum<TPR>(v);
+    } else {
+        v = group_sum<64>(v);
+        const int wave = threadIdx.x >> 6, first = (int)threadIdx.x / TPR * (TPR / 64);
+        __syncthreads(); // the last row's sums have been read
+        if ((threadIdx.x & 63) == 0) {
+            waves[wave] = v;
+        }
+        __syncthreads();
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < TPR / 64; ++w) {
+            sum += waves[first + w];
+        }
+        return sum;
+    }
+}
+
+struct NormParams {
+    const void *x, *residual;
+    void *sum, *out;
+    uint8_t *out8;
+    const float *gamma;
+    float *scales;
+    int64_t x_ld, residual_ld, sum_ld, out_ld, out8_ld, scales_ld, rows;
+    int size;
+    float eps;
+};
+
+template <int TPR>
+constexpr int threads_of() { return TPR > 256 ? TPR : 256; }
+
+template <typename T, int TPR, int NV>
+__global__ __launch_bounds__(threads_of<TPR>()) void rms_norm_kernel(const NormParams p)
+{
+    constexpr int ROWS = threads_of<TPR>() / TPR;
+    __shared__ float waves[threads_of<TPR>() / 64];
+    const int t = (int)threadIdx.x % TPR;
+    const int64_t row = (int64_t)blockIdx.x * ROWS + (int)threadIdx.x / TPR;
+    const bool there = row < p.rows;
+    const int64_t at = there ? row : 0;
+    const int size = there ? p.size : 0; // a row past the end reads and writes nothing
+    const T *x = (const T *)p.x + at * p.x_ld;
+    float v[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        load_chunk(v[i], x, 8 * (TPR * i + t), size);
+    }
+    if (p.residual != nullptr) {
+        const T *residual = (const T *)p.residual + at * p.residual_ld;
+        float add[NV][8];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            load_chunk(add[i], residual, 8 * (TPR * i + t), size);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[i][e] += add[i][e];
+            }
+        }
+    }
+    float squares = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            squares = fmaf(v[i][e], v[i][e], squares);
+        }
+    }
+    if (p.sum != nullptr) {
+        T *sum = (T *)p.sum + at * p.sum_ld;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            store_chunk(v[i], sum, 8 * (TPR * i + t), size);
+        }
+    }
+    const float r = 1.0f / sqrtf(row_sum<TPR>(squares, waves) / (float)p.size + p.eps);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = 8 * (TPR * i + t);
+        if (p.gamma != nullptr) {
+            float gamma[8];
+            load_chunk(gamma, p.gamma, c, p.size);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[i][e] = v[i][e] * r * gamma[e];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[i][e] *= r;
+            }
+        }
+        if (p.out != nullptr) {
+            store_chunk(v[i], (T *)p.out + at * p.out_ld, c, size);
+        }
+        if (p.out8 != nullptr) {
+            const float scale = fp8_scale(lanes_max<(TPR < 16 ? 8 : 16)>(abs_max(v[i])));
+            store_fp8_chunk(fp8_quotients(v[i], scale), p.out8 + at * p.out8_ld, c, size);
+            if (c < size && c % FP8_BLOCK == 0) {
+                p.scales[at * p.scales_ld + c / FP8_BLOCK] = scale;
+            }
+        }
+    }
+}
+
+struct BackwardParams {
+    const void *x, *grad_out, *grad_sum;
+    const float *gamma;
+    void *grad_x;
+    float *partial; // [workgroups][size]: each one's share of dgamma
+    int64_t x_ld, grad_out_ld, grad_sum_ld, grad_x_ld, rows;
+    int size;
+    float eps;
+};
+
+// A workgroup walks rows, ROWS at a time, and keeps its share of dgamma in registers.  The shares meet in the LDS and then, in another kernel,
+// over the workgroups, always in one order.
+template <typename T, int TPR, int NV>
+__global__ __launch_bounds__(threads_of<TPR>()) void rms_norm_backward_kernel(const BackwardParams p)
+{
+    constexpr int THREADS = threads_of<TPR>(), ROWS = THREADS / TPR;
+    __shared__ float waves[THREADS / 64];
+    __shared__ float shares[ROWS > 1 ? THREADS * 8 : 1];
+    const int t = (int)threadIdx.x % TPR, group = (int)threadIdx.x / TPR;
+    float gamma[NV][8], share[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if (p.gamma != nullptr) {
+            load_chunk(gamma[i], p.gamma, 8 * (TPR * i + t), p.size);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            gamma[i][e] = p.gamma != nullptr ? gamma[i][e] : 1.f;
+            share[i][e] = 0.f;
+        }
+    }
+    for (int64_t first = (int64_t)blockIdx.x * ROWS; first < p.rows; first += (int64_t)gridDim.x * ROWS) {
+        const bool there = first + group < p.rows;
+        const int64_t at = there ? first + group : 0;
+        const int size = there ? p.size : 0;
+        float x[NV][8], dy[NV][8];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            load_chunk(x[i], (const T *)p.x + at * p.x_ld, 8 * (TPR * i + t), size);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            load_chunk(dy[i], (const T *)p.grad_out + at * p.grad_out_ld, 8 * (TPR * i + t), size);
+        }
+        float squares = 0.f, products = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                squares = fmaf(x[i][e], x[i][e], squares);
+                products = fmaf(dy[i][e] * gamma[i][e], x[i][e], products);
+            }
+        }
+        const float n = (float)p.size;
+        const float r = 1.0f / sqrtf(row_sum<TPR>(squares, waves) / n + p.eps);
+        const float pull = r * r * (row_sum<TPR>(products, waves) / n);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = 8 * (TPR * i + t);
+            float dx[8];
+            if (p.grad_sum != nullptr) {
+                load_chunk(dx, (const T *)p.grad_sum + at * p.grad_sum_ld, c, size);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float own = r * (dy[i][e] * gamma[i][e] - x[i][e] * pull);
+                dx[e] = p.grad_sum != nullptr ? dx[e] + own : own;
+                share[i][e] = there ? fmaf(dy[i][e] * x[i][e], r, share[i][e]) : share[i][e];
+            }
+            if (p.grad_x != nullptr) {
+                store_chunk(dx, (T *)p.grad_x + at * p.grad_x_ld, c, size);
+            }
+        }
+    }
+    if (p.partial == nullptr) {
+        return;
+    }
+    float *partial = p.partial + (int64_t)blockIdx.x * p.size;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if constexpr (ROWS > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                shares[(group * TPR + t) * 8 + e] = share[i][e];
+            }
+            __syncthreads();
+            for (int j = threadIdx.x; j < TPR * 8; j += THREADS) {
+                float sum = 0.f;
+                for (int g = 0; g < ROWS; ++g) {
+                    sum += shares[g * TPR * 8 + j];
+                }
+                if (8 * TPR * i + j < p.size) {
+                    partial[8 * TPR * i + j] = sum;
+                }
+            }
+        } else {
+            store_chunk(share[i], partial, 8 * (TPR * i + t), p.size);
+        }
+    }
+}
+
+// dgamma from its shares: 32 columns a workgroup, 8 threads a column
+__global__ __launch_bounds__(256) void column_sums_kernel(const float *partial, float *out, int count, int size)
+{
+    __shared__ float part[8][32];
+    const int c = (int)threadIdx.x & 31, slice = (int)threadIdx.x >> 5, column = (int)blockIdx.x * 32 + c;
+    float sum = 0.f;
+    if (column < size) {
+        for (int i = slice; i < count; i += 8) {
+            sum += partial[(int64_t)i * size + column];
+        }
+    }
+    part[slice][c] = sum;
+    __syncthreads();
+    if (slice == 0 && column < size) {
+#pragma unroll
+        for (int s = 1; s < 8; ++s) {
+            sum += part[s][c];
+        }
+        out[column] = sum;
+    }
+}
+
+// Blocks of BLOCK_ROWS x 128 values with a scale each: 16 lanes a row of a block, and 256 threads a block of 128 rows (8 rows each)
+// or 16 blocks of one row.
+struct QuantizeParams {
+    const void *x;
+    uint8_t *out;
+    float *scales;
+    int64_t x_ld, out_ld, scales_ld, rows;
+    int size, blocks_across;
+};
+
+template <typename T, int BLOCK_ROWS>
+__global__ __launch_bounds__(256) void quantize_fp8_kernel(const QuantizeParams p)
+{
+    constexpr int NV = BLOCK_ROWS == 1 ? 1 : BLOCK_ROWS / 16;
+    __shared__ float waves[4];
+    const int lane16 = (int)threadIdx.x & 15, sub = (int)threadIdx.x >> 4;
+    int64_t row0;
+    int block;
+    bool there = true;
+    if constexpr (BLOCK_ROWS == 1) {
+        const int64_t unit = (int64_t)blockIdx.x * 16 + sub;
+        there = unit < p.rows * p.blocks_across;
+        row0 = there ? unit / p.blocks_across : 0;
+        block = there ? (int)(unit % p.blocks_across) : 0;
+    } else {
+        row0 = (int64_t)(blockIdx.x / (unsigned)p.blocks_across) * BLOCK_ROWS + sub;
+        block = (int)(blockIdx.x % (unsigned)p.blocks_across);
+    }
+    const int c = block * FP8_BLOCK + lane16 * 8;
+    float v[NV][8], largest = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int64_t row = row0 + 16 * i;
+        load_chunk(v[i], (const T *)p.x + (row < p.rows ? row : 0) * p.x_ld, c, there && row < p.rows ? p.size : 0);
+        largest = __builtin_elementwise_maximum(largest, abs_max(v[i]));
+    }
+    largest = lanes_max<16>(largest);
+    if constexpr (BLOCK_ROWS != 1) {
+        largest = __builtin_elementwise_maximum(largest, __shfl_xor(largest, 16, 64));
+        largest = __builtin_elementwise_maximum(largest, __shfl_xor(largest, 32, 64));
+        if ((threadIdx.x & 63) == 0) {
+            waves[threadIdx.x >> 6] = largest;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            largest = __builtin_elementwise_maximum(largest, waves[w]);
+        }
+    }
+    const float scale = fp8_scale(largest);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int64_t row = row0 + 16 * i;
+        if (there && row < p.rows) {
+            store_fp8_chunk(fp8_quotients(v[i], scale), p.out + row * p.out_ld, c, p.size);
+        }
+    }
+    if (there && lane16 == 0 && (BLOCK_ROWS == 1 || sub == 0)) {
+        p.scales[row0 / BLOCK_ROWS * p.scales_ld + block] = scale;
+    }
+}
+
+// Threads a row and chunks a thread for a row of `size`, as f(TPR, NV): the fewest that hold it, up to a wave with two chunks ...
+template <typename F>
+int by_size(int64_t size, F f)
+{
+    using std::integral_constant;
+#define KUTACC_ROW(limit, tpr, nv)                                                   \
+    if (size <= (limit)) {                                                            \
+        return f(integral_constant<int, tpr>{}, integral_constant<int, nv>{});        \
+    }
+    KUTACC_ROW(64, 8, 1)
+    KUTACC_ROW(128, 16, 1)
+    KUTACC_ROW(256, 32, 1)
+    KUTACC_ROW(512, 64, 1)
+    KUTACC_ROW(1024, 64, 2)
+    KUTACC_ROW(2048, 256, 1) // ... then workgroups
+    KUTACC_ROW(4096, 256, 2)
+    KUTACC_ROW(8192, 512, 2)
+    KUTACC_ROW(MAX_SIZE, 1024, 2)
+#undef KUTACC_ROW
+    return KUTACC_HIP_EUNSUPPORTED;
+}
+
+template <typename F>
+int by_type(int32_t dtype, F f)
+{
+    return dtype == KUTACC_DTYPE_BF16 ? f(bf16_t{}) : f(float{});
+}
+
+// workgroups of the backward pass: as many as the chip holds twice over, each with its share of dgamma
+int64_t backward_groups(int64_t rows, int64_t size)
+{
+    int per_group = 1;
+    (void)by_size(size, [&](auto tpr, auto) {
+        per_group = threads_of<decltype(tpr)::value>() / decltype(tpr)::value;
+        return 0;
+    });
+    const int64_t needed = (rows + per_group - 1) / per_group;
+    return std::min<int64_t>(needed, 4 * (int64_t)kutacc_cu_count());
+}
+} // namespace
+
+namespace kutacc_launch {
+
+int rms_norm(const kutacc_hip_rms_norm_args_t &a, hipStream_t stream)
+{
+    const NormParams p = {a.x, a.residual, a.sum, a.out, (uint8_t *)a.out8, a.gamma, a.scales,
+                          a.x_ld, a.residual_ld, a.sum_ld, a.out_ld, a.out8_ld, a.scales_ld, a.rows, (int)a.size, a.eps};
+    return by_type(a.dtype, [&](auto type) {
+        return by_size(a.size, [&](auto tpr, auto nv) {
+            constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, THREADS = threads_of<TPR>();
+            const int64_t blocks = (p.rows + THREADS / TPR - 1) / (THREADS / TPR);
+            if (blocks > INT32_MAX) {
+                return KUTACC_HIP_EUNSUPPORTED;
+            }
+            kutacc_prof::KernelTimer t("rms_norm_kernel", 8.0 * (double)p.rows * (double)p.size, stream);
+            rms_norm_kernel<decltype(type), TPR, NV><<<dim3((unsigned)blocks), THREADS, 0, stream>>>(p);
+            return kutacc_hip_status(hipGetLastError());
+        });
+    });
+}
+
+int64_t rms_norm_backward_workspace(int64_t rows, int64_t size) { return backward_groups(rows, size) * size * (int64_t)sizeof(float); }
+
+int rms_norm_backward(const kutacc_hip_rms_norm_backward_args_t &a, hipStream_t stream)
+{
+    const int64_t groups = backward_groups(a.rows, a.size);
+    const BackwardParams p = {a.x, a.grad_out, a.grad_sum, a.gamma, a.grad_x, a.grad_gamma != nullptr ? (float *)a.workspace : nullptr,
+                              a.x_ld, a.grad_out_ld, a.grad_sum_ld, a.grad_x_ld, a.rows, (int)a.size, a.eps};
+    const int rc = by_type(a.dtype, [&](auto type) {
+        return by_size(a.size, [&](auto tpr, auto nv) {
+            constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
+            kutacc_prof::KernelTimer t("rms_norm_backward_kernel", 12.0 * (double)p.rows * (double)p.size, stream);
+            rms_norm_backward_kernel<decltype(type), TPR, NV><<<dim3((unsigned)groups), threads_of<TPR>(), 0, stream>>>(p);
+            return kutacc_hip_status(hipGetLastError());
+        });
+    });
+    if (rc != 0 || a.grad_gamma == nullptr) {
+        return rc;
+    }
+    kutacc_prof::KernelTimer t("column_sums_kernel", (double)groups * (double)a.size, stream);
+    column_sums_kernel<<<dim3((unsigned)((a.size + 31) / 32)), 256, 0, stream>>>(p.partial, a.grad_gamma, (int)groups, (int)a.size);
+    return kutacc_hip_status(hipGetLastError());
+}
+
+int quantize_fp8(const void *x, int64_t x_ld, void *out, int64_t out_ld, float *scales, int64_t scales_ld, int64_t rows, int64_t size,
+                 int32_t block_rows, int32_t dtype, hipStream_t stream)
+{
+    const int across = (int)((size + FP8_BLOCK - 1) / FP8_BLOCK);
+    const QuantizeParams p = {x, (uint8_t *)out, scales, x_ld, out_ld, scales_ld, rows, (int)size, across};
+    const int64_t blocks = block_rows == 1 ? (rows * across + 15) / 16 : (rows + FP8_BLOCK - 1) / FP8_BLOCK * across;
+    if (blocks > INT32_MAX) {
+        return KUTACC_HIP_EUNSUPPORTED;
+    }
+    return by_type(dtype, [&](auto type) {
+        kutacc_prof::KernelTimer t("quantize_fp8_kernel", (double)rows * (double)size, stream);
+        if (block_rows == 1) {
+            quantize_fp8_kernel<decltype(type), 1><<<dim3((unsigned)blocks), 256, 0, stream>>>(p);
+        } else {
+            quantize_fp8_kernel<decltype(type), FP8_BLOCK><<<dim3((unsigned)blocks), 256, 0, stream>>>(p);
+        }
+        return kutacc_hip_status(hipGetLastError());
+    });
+}
+
+bool rms_norm_supports(int64_t size) { return size <= MAX_SIZE; }
+
+} // namespace kutacc_launch

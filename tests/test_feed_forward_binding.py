@@ -1,0 +1,48 @@
+"""What the Python owners of the feed-forward calls refuse of their tensors, on the CPU."""
+import pytest
+import torch
+
+from kutacc_amd import capi
+
+BF16, E4M3 = torch.bfloat16, torch.float8_e4m3fn
+
+
+def e(*shape, dtype=BF16):
+    return torch.empty(*shape, dtype=dtype)
+
+
+def test_rms_norm_owner_refuses_wrong_tensors():
+    x = e(4, 64)
+    capi.RmsNorm(x, None, out=e(4, 64))
+    for bad in (dict(out=e(4, 63)), dict(out=e(4, 64, dtype=torch.float32)), dict(residual=e(64, 4).t()), dict(out8=e(4, 64)), dict(scales=e(4, 2, dtype=torch.float32)),
+                dict(out=torch.empty(4, 64, dtype=BF16, device="meta"))):
+        with pytest.raises(ValueError):
+            capi.RmsNorm(x, None, **bad)
+    with pytest.raises(ValueError):
+        capi.RmsNorm(x, e(64), out=e(4, 64))  # gamma is fp32
+    with pytest.raises(ValueError):
+        capi.RmsNormBackward(x, None, e(4, 65), grad_x=e(4, 64))
+
+
+def test_linear_owner_refuses_wrong_tensors():
+    a, s, w, ws = e(4, 300, dtype=E4M3), e(4, 3, dtype=torch.float32), e(200, 300, dtype=E4M3), e(2, 3, dtype=torch.float32)
+    capi.LinearFp8(a, s, w, ws, e(4, 200))
+    for args in ((e(4, 300), s, w, ws, e(4, 200)), (a, e(4, 2, dtype=torch.float32), w, ws, e(4, 200)), (a, s, e(200, 301, dtype=E4M3), ws, e(4, 200)),
+                 (a, s, w, e(1, 3, dtype=torch.float32), e(4, 200)), (a, s, w, ws, e(4, 201)), (a, s, w, ws, e(4, 200, dtype=torch.float16))):
+        with pytest.raises((ValueError, TypeError)):
+            capi.LinearFp8(*args)
+    with pytest.raises(ValueError):
+        capi.QuantizeFp8(e(4, 300), e(4, 300, dtype=E4M3), e(4, 2, dtype=torch.float32))
+
+
+def test_transition_owner_refuses_wrong_tensors():
+    x, wide, tall = e(4, 64), e(96, 64), e(64, 96)
+    capi.GatedTransition(x, wide, wide, tall, e(4, 64))
+    for args in ((x, wide, e(95, 64), tall, e(4, 64)), (x, wide, wide, wide, e(4, 64)), (x, wide, wide, e(96, 64).t(), e(4, 64)), (x, wide, wide, tall, e(4, 65)),
+                 (x.float(), wide, wide, tall, e(4, 64))):
+        with pytest.raises(ValueError):
+            capi.GatedTransition(*args)
+    with pytest.raises(KeyError):
+        capi.GatedTransition(x, wide, wide, tall, e(4, 64), activation="relu")
+    with pytest.raises(ValueError):
+        capi.GatedTransitionBackward(x, wide, wide, tall, e(4, 64), grad_gate_w=tall)
