@@ -250,6 +250,19 @@ def test_linear_fp8(out, m, n, k):
         room.untouched("out")
 
 
+# enough 128 x 128 and 256 x 256 tiles for kernels of their own: ragged sides, a cut last block, several spans of scales, one block alone
+@pytest.mark.parametrize("out,m,n,k", [("bf16", 1700, 1500, 2448), ("fp32", 1700, 1500, 2448), ("bf16", 1793, 1409, 112), ("fp32", 1665, 1537, 144), ("bf16", 2900, 4100, 1168),
+                                       ("bf16", 3329, 3841, 96), ("bf16", 3400, 3800, 128), ("bf16", 23000, 130, 256)])
+def test_linear_fp8_of_many_rows(out, m, n, k):
+    dt = TYPES[out]
+    a, a_scales, w, w_scales = eight_bits(m + n + k, m, n, k)
+    room = Room(m, n, dt)
+    ok(capi.LinearFp8(a.cuda(), a_scales.cuda(), w.cuda(), w_scales.cuda(), room.view))
+    want, off = oracle.linear_fp8(a, a_scales, w, w_scales, None, dt)
+    oracle.close(room.view, want, oracle.stored(want, off, dt), f"{m} x {n} x {k}")
+    room.untouched("out")
+
+
 @pytest.mark.parametrize("m,n,k,pad,offset", [(3, 200, 256, 16, 16), (3, 200, 256, 5, 3), (40, 130, 300, 1, 1), (150, 260, 512, 16, 0), (150, 260, 512, 7, 9)])
 def test_linear_fp8_of_rows_on_any_address(m, n, k, pad, offset):
     a, a_scales, w, w_scales = eight_bits(9, m, n, k)
