@@ -24,7 +24,7 @@ using namespace kutacc_dev;
 
 constexpr int MAX_SIZE = 16384; // of a row: what 1024 threads hold with two chunks each (with four the backward pass has no registers)
 
-// the sum over the TPR threads of a row, in all of them; `waves` for more than a wave a row: one float for each wave of the workgroup
+// the sum over the TPR threads of a row, in all of them; `waves` where these are a whole workgroup: one float for each of its waves
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float *waves)
 {
@@ -32,18 +32,37 @@ __device__ __forceinline__ float row_sum(float v, float *waves)
         return group_sum<TPR>(v);
     } else {
         v = group_sum<64>(v);
-        const int wave = threadIdx.x >> 6, first = (int)threadIdx.x / TPR * (TPR / 64);
-        __syncthreads(); // the last row's sums have been read
         if ((threadIdx.x & 63) == 0) {
-            waves[wave] = v;
+            waves[threadIdx.x >> 6] = v;
         }
         __syncthreads();
         float sum = 0.f;
 #pragma unroll
         for (int w = 0; w < TPR / 64; ++w) {
-            sum += waves[first + w];
+            sum += waves[w];
         }
         return sum;
+    }
+}
+
+// two sums at once
+template <int TPR>
+__device__ __forceinline__ void row_sums(float &a, float &b, float *waves)
+{
+    if constexpr (TPR <= 64) {
+        a = group_sum<TPR>(a), b = group_sum<TPR>(b);
+    } else {
+        a = group_sum<64>(a), b = group_sum<64>(b);
+        __syncthreads(); // the last row's sums have been read
+        if ((threadIdx.x & 63) == 0) {
+            waves[2 * (threadIdx.x >> 6)] = a, waves[2 * (threadIdx.x >> 6) + 1] = b;
+        }
+        __syncthreads();
+        a = b = 0.f;
+#pragma unroll
+        for (int w = 0; w < TPR / 64; ++w) {
+            a += waves[2 * w], b += waves[2 * w + 1];
+        }
     }
 }
 
@@ -153,7 +172,7 @@ template <typename T, int TPR, int NV>
 __global__ __launch_bounds__(threads_of<TPR>()) void rms_norm_backward_kernel(const BackwardParams p)
 {
     constexpr int THREADS = threads_of<TPR>(), ROWS = THREADS / TPR;
-    __shared__ float waves[THREADS / 64];
+    __shared__ float waves[THREADS / 32];
     __shared__ float shares[ROWS > 1 ? THREADS * 8 : 1];
     const int t = (int)threadIdx.x % TPR, group = (int)threadIdx.x / TPR;
     float gamma[NV][8], share[NV][8];
@@ -168,46 +187,69 @@ __global__ __launch_bounds__(threads_of<TPR>()) void rms_norm_backward_kernel(co
             share[i][e] = 0.f;
         }
     }
-    for (int64_t first = (int64_t)blockIdx.x * ROWS; first < p.rows; first += (int64_t)gridDim.x * ROWS) {
-        const bool there = first + group < p.rows;
-        const int64_t at = there ? first + group : 0;
-        const int size = there ? p.size : 0;
+    struct Row {
         float x[NV][8], dy[NV][8];
+        bool there;
+        int64_t at;
+    } now, next;
+    auto load = [&](Row &row, int64_t first) {
+        row.there = first + group < p.rows;
+        row.at = row.there ? first + group : 0;
+        const int size = row.there ? p.size : 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            load_chunk(x[i], (const T *)p.x + at * p.x_ld, 8 * (TPR * i + t), size);
+            load_chunk(row.x[i], (const T *)p.x + row.at * p.x_ld, 8 * (TPR * i + t), size);
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            load_chunk(dy[i], (const T *)p.grad_out + at * p.grad_out_ld, 8 * (TPR * i + t), size);
+            load_chunk(row.dy[i], (const T *)p.grad_out + row.at * p.grad_out_ld, 8 * (TPR * i + t), size);
         }
+    };
+    const int64_t step = (int64_t)gridDim.x * ROWS;
+    int64_t first = (int64_t)blockIdx.x * ROWS;
+    constexpr bool AHEAD = TPR * NV < 2048; // beyond, two rows have no registers
+    load(now, first);
+    for (; first < p.rows; first += step) {
+        const bool more = first + step < p.rows;
+        if (AHEAD && more) {
+            load(next, first + step); // on its way while this one is reduced and written
+        }
+        const int size = now.there ? p.size : 0;
         float squares = 0.f, products = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                squares = fmaf(x[i][e], x[i][e], squares);
-                products = fmaf(dy[i][e] * gamma[i][e], x[i][e], products);
+                squares = fmaf(now.x[i][e], now.x[i][e], squares);
+                products = fmaf(now.dy[i][e] * gamma[i][e], now.x[i][e], products);
             }
         }
         const float n = (float)p.size;
-        const float r = 1.0f / sqrtf(row_sum<TPR>(squares, waves) / n + p.eps);
-        const float pull = r * r * (row_sum<TPR>(products, waves) / n);
+        row_sums<TPR>(squares, products, waves);
+        const float r = 1.0f / sqrtf(squares / n + p.eps);
+        const float pull = r * r * (products / n);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = 8 * (TPR * i + t);
             float dx[8];
             if (p.grad_sum != nullptr) {
-                load_chunk(dx, (const T *)p.grad_sum + at * p.grad_sum_ld, c, size);
+                load_chunk(dx, (const T *)p.grad_sum + now.at * p.grad_sum_ld, c, size);
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float own = r * (dy[i][e] * gamma[i][e] - x[i][e] * pull);
+                const float own = r * (now.dy[i][e] * gamma[i][e] - now.x[i][e] * pull);
                 dx[e] = p.grad_sum != nullptr ? dx[e] + own : own;
-                share[i][e] = there ? fmaf(dy[i][e] * x[i][e], r, share[i][e]) : share[i][e];
+                share[i][e] = now.there ? fmaf(now.dy[i][e] * now.x[i][e], r, share[i][e]) : share[i][e];
             }
             if (p.grad_x != nullptr) {
-                store_chunk(dx, (T *)p.grad_x + at * p.grad_x_ld, c, size);
+                store_chunk(dx, (T *)p.grad_x + now.at * p.grad_x_ld, c, size);
+            }
+        }
+        if (more) {
+            if constexpr (AHEAD) {
+                now = next;
+            } else {
+                load(now, first + step);
             }
         }
     }
@@ -239,25 +281,27 @@ __global__ __launch_bounds__(threads_of<TPR>()) void rms_norm_backward_kernel(co
     }
 }
 
-// dgamma from its shares: 32 columns a workgroup, 8 threads a column
-__global__ __launch_bounds__(256) void column_sums_kernel(const float *partial, float *out, int count, int size)
+// dgamma from its shares: 16 columns a workgroup, 64 threads a column
+__global__ __launch_bounds__(1024) void column_sums_kernel(const float *partial, float *out, int count, int size)
 {
-    __shared__ float part[8][32];
-    const int c = (int)threadIdx.x & 31, slice = (int)threadIdx.x >> 5, column = (int)blockIdx.x * 32 + c;
+    __shared__ float part[64][17];
+    const int c = (int)threadIdx.x & 15, slice = (int)threadIdx.x >> 4, column = (int)blockIdx.x * 16 + c;
     float sum = 0.f;
     if (column < size) {
-        for (int i = slice; i < count; i += 8) {
+#pragma unroll 8
+        for (int i = slice; i < count; i += 64) {
             sum += partial[(int64_t)i * size + column];
         }
     }
     part[slice][c] = sum;
     __syncthreads();
-    if (slice == 0 && column < size) {
-#pragma unroll
-        for (int s = 1; s < 8; ++s) {
-            sum += part[s][c];
+    if (threadIdx.x < 256) { // 16 threads a column now, each with four of the shares
+        const int col = (int)threadIdx.x >> 4, lane = (int)threadIdx.x & 15;
+        const float four = (part[lane][col] + part[lane + 16][col]) + (part[lane + 32][col] + part[lane + 48][col]);
+        const float all = group_sum<16>(four);
+        if (lane == 0 && (int)blockIdx.x * 16 + col < size) {
+            out[(int)blockIdx.x * 16 + col] = all;
         }
-        out[column] = sum;
     }
 }
 
@@ -351,7 +395,7 @@ int by_type(int32_t dtype, F f)
     return dtype == KUTACC_DTYPE_BF16 ? f(bf16_t{}) : f(float{});
 }
 
-// workgroups of the backward pass: as many as the chip holds twice over, each with its share of dgamma
+// workgroups of the backward pass, each with its share of dgamma
 int64_t backward_groups(int64_t rows, int64_t size)
 {
     int per_group = 1;
@@ -360,7 +404,7 @@ int64_t backward_groups(int64_t rows, int64_t size)
         return 0;
     });
     const int64_t needed = (rows + per_group - 1) / per_group;
-    return std::min<int64_t>(needed, 4 * (int64_t)kutacc_cu_count());
+    return std::min<int64_t>(needed, (size <= 1024 ? 8 : 2) * (int64_t)kutacc_cu_count());
 }
 } // namespace
 
@@ -403,7 +447,7 @@ int rms_norm_backward(const kutacc_hip_rms_norm_backward_args_t &a, hipStream_t 
         return rc;
     }
     kutacc_prof::KernelTimer t("column_sums_kernel", (double)groups * (double)a.size, stream);
-    column_sums_kernel<<<dim3((unsigned)((a.size + 31) / 32)), 256, 0, stream>>>(p.partial, a.grad_gamma, (int)groups, (int)a.size);
+    column_sums_kernel<<<dim3((unsigned)((a.size + 15) / 16)), 1024, 0, stream>>>(p.partial, a.grad_gamma, (int)groups, (int)a.size);
     return kutacc_hip_status(hipGetLastError());
 }
 
