@@ -57,6 +57,8 @@ struct TilesParams {
     int64_t c_ld[3];
     int M[3], N[3], tiles[3]; // of the products of WEIGHT_GRADIENTS, which have tiles of their own; else the first alone
     int K, activation;
+    int splits;   // of WEIGHT_GRADIENTS' rows, whose sums then meet in `shares`
+    float *shares;
 };
 
 constexpr int TILE = 128, OPERAND_SLOTS = 1024, CT_LD = 136;
@@ -210,13 +212,313 @@ __global__ __launch_bounds__(256, MODE == GATED || MODE == HIDDEN_GRADIENTS ? 1 
     }
 }
 
+// ---- whole 16-byte pieces: WM x WN waves a workgroup, 32 MI x 64 of the tile a wave: 256 x 256 by 2 x 4 waves or 128 x 128 by 2 x 2 ----
+//
+// Operands come straight into the LDS, 64 k a stage (A's rows, then B's; 128 bytes a row, its 16-byte slots XOR-ed with the row's number & 7),
+// two stages: a stage is asked for when the one before it has been read by all.  M-major operands (their tile's rows contiguous) lie in sub-tiles of
+// 64 k x 128 as mm_fragment expects them.  The last quarter of a stage's products runs behind the barrier at which the stage is given back and hides
+// the first reads of the next; in every quarter the fragments of the next one come out of the LDS between the products.
+//
+// A tile of GATED is SIDE rows of x by SIDE / 2 hidden units: of every 64 columns 32 are of the gate and 32 of the other projection, so that a wave
+// holds both of the same hidden units.  HIDDEN_GRADIENTS then multiplies dy with SIDE / 2 columns of down_w into sums of their own.
+template <int MODE, int MI, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void ff_pieces_kernel(const TilesParams p)
+{
+    constexpr int SIDE = 32 * MI * WM, HALF = WM * WN / 2, STAGE = 2 * SIDE * 8; // waves that bring an operand; 16-byte slots of a stage
+    static_assert(SIDE == 64 * WN && SIDE == 64 * HALF, "a wave brings eight units of 1 KB");
+    constexpr bool HIDDEN = MODE == GATED || MODE == HIDDEN_GRADIENTS, TWO = MODE == HIDDEN_GRADIENTS || MODE == INPUT_GRADIENT;
+    constexpr int COLUMNS = HIDDEN ? SIDE / 2 : SIDE;
+    constexpr bool A_MMAJOR = MODE == WEIGHT_GRADIENTS, B_MMAJOR = MODE == WEIGHT_GRADIENTS || MODE == INPUT_GRADIENT;
+    extern __shared__ uint4 lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 31, g = lane >> 5, wm = wave / WN, wn = wave % WN;
+
+    int which = 0, split = 0;
+    unsigned tile = blockIdx.x;
+    if constexpr (MODE == WEIGHT_GRADIENTS) {
+        const unsigned all = (unsigned)(p.tiles[0] + p.tiles[1] + p.tiles[2]);
+        split = (int)(tile / all), tile = tile % all;
+        while (which < 2 && tile >= (unsigned)p.tiles[which]) {
+            tile -= (unsigned)p.tiles[which++];
+        }
+    } else {
+        // Workgroup ids are dealt round robin over the 8 XCDs: each gets a contiguous run of the walk
+        const unsigned per = (unsigned)p.tiles[0] / 8;
+        tile = tile < per * 8 ? tile % 8 * per + tile / 8 : tile;
+    }
+    const int M = p.M[which], N = p.N[which];
+    // ... which goes through bands of 8 tiles of rows, column by column, so that neighbours share both operands in their L2
+    const unsigned MT = (unsigned)(M + SIDE - 1) / SIDE, NT = (unsigned)(N + COLUMNS - 1) / COLUMNS;
+    const unsigned band = tile / (8 * NT), height = min(8u, MT - 8 * band), in = tile - band * 8 * NT;
+    const int m0 = (int)(8 * band + in % height) * SIDE, n0 = (int)(in / height) * COLUMNS;
+
+    // stages of the first list of products (and of the second, as many)
+    const int all_stages = (p.K + 63) / 64;
+    int first_stage = 0, stages = all_stages;
+    if constexpr (MODE == WEIGHT_GRADIENTS) {
+        first_stage = (int)((int64_t)all_stages * split / p.splits), stages = (int)((int64_t)all_stages * (split + 1) / p.splits) - first_stage;
+    }
+    const int total = TWO ? 2 * stages : stages;
+    // Tiles of neighbouring columns start at different stages: with rows a power of two apart, all rows' bytes of one stage lie in one or two channels
+    // of the L2.
+    const int turn = MODE == WEIGHT_GRADIENTS ? 0 : (int)((unsigned)(n0 / COLUMNS) * 2u % (unsigned)stages);
+
+    const bool brings_a = wave < HALF;
+    const int w8 = 8 * (wave % HALF); // this wave's first unit of the operand
+    const uint32_t to = (uint32_t)(uintptr_t)(const lds_char *)lds + (brings_a ? 0u : SIDE * 128u) + (uint32_t)w8 * 1024u;
+    uint4 *const slots = lds + (brings_a ? 0 : SIDE * 8) + w8 * 64 + lane;
+    const int chunk = (lane & 7) ^ (lane >> 3);                 // K-major: eight rows a unit
+    const int mm_k = lane >> 4, mm_m = 8 * ((lane & 15) ^ (4 * (lane >> 4))); // M-major: four k by 128
+    // this lane's elements of the operand, from the tile's first
+    auto kmajor_from = [&](int row, int rows, int64_t ld) { return 2u * ((uint32_t)min(row, rows) * (uint32_t)ld + 8u * (uint32_t)chunk); };
+    auto mmajor_from = [&](int u, int rows, int64_t ld) { return 2u * ((uint32_t)(4 * (u & 15) + mm_k) * (uint32_t)ld + (uint32_t)max(0, min(128 * (u >> 4) + mm_m, rows))); };
+    uint32_t from[8], from_second[8];
+    const Product &q0 = p.product[which];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int u = w8 + i;
+        if (brings_a) {
+            from[i] = A_MMAJOR ? mmajor_from(u, M - m0 - 8, q0.a_ld) : kmajor_from(8 * u + (lane >> 3), M - m0 - 1, q0.a_ld);
+        } else if constexpr (B_MMAJOR) {
+            from[i] = mmajor_from(u, N - n0 - 8, q0.b_ld);
+        } else if constexpr (HIDDEN) { // units 0 .. 3 of eight the gate's 32 rows, 4 .. 7 the other projection's
+            from[i] = kmajor_from(32 * (w8 / 8) + 8 * (i & 3) + (lane >> 3), N - n0 - 1, q0.b_ld);
+        } else {
+            from[i] = kmajor_from(8 * u + (lane >> 3), N - n0 - 1, q0.b_ld);
+        }
+        if constexpr (MODE == HIDDEN_GRADIENTS) {
+            from_second[i] = brings_a ? kmajor_from(8 * u + (lane >> 3), M - m0 - 1, p.product[2].a_ld) : mmajor_from(u, N - n0 - 8, p.product[2].b_ld);
+        }
+    }
+    auto ask = [&](int t, int half) { // stage t of all
+        const bool second = TWO && t >= stages;
+        int s = (second ? t - stages : t) + turn;
+        s = (s >= stages ? s - stages : s) + first_stage;
+        const Product &q = p.product[MODE == HIDDEN_GRADIENTS ? (second ? 2 : 0) : MODE == INPUT_GRADIENT ? (second ? 1 : 0) : which];
+        const uint32_t stage = to + (uint32_t)half * (STAGE * 16u);
+        uint4 *const zeros = slots + half * STAGE;
+        const int left = p.K - 64 * s;
+        const bool b_second = MODE == HIDDEN_GRADIENTS && second && !brings_a;
+        if (brings_a ? A_MMAJOR : (B_MMAJOR || b_second)) {
+            const char *base = reinterpret_cast<const char *>(brings_a ? q.a + (int64_t)64 * s * q.a_ld + m0 : q.b + (int64_t)64 * s * q.b_ld + n0);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int u = w8 + i;
+                if (b_second && u >= 16) {
+                    continue; // SIDE / 2 columns, or 128 at least
+                }
+                if (4 * (u & 15) + mm_k < left) {
+                    load_to_lds(stage + i * 1024u, base, b_second ? from_second[i] : from[i]);
+                } else {
+                    zeros[i * 64] = zero_u4();
+                }
+            }
+        } else {
+            const bool there = 8 * chunk < left;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const bf16_t *operand = brings_a ? q.a + (int64_t)m0 * q.a_ld : (HIDDEN && i >= 4 ? p.product[1].b : q.b) + (int64_t)n0 * q.b_ld;
+                if (there) {
+                    load_to_lds(stage + i * 1024u, operand + 64 * s, MODE == HIDDEN_GRADIENTS && second ? from_second[i] : from[i]);
+                } else {
+                    zeros[i * 64] = zero_u4();
+                }
+            }
+        }
+    };
+
+    constexpr int SUMS = MODE == HIDDEN_GRADIENTS ? 3 : 2; // 32-wide column blocks of a wave
+    f32x16 acc[SUMS][MI];
+#pragma unroll
+    for (int j = 0; j < SUMS; ++j) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            acc[j][i] = zero16();
+        }
+    }
+    // where this lane points the transposing reads for the wave's blocks of an M-major operand
+    int a_mm[MI], b_mm[2], own_mm = mm_fragment_offset(wn & 3, lane);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+        a_mm[i] = ((MI * wm + i) >> 2) * 16384 + mm_fragment_offset((MI * wm + i) & 3, lane);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        b_mm[j] = ((2 * wn + j) >> 2) * 16384 + mm_fragment_offset((2 * wn + j) & 3, lane);
+    }
+    const int odd = r & 7;
+    auto kmajor_fragment = [&](const uint4 *operand, int block, int s) { return as_bf16x8(operand[(32 * block + r) * 8 + ((2 * s + g) ^ odd)]); };
+    int t = 0; // the current stage, of all
+    auto run = [&](auto is_second) {
+        constexpr bool SECOND = decltype(is_second)::value;
+        constexpr bool OWN = SECOND && MODE == HIDDEN_GRADIENTS; // sums of its own, one block of columns
+        constexpr int NB = OWN ? 1 : 2;
+        bf16x8 a[2][MI], b[2][NB];
+        auto fetch = [&](int set, const uint4 *stage, int s, int n) { // fragment n of a quarter's MI + NB
+            const uint4 *columns = stage + SIDE * 8;
+            if (n < NB) {
+                if constexpr (OWN) {
+                    b[set][n] = mm_fragment((const lds_char *)columns, own_mm, s);
+                } else if constexpr (B_MMAJOR) {
+                    b[set][n] = mm_fragment((const lds_char *)columns, b_mm[n], s);
+                } else {
+                    b[set][n] = kmajor_fragment(columns, 2 * wn + n, s);
+                }
+            } else if constexpr (A_MMAJOR) {
+                a[set][n - NB] = mm_fragment((const lds_char *)stage, a_mm[n - NB], s);
+            } else {
+                a[set][n - NB] = kmajor_fragment(stage, MI * wm + n - NB, s);
+            }
+        };
+#pragma unroll
+        for (int n = 0; n < MI + NB; ++n) {
+            fetch(0, lds + (t & 1) * STAGE, 0, n);
+        }
+        for (const int end = t + stages; t < end; ++t) {
+            const uint4 *stage = lds + (t & 1) * STAGE, *other = lds + ((t + 1) & 1) * STAGE;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                if (s == 3) { // the next stage is there, and all have read this one; behind the last one what is read is not used
+                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                    if (t + 2 < total) {
+                        ask(t + 2, t & 1);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int n = 0; n < MI * NB; ++n) {
+                    const int i = n / NB, j = n % NB;
+                    f32x16 &sum = acc[OWN ? 2 : j][i];
+                    sum = mfma(b[s & 1][j], a[s & 1][i], sum);
+                    asm volatile("" : "+a"(sum));
+                    // the next quarter's fragments, one or two beside a product
+                    constexpr int TOTAL = MI + NB, STEPS = MI * NB;
+#pragma unroll
+                    for (int f = n * TOTAL / STEPS; f < (n + 1) * TOTAL / STEPS; ++f) {
+                        fetch((s + 1) & 1, s == 3 ? other : stage, (s + 1) & 3, f);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        }
+    };
+    ask(0, 0);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (total > 1) {
+        ask(1, 1);
+    }
+    run(std::false_type{});
+    if constexpr (TWO) {
+        run(std::true_type{});
+    }
+
+    if constexpr (MODE == WEIGHT_GRADIENTS) {
+        if (p.splits > 1) { // a share of the sums, lane by lane: [split][tile of all three][wave][MI][2][4][64] of 16 bytes
+            f32x4 *share = reinterpret_cast<f32x4 *>(p.shares) + ((int64_t)blockIdx.x * (WM * WN) + wave) * (MI * 2 * 4 * 64) + lane;
+#pragma unroll
+            for (int i = 0; i < MI; ++i) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        share[((i * 2 + j) * 4 + e) * 64] = f32x4{acc[j][i][4 * e], acc[j][i][4 * e + 1], acc[j][i][4 * e + 2], acc[j][i][4 * e + 3]};
+                    }
+                }
+            }
+            return;
+        }
+    }
+    // results as bf16 through a strip of the LDS of the wave's own, 32 rows by WIDTH columns, out in whole runs of WIDTH
+    constexpr int WIDTH = HIDDEN ? 32 : 64, STRIP_LD = WIDTH + 8;
+    static_assert(WM * WN * 32 * STRIP_LD * 2 <= 2 * STAGE * 16, "the strips lie where the operands were");
+    __syncthreads(); // what the other waves have read ahead lies there
+    bf16_t *strip = reinterpret_cast<bf16_t *>(lds) + wave * 32 * STRIP_LD;
+    auto store = [&](bf16_t *c, int64_t ld, int i, auto value) {
+#pragma unroll
+        for (int j = 0; j < WIDTH / 32; ++j) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                bf16x4 o;
+#pragma unroll
+                for (int f = 0; f < 4; ++f) {
+                    o[f] = (bf16_t)value(j, 4 * e + f);
+                }
+                *reinterpret_cast<bf16x4 *>(strip + r * STRIP_LD + 32 * j + 8 * e + 4 * g) = o;
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int e = 0; e < WIDTH / 16; ++e) {
+            const int piece = lane + 64 * e, row = piece / (WIDTH / 8), part = piece % (WIDTH / 8);
+            const int m = m0 + 32 * (MI * wm + i) + row, n = n0 + WIDTH * wn + 8 * part;
+            if (m < M && n < N) {
+                *reinterpret_cast<uint4 *>(c + (int64_t)m * ld + n) = *reinterpret_cast<const uint4 *>(strip + row * STRIP_LD + 8 * part);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    };
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+        if constexpr (HIDDEN) {
+            f32x16 h, dg, du;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                float slope = 0.f;
+                const float act = activate<MODE == HIDDEN_GRADIENTS>(acc[0][i][e], p.activation, slope), u = acc[1][i][e];
+                h[e] = act * u;
+                if constexpr (MODE == HIDDEN_GRADIENTS) {
+                    dg[e] = acc[2][i][e] * u * slope;
+                    du[e] = acc[2][i][e] * act;
+                }
+            }
+            store(p.c[0], p.c_ld[0], i, [&](int, int e) { return h[e]; });
+            if constexpr (MODE == HIDDEN_GRADIENTS) {
+                store(p.c[1], p.c_ld[1], i, [&](int, int e) { return dg[e]; });
+                store(p.c[2], p.c_ld[2], i, [&](int, int e) { return du[e]; });
+            }
+        } else {
+            store(p.c[which], p.c_ld[which], i, [&](int j, int e) { return acc[j][i][e]; });
+        }
+    }
+}
+
+// The weights' gradients from their shares: a thread adds four columns of a row over the splits, in one order.
+template <int MI, int WM, int WN>
+__global__ __launch_bounds__(256) void ff_shares_kernel(const TilesParams p)
+{
+    constexpr int SIDE = 32 * MI * WM, PER_TILE = WM * WN * MI * 2 * 4 * 64;
+    const unsigned all = (unsigned)(p.tiles[0] + p.tiles[1] + p.tiles[2]);
+    const int64_t index = (int64_t)blockIdx.x * 256 + threadIdx.x, pitch = (int64_t)all * PER_TILE;
+    const f32x4 *share = reinterpret_cast<const f32x4 *>(p.shares) + index;
+    f32x4 sum = share[0];
+#pragma unroll 8
+    for (int s = 1; s < p.splits; ++s) {
+        sum += share[s * pitch];
+    }
+    unsigned tile = (unsigned)(index / PER_TILE);
+    const int in = (int)(index % PER_TILE), lane = in & 63, e = (in >> 6) & 3, j = (in >> 8) & 1, i = (in >> 9) % MI, wave = in / (512 * MI);
+    int which = 0;
+    while (which < 2 && tile >= (unsigned)p.tiles[which]) {
+        tile -= (unsigned)p.tiles[which++];
+    }
+    const int M = p.M[which], N = p.N[which];
+    const unsigned MT = (unsigned)(M + SIDE - 1) / SIDE, NT = (unsigned)(N + SIDE - 1) / SIDE;
+    const unsigned band = tile / (8 * NT), height = min(8u, MT - 8 * band), of = tile - band * 8 * NT;
+    const int m = (int)(8 * band + of % height) * SIDE + 32 * (MI * (wave / WN) + i) + (lane & 31);
+    const int n = (int)(of / height) * SIDE + 64 * (wave % WN) + 32 * j + 8 * e + 4 * (lane >> 5);
+    if (m < M && n < N) {
+        const bf16x4 o = {(bf16_t)sum[0], (bf16_t)sum[1], (bf16_t)sum[2], (bf16_t)sum[3]};
+        *reinterpret_cast<bf16x4 *>(p.c[which] + (int64_t)m * p.c_ld[which] + n) = o;
+    }
+}
+
 // Whether a product's operands fill whole 16-byte pieces: pointers, pitches, and the extents along which rows are contiguous
-bool pieces(const void *ptr, int64_t ld, int64_t contiguous) { return kutacc_hip_aligned16(ptr) && ld % 8 == 0 && contiguous % 8 == 0; }
+bool pieces(const void *ptr, int64_t ld, int64_t contiguous) { return kutacc_hip_aligned16(ptr) && ld % 8 == 0 && contiguous % 8 == 0 && ld < (1 << 23); }
 
 int64_t tiles_of(int64_t m, int64_t n) { return (m + TILE - 1) / TILE * ((n + TILE - 1) / TILE); }
 
 template <int MODE>
-int launch_tiles(TilesParams p, bool any, double flops, const char *name, hipStream_t stream)
+int launch_any(TilesParams p, bool any, double flops, const char *name, hipStream_t stream)
 {
     static size_t configured[2][KUTACC_DEVICE_SLOTS] = {};
     int64_t blocks = 0;
@@ -237,6 +539,80 @@ int launch_tiles(TilesParams p, bool any, double flops, const char *name, hipStr
     return kutacc_hip_status(hipGetLastError());
 }
 
+// tiles of SIDE rows by `columns`, of all products; p.tiles filled in
+int64_t count_tiles(TilesParams &p, int side, int columns)
+{
+    int64_t all = 0;
+    for (int i = 0; i < 3; ++i) {
+        const int64_t tiles = ((int64_t)p.M[i] + side - 1) / side * (((int64_t)p.N[i] + columns - 1) / columns);
+        p.tiles[i] = (int)std::min<int64_t>(tiles, INT32_MAX);
+        all += tiles;
+    }
+    return all;
+}
+
+template <int MODE, int MI, int WM, int WN>
+int launch_pieces(TilesParams p, hipStream_t stream)
+{
+    constexpr int SIDE = 32 * MI * WM;
+    static size_t configured[KUTACC_DEVICE_SLOTS] = {};
+    const auto kernel = &ff_pieces_kernel<MODE, MI, WM, WN>;
+    const int64_t tiles = count_tiles(p, SIDE, MODE == GATED || MODE == HIDDEN_GRADIENTS ? SIDE / 2 : SIDE), groups = tiles * p.splits;
+    if (groups > INT32_MAX) {
+        return KUTACC_HIP_EUNSUPPORTED;
+    }
+    if (const hipError_t e = kutacc_opt_in_lds(reinterpret_cast<const void *>(kernel), 2 * 2 * SIDE * 128, configured)) {
+        return kutacc_hip_status(e);
+    }
+    kernel<<<dim3((unsigned)groups), 64 * WM * WN, 2 * 2 * SIDE * 128, stream>>>(p);
+    if (MODE == WEIGHT_GRADIENTS && p.splits > 1) {
+        ff_shares_kernel<MI, WM, WN><<<dim3((unsigned)(tiles * WM * WN * MI * 2)), 256, 0, stream>>>(p);
+    }
+    return kutacc_hip_status(hipGetLastError());
+}
+
+bool enough_large(TilesParams p, int columns) { return 4 * count_tiles(p, 256, columns) >= 3 * kutacc_cu_count(); }
+
+template <int MODE>
+int launch_tiles(const TilesParams &p, bool any, double flops, const char *name, hipStream_t stream)
+{
+    if (any) {
+        return launch_any<MODE>(p, true, flops, name, stream);
+    }
+    kutacc_prof::KernelTimer t(name, flops, stream);
+    if constexpr (MODE != HIDDEN_GRADIENTS) {
+        if (enough_large(p, MODE == GATED ? 128 : 256)) {
+            return launch_pieces<MODE, 4, 2, 4>(p, stream);
+        }
+    }
+    return launch_pieces<MODE, 2, 2, 2>(p, stream);
+}
+
+// How many ways the rows are split for the weights' gradients: 128 x 128 tiles of fewer than two workgroups a CU, into ranges of at least eight stages
+int weight_splits(int64_t rows, int64_t c_o, int64_t c_i)
+{
+    TilesParams p = {};
+    p.M[0] = p.M[1] = (int)c_i, p.N[0] = p.N[1] = (int)c_o, p.M[2] = (int)c_o, p.N[2] = (int)c_i;
+    if (enough_large(p, 256)) {
+        return 1;
+    }
+    const int64_t tiles = count_tiles(p, 128, 128), stages = (rows + 63) / 64;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(2 * kutacc_cu_count() / tiles, stages / 8));
+}
+int launch_weight_gradients(const TilesParams &p, bool any, double flops, const char *name, hipStream_t stream)
+{
+    if (any) {
+        return launch_any<WEIGHT_GRADIENTS>(p, true, flops, name, stream);
+    }
+    kutacc_prof::KernelTimer t(name, flops, stream);
+    return p.splits == 1 && enough_large(p, 256) ? launch_pieces<WEIGHT_GRADIENTS, 4, 2, 4>(p, stream) : launch_pieces<WEIGHT_GRADIENTS, 2, 2, 2>(p, stream);
+}
+int64_t shares_bytes(int64_t rows, int64_t c_o, int64_t c_i)
+{
+    const int64_t splits = weight_splits(rows, c_o, c_i);
+    return splits == 1 ? 0 : splits * ((c_i + 127) / 128) * ((c_o + 127) / 128) * 3 * 128 * 128 * 4;
+}
+
 int64_t padded(int64_t v) { return (v + 31) / 32 * 32; }
 int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 } // namespace
@@ -250,22 +626,25 @@ int gated_transition(const kutacc_hip_gated_transition_args_t &a, hipStream_t st
     const int64_t rows = a.rows, c_o = a.c_o, c_i = a.c_i, h_ld = padded(c_i);
     bf16_t *h = (bf16_t *)a.workspace;
     TilesParams p = {};
+    p.splits = 1;
     p.product[0] = {(const bf16_t *)a.x, (const bf16_t *)a.gate_w, a.x_ld, c_o};
     p.product[1] = {(const bf16_t *)a.x, (const bf16_t *)a.up_w, a.x_ld, c_o};
     p.c[0] = h, p.c_ld[0] = h_ld;
     p.M[0] = (int)rows, p.N[0] = (int)c_i, p.K = (int)c_o, p.activation = a.activation;
-    const bool any_in = !pieces(a.x, a.x_ld, c_o) || !kutacc_hip_aligned16(a.gate_w) || !kutacc_hip_aligned16(a.up_w);
+    const bool widths = c_o % 8 == 0 && c_i % 8 == 0;
+    const bool any_in = !widths || !pieces(a.x, a.x_ld, c_o) || !kutacc_hip_aligned16(a.gate_w) || !kutacc_hip_aligned16(a.up_w);
     if (const int rc = launch_tiles<GATED>(p, any_in, 4.0 * (double)rows * (double)c_o * (double)c_i, "ff_tiles_kernel<gated>", stream)) {
         return rc;
     }
     TilesParams d = {};
+    d.splits = 1;
     d.product[0] = {h, (const bf16_t *)a.down_w, h_ld, c_i};
     d.c[0] = (bf16_t *)a.out, d.c_ld[0] = a.out_ld;
     d.M[0] = (int)rows, d.N[0] = (int)c_o, d.K = (int)c_i;
-    return launch_tiles<PLAIN>(d, !pieces(a.down_w, c_i, c_i), 2.0 * (double)rows * (double)c_o * (double)c_i, "ff_tiles_kernel<plain>", stream);
+    return launch_tiles<PLAIN>(d, !widths || !kutacc_hip_aligned16(a.down_w) || !pieces(a.out, a.out_ld, c_o), 2.0 * (double)rows * (double)c_o * (double)c_i, "ff_tiles_kernel<plain>", stream);
 }
 
-int64_t gated_transition_backward_workspace(int64_t rows, int64_t c_o, int64_t c_i) { return 3 * align256(2 * rows * padded(c_i)); }
+int64_t gated_transition_backward_workspace(int64_t rows, int64_t c_o, int64_t c_i) { return 3 * align256(2 * rows * padded(c_i)) + shares_bytes(rows, c_o, c_i); }
 
 int gated_transition_backward(const kutacc_hip_gated_transition_backward_args_t &a, hipStream_t stream)
 {
@@ -274,23 +653,26 @@ int gated_transition_backward(const kutacc_hip_gated_transition_backward_args_t 
     const bf16_t *x = (const bf16_t *)a.x, *dy = (const bf16_t *)a.grad_out;
     const bf16_t *wg = (const bf16_t *)a.gate_w, *wu = (const bf16_t *)a.up_w, *wd = (const bf16_t *)a.down_w;
     const double flops = 2.0 * (double)rows * (double)c_o * (double)c_i;
-    const bool rows_fit = pieces(x, a.x_ld, c_o) && pieces(dy, a.grad_out_ld, c_o), weights_fit = kutacc_hip_aligned16(wg) && kutacc_hip_aligned16(wu) && c_o % 8 == 0;
+    const bool rows_fit = pieces(x, a.x_ld, c_o) && pieces(dy, a.grad_out_ld, c_o), widths = c_o % 8 == 0 && c_i % 8 == 0;
+    const bool weights_fit = widths && kutacc_hip_aligned16(wg) && kutacc_hip_aligned16(wu);
     TilesParams p = {};
+    p.splits = 1;
     p.product[0] = {x, wg, a.x_ld, c_o};
     p.product[1] = {x, wu, a.x_ld, c_o};
     p.product[2] = {dy, wd, a.grad_out_ld, c_i};
     p.c[0] = h, p.c[1] = dg, p.c[2] = du, p.c_ld[0] = p.c_ld[1] = p.c_ld[2] = ld;
     p.M[0] = (int)rows, p.N[0] = (int)c_i, p.K = (int)c_o, p.activation = a.activation;
-    if (const int rc = launch_tiles<HIDDEN_GRADIENTS>(p, !rows_fit || !weights_fit || !pieces(wd, c_i, c_i), 3 * flops, "ff_tiles_kernel<hidden gradients>", stream)) {
+    if (const int rc = launch_tiles<HIDDEN_GRADIENTS>(p, !rows_fit || !weights_fit || !kutacc_hip_aligned16(wd), 3 * flops, "ff_tiles_kernel<hidden gradients>", stream)) {
         return rc;
     }
     if (a.grad_x != nullptr) {
         TilesParams d = {};
+    d.splits = 1;
         d.product[0] = {dg, wg, ld, c_o};
         d.product[1] = {du, wu, ld, c_o};
         d.c[0] = (bf16_t *)a.grad_x, d.c_ld[0] = a.grad_x_ld;
         d.M[0] = (int)rows, d.N[0] = (int)c_o, d.K = (int)c_i;
-        if (const int rc = launch_tiles<INPUT_GRADIENT>(d, !weights_fit || c_i % 8 != 0, 2 * flops, "ff_tiles_kernel<input gradient>", stream)) {
+        if (const int rc = launch_tiles<INPUT_GRADIENT>(d, !weights_fit || !pieces(a.grad_x, a.grad_x_ld, c_o), 2 * flops, "ff_tiles_kernel<input gradient>", stream)) {
             return rc;
         }
     }
@@ -307,7 +689,10 @@ int gated_transition_backward(const kutacc_hip_gated_transition_backward_args_t 
     add({dg, x, ld, a.x_ld}, a.grad_gate_w, c_i, c_o);
     add({du, x, ld, a.x_ld}, a.grad_up_w, c_i, c_o);
     add({dy, h, a.grad_out_ld, ld}, a.grad_down_w, c_o, c_i);
-    return count == 0 ? 0 : launch_tiles<WEIGHT_GRADIENTS>(w, !rows_fit || c_i % 8 != 0, count * flops, "ff_tiles_kernel<weight gradients>", stream);
+    const bool aligned = (!a.grad_gate_w || kutacc_hip_aligned16(a.grad_gate_w)) && (!a.grad_up_w || kutacc_hip_aligned16(a.grad_up_w)) && (!a.grad_down_w || kutacc_hip_aligned16(a.grad_down_w));
+    w.splits = weight_splits(rows, c_o, c_i);
+    w.shares = reinterpret_cast<float *>(du + each);
+    return count == 0 ? 0 : launch_weight_gradients(w, !rows_fit || !widths || !aligned, count * flops, "ff_tiles_kernel<weight gradients>", stream);
 }
 
 } // namespace kutacc_launch

@@ -175,15 +175,24 @@ __global__ __launch_bounds__(threads_of<TPR>()) void rms_norm_backward_kernel(co
     __shared__ float waves[THREADS / 32];
     __shared__ float shares[ROWS > 1 ? THREADS * 8 : 1];
     const int t = (int)threadIdx.x % TPR, group = (int)threadIdx.x / TPR;
+    constexpr bool AHEAD = TPR * NV < 2048; // beyond, a thread has no registers for two rows, nor for gamma
     float gamma[NV][8], share[NV][8];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
+    auto load_gamma = [&](float (&to)[8], int i) {
         if (p.gamma != nullptr) {
-            load_chunk(gamma[i], p.gamma, 8 * (TPR * i + t), p.size);
+            load_chunk(to, p.gamma, 8 * (TPR * i + t), p.size);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            gamma[i][e] = p.gamma != nullptr ? gamma[i][e] : 1.f;
+            to[e] = p.gamma != nullptr ? to[e] : 1.f;
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if constexpr (AHEAD) {
+            load_gamma(gamma[i], i);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
             share[i][e] = 0.f;
         }
     }
@@ -207,21 +216,28 @@ __global__ __launch_bounds__(threads_of<TPR>()) void rms_norm_backward_kernel(co
     };
     const int64_t step = (int64_t)gridDim.x * ROWS;
     int64_t first = (int64_t)blockIdx.x * ROWS;
-    constexpr bool AHEAD = TPR * NV < 2048; // beyond, two rows have no registers
-    load(now, first);
+    if constexpr (AHEAD) {
+        load(now, first);
+    }
     for (; first < p.rows; first += step) {
         const bool more = first + step < p.rows;
-        if (AHEAD && more) {
+        if constexpr (!AHEAD) {
+            load(now, first);
+        } else if (more) {
             load(next, first + step); // on its way while this one is reduced and written
         }
         const int size = now.there ? p.size : 0;
         float squares = 0.f, products = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
+            if constexpr (!AHEAD) {
+                load_gamma(gamma[0], i);
+            }
+            constexpr int KEPT = AHEAD ? 1 : 0;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 squares = fmaf(now.x[i][e], now.x[i][e], squares);
-                products = fmaf(now.dy[i][e] * gamma[i][e], now.x[i][e], products);
+                products = fmaf(now.dy[i][e] * gamma[KEPT * i][e], now.x[i][e], products);
             }
         }
         const float n = (float)p.size;
@@ -232,12 +248,16 @@ __global__ __launch_bounds__(threads_of<TPR>()) void rms_norm_backward_kernel(co
         for (int i = 0; i < NV; ++i) {
             const int c = 8 * (TPR * i + t);
             float dx[8];
+            if constexpr (!AHEAD) {
+                load_gamma(gamma[0], i);
+            }
+            constexpr int KEPT = AHEAD ? 1 : 0;
             if (p.grad_sum != nullptr) {
                 load_chunk(dx, (const T *)p.grad_sum + now.at * p.grad_sum_ld, c, size);
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float own = r * (now.dy[i][e] * gamma[i][e] - now.x[i][e] * pull);
+                const float own = r * (now.dy[i][e] * gamma[KEPT * i][e] - now.x[i][e] * pull);
                 dx[e] = p.grad_sum != nullptr ? dx[e] + own : own;
                 share[i][e] = now.there ? fmaf(now.dy[i][e] * now.x[i][e], r, share[i][e]) : share[i][e];
             }
@@ -245,12 +265,8 @@ __global__ __launch_bounds__(threads_of<TPR>()) void rms_norm_backward_kernel(co
                 store_chunk(dx, (T *)p.grad_x + now.at * p.grad_x_ld, c, size);
             }
         }
-        if (more) {
-            if constexpr (AHEAD) {
-                now = next;
-            } else {
-                load(now, first + step);
-            }
+        if (AHEAD && more) {
+            now = next;
         }
     }
     if (p.partial == nullptr) {
