@@ -212,6 +212,13 @@ __global__ __launch_bounds__(256, MODE == GATED || MODE == HIDDEN_GRADIENTS ? 1 
     }
 }
 
+// a pointer that is the same in all lanes, in scalar registers
+__device__ __forceinline__ const void *same_in_all_lanes(const void *p)
+{
+    const uint64_t v = (uint64_t)p;
+    return (const void *)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v) | (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32)) << 32);
+}
+
 // ---- whole 16-byte pieces: WM x WN waves a workgroup, 32 MI x 64 of the tile a wave: 256 x 256 by 2 x 4 waves or 128 x 128 by 2 x 2 ----
 //
 // Operands come straight into the LDS, 64 k a stage (A's rows, then B's; 128 bytes a row, its 16-byte slots XOR-ed with the row's number & 7),
@@ -221,110 +228,138 @@ __global__ __launch_bounds__(256, MODE == GATED || MODE == HIDDEN_GRADIENTS ? 1 
 //
 // A tile of GATED is SIDE rows of x by SIDE / 2 hidden units: of every 64 columns 32 are of the gate and 32 of the other projection, so that a wave
 // holds both of the same hidden units.  HIDDEN_GRADIENTS then multiplies dy with SIDE / 2 columns of down_w into sums of their own.
-template <int MODE, int MI, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN, 2) void ff_pieces_kernel(const TilesParams p)
+template <int MODE, int MI, int WM, int WN, int GROUPS>
+__global__ __launch_bounds__(64 * WM * WN * GROUPS, 2) void ff_pieces_kernel(const TilesParams p)
 {
-    constexpr int SIDE = 32 * MI * WM, HALF = WM * WN / 2, STAGE = 2 * SIDE * 8; // waves that bring an operand; 16-byte slots of a stage
-    static_assert(SIDE == 64 * WN && SIDE == 64 * HALF, "a wave brings eight units of 1 KB");
+    constexpr int ROWS = 32 * MI * WM, SIDE = 64 * WN, STAGE = (ROWS + SIDE) * 8; // of A and B; 16-byte slots of a stage
+    constexpr int A_UNITS = ROWS / 8, UNITS = (ROWS + SIDE) / 8 / (WM * WN);      // of 1 KB: of A, and those that a wave brings
+    static_assert((ROWS + SIDE) % (8 * WM * WN) == 0, "all waves bring as much");
     constexpr bool HIDDEN = MODE == GATED || MODE == HIDDEN_GRADIENTS, TWO = MODE == HIDDEN_GRADIENTS || MODE == INPUT_GRADIENT;
     constexpr int COLUMNS = HIDDEN ? SIDE / 2 : SIDE;
     constexpr bool A_MMAJOR = MODE == WEIGHT_GRADIENTS, B_MMAJOR = MODE == WEIGHT_GRADIENTS || MODE == INPUT_GRADIENT;
-    extern __shared__ uint4 lds[];
+    static_assert(!A_MMAJOR || ROWS % 128 == 0, "sub-tiles of M-major operands");
+    static_assert(GROUPS == 1 || MODE == PLAIN || MODE == INPUT_GRADIENT, "sums that meet in the LDS");
+    extern __shared__ uint4 all_lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int r = lane & 31, g = lane >> 5, wm = wave / WN, wn = wave % WN;
+    const int group = wave / (WM * WN), member = wave % (WM * WN);
+    const int r = lane & 31, g = lane >> 5, wm = member / WN, wn = member % WN;
+    uint4 *const lds = all_lds + group * 2 * STAGE;
 
-    int which = 0, split = 0;
+    // Workgroup ids are dealt round robin over the 8 XCDs: each gets a contiguous run of the walk
     unsigned tile = blockIdx.x;
-    if constexpr (MODE == WEIGHT_GRADIENTS) {
+    {
+        const unsigned per = gridDim.x / 8;
+        tile = tile < per * 8 ? tile % 8 * per + tile / 8 : tile;
+    }
+    int which = 0, split = 0;
+    const unsigned place = tile; // of a share of the sums
+    if constexpr (MODE == WEIGHT_GRADIENTS) { // (all tiles of a range of rows, which share them, and then the next range's)
         const unsigned all = (unsigned)(p.tiles[0] + p.tiles[1] + p.tiles[2]);
-        split = (int)(tile / all), tile = tile % all;
+        split = __builtin_amdgcn_readfirstlane((int)(tile / all)), tile = (unsigned)__builtin_amdgcn_readfirstlane((int)(tile % all));
         while (which < 2 && tile >= (unsigned)p.tiles[which]) {
             tile -= (unsigned)p.tiles[which++];
         }
-    } else {
-        // Workgroup ids are dealt round robin over the 8 XCDs: each gets a contiguous run of the walk
-        const unsigned per = (unsigned)p.tiles[0] / 8;
-        tile = tile < per * 8 ? tile % 8 * per + tile / 8 : tile;
     }
     const int M = p.M[which], N = p.N[which];
-    // ... which goes through bands of 8 tiles of rows, column by column, so that neighbours share both operands in their L2
-    const unsigned MT = (unsigned)(M + SIDE - 1) / SIDE, NT = (unsigned)(N + COLUMNS - 1) / COLUMNS;
+    // ... a walk through bands of 8 tiles of rows, column by column, so that neighbours share both operands in their L2
+    const unsigned MT = (unsigned)(M + ROWS - 1) / ROWS, NT = (unsigned)(N + COLUMNS - 1) / COLUMNS;
     const unsigned band = tile / (8 * NT), height = min(8u, MT - 8 * band), in = tile - band * 8 * NT;
-    const int m0 = (int)(8 * band + in % height) * SIDE, n0 = (int)(in / height) * COLUMNS;
+    // (quotients come from vector instructions: back into scalar registers, for the addresses)
+    const int m0 = __builtin_amdgcn_readfirstlane((int)(8 * band + in % height) * ROWS), n0 = __builtin_amdgcn_readfirstlane((int)(in / height) * COLUMNS);
 
     // stages of the first list of products (and of the second, as many)
     const int all_stages = (p.K + 63) / 64;
     int first_stage = 0, stages = all_stages;
     if constexpr (MODE == WEIGHT_GRADIENTS) {
-        first_stage = (int)((int64_t)all_stages * split / p.splits), stages = (int)((int64_t)all_stages * (split + 1) / p.splits) - first_stage;
+        first_stage = __builtin_amdgcn_readfirstlane((int)((int64_t)all_stages * split / p.splits));
+        stages = __builtin_amdgcn_readfirstlane((int)((int64_t)all_stages * (split + 1) / p.splits)) - first_stage;
     }
-    const int total = TWO ? 2 * stages : stages;
+    // of the stages a group takes every other one; a group that has one less multiplies zeros
+    const int steps = (stages + GROUPS - 1) / GROUPS, total = TWO ? 2 * steps : steps;
     // Tiles of neighbouring columns start at different stages: with rows a power of two apart, all rows' bytes of one stage lie in one or two channels
     // of the L2.
-    const int turn = MODE == WEIGHT_GRADIENTS ? 0 : (int)((unsigned)(n0 / COLUMNS) * 2u % (unsigned)stages);
+    const int turn = MODE == WEIGHT_GRADIENTS ? 0 : __builtin_amdgcn_readfirstlane((int)((unsigned)(n0 / COLUMNS) * 2u % (unsigned)stages));
 
-    const bool brings_a = wave < HALF;
-    const int w8 = 8 * (wave % HALF); // this wave's first unit of the operand
-    const uint32_t to = (uint32_t)(uintptr_t)(const lds_char *)lds + (brings_a ? 0u : SIDE * 128u) + (uint32_t)w8 * 1024u;
-    uint4 *const slots = lds + (brings_a ? 0 : SIDE * 8) + w8 * 64 + lane;
-    const int chunk = (lane & 7) ^ (lane >> 3);                 // K-major: eight rows a unit
+    const int first_unit = member * UNITS; // this wave's, of A's and then B's
+    const uint32_t to = (uint32_t)(uintptr_t)(const lds_char *)lds + (uint32_t)first_unit * 1024u;
+    uint4 *const slots = lds + first_unit * 64 + lane;
+    const int chunk = (lane & 7) ^ (lane >> 3);                               // K-major: eight rows a unit
     const int mm_k = lane >> 4, mm_m = 8 * ((lane & 15) ^ (4 * (lane >> 4))); // M-major: four k by 128
     // this lane's elements of the operand, from the tile's first
-    auto kmajor_from = [&](int row, int rows, int64_t ld) { return 2u * ((uint32_t)min(row, rows) * (uint32_t)ld + 8u * (uint32_t)chunk); };
-    auto mmajor_from = [&](int u, int rows, int64_t ld) { return 2u * ((uint32_t)(4 * (u & 15) + mm_k) * (uint32_t)ld + (uint32_t)max(0, min(128 * (u >> 4) + mm_m, rows))); };
-    uint32_t from[8], from_second[8];
+    auto kmajor_from = [&](int row, int last, int64_t ld) { return 2u * ((uint32_t)min(row, last) * (uint32_t)ld + 8u * (uint32_t)chunk); };
+    auto mmajor_from = [&](int u, int last, int64_t ld) { return 2u * ((uint32_t)(4 * (u & 15) + mm_k) * (uint32_t)ld + (uint32_t)max(0, min(128 * (u >> 4) + mm_m, last))); };
+    uint32_t from[UNITS], from_second[MODE == HIDDEN_GRADIENTS ? UNITS : 1];
     const Product &q0 = p.product[which];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int u = w8 + i;
-        if (brings_a) {
+    for (int i = 0; i < UNITS; ++i) {
+        const bool is_a = first_unit + i < A_UNITS;
+        const int u = is_a ? first_unit + i : first_unit + i - A_UNITS;
+        if (is_a) {
             from[i] = A_MMAJOR ? mmajor_from(u, M - m0 - 8, q0.a_ld) : kmajor_from(8 * u + (lane >> 3), M - m0 - 1, q0.a_ld);
         } else if constexpr (B_MMAJOR) {
             from[i] = mmajor_from(u, N - n0 - 8, q0.b_ld);
-        } else if constexpr (HIDDEN) { // units 0 .. 3 of eight the gate's 32 rows, 4 .. 7 the other projection's
-            from[i] = kmajor_from(32 * (w8 / 8) + 8 * (i & 3) + (lane >> 3), N - n0 - 1, q0.b_ld);
+        } else if constexpr (HIDDEN) { // of eight units 0 .. 3 the gate's 32 rows, 4 .. 7 the other projection's
+            from[i] = kmajor_from(32 * (u >> 3) + 8 * (u & 3) + (lane >> 3), N - n0 - 1, q0.b_ld);
         } else {
             from[i] = kmajor_from(8 * u + (lane >> 3), N - n0 - 1, q0.b_ld);
         }
         if constexpr (MODE == HIDDEN_GRADIENTS) {
-            from_second[i] = brings_a ? kmajor_from(8 * u + (lane >> 3), M - m0 - 1, p.product[2].a_ld) : mmajor_from(u, N - n0 - 8, p.product[2].b_ld);
+            from_second[i] = is_a ? kmajor_from(8 * u + (lane >> 3), M - m0 - 1, p.product[2].a_ld) : mmajor_from(u, N - n0 - 8, p.product[2].b_ld);
         }
     }
-    auto ask = [&](int t, int half) { // stage t of all
-        const bool second = TWO && t >= stages;
-        int s = (second ? t - stages : t) + turn;
+    // what this wave asks for at step t of all: where its units start, and how much of k is left there
+    struct Stage {
+        uint64_t a, b, up; // addresses
+        uint32_t to;
+        int half, left;
+        bool own; // the second products of HIDDEN_GRADIENTS
+    };
+    auto stage_of = [&](int t, int half) {
+        const bool second = TWO && t >= steps;
+        const int in_order = (second ? t - steps : t) * GROUPS + group; // of the stages, before their turn
+        int s = in_order + turn;
         s = (s >= stages ? s - stages : s) + first_stage;
         const Product &q = p.product[MODE == HIDDEN_GRADIENTS ? (second ? 2 : 0) : MODE == INPUT_GRADIENT ? (second ? 1 : 0) : which];
-        const uint32_t stage = to + (uint32_t)half * (STAGE * 16u);
-        uint4 *const zeros = slots + half * STAGE;
-        const int left = p.K - 64 * s;
-        const bool b_second = MODE == HIDDEN_GRADIENTS && second && !brings_a;
-        if (brings_a ? A_MMAJOR : (B_MMAJOR || b_second)) {
-            const char *base = reinterpret_cast<const char *>(brings_a ? q.a + (int64_t)64 * s * q.a_ld + m0 : q.b + (int64_t)64 * s * q.b_ld + n0);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int u = w8 + i;
-                if (b_second && u >= 16) {
-                    continue; // SIDE / 2 columns, or 128 at least
-                }
-                if (4 * (u & 15) + mm_k < left) {
-                    load_to_lds(stage + i * 1024u, base, b_second ? from_second[i] : from[i]);
-                } else {
-                    zeros[i * 64] = zero_u4();
-                }
-            }
+        Stage st;
+        st.own = MODE == HIDDEN_GRADIENTS && second;
+        st.a = (uint64_t)(q.a + (A_MMAJOR ? (int64_t)64 * s * q.a_ld + m0 : (int64_t)m0 * q.a_ld + 64 * s));
+        st.b = (uint64_t)(q.b + (B_MMAJOR || st.own ? (int64_t)64 * s * q.b_ld + n0 : (int64_t)n0 * q.b_ld + 64 * s));
+        st.up = HIDDEN && !st.own ? (uint64_t)(p.product[1].b + (int64_t)n0 * p.product[1].b_ld + 64 * s) : st.b;
+        st.to = to + (uint32_t)half * (STAGE * 16u);
+        st.half = half;
+        st.left = GROUPS > 1 && in_order >= stages ? 0 : p.K - 64 * s;
+        return st;
+    };
+    auto base_of = [&](Stage st, bool is_a, int u) {
+        const uint64_t b = HIDDEN && (u & 4) ? st.up : st.b;
+        return same_in_all_lanes((const void *)(is_a ? st.a : b));
+    };
+    auto from_of = [&](Stage st, int i) {
+        if constexpr (MODE == HIDDEN_GRADIENTS) {
+            return st.own ? from_second[i] : from[i];
         } else {
-            const bool there = 8 * chunk < left;
+            return from[i];
+        }
+    };
+    auto ask = [&](Stage st) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const bf16_t *operand = brings_a ? q.a + (int64_t)m0 * q.a_ld : (HIDDEN && i >= 4 ? p.product[1].b : q.b) + (int64_t)n0 * q.b_ld;
-                if (there) {
-                    load_to_lds(stage + i * 1024u, operand + 64 * s, MODE == HIDDEN_GRADIENTS && second ? from_second[i] : from[i]);
-                } else {
-                    zeros[i * 64] = zero_u4();
-                }
+        for (int i = 0; i < UNITS; ++i) {
+            const bool is_a = first_unit + i < A_UNITS;
+            const int u = is_a ? first_unit + i : first_unit + i - A_UNITS;
+            if ((is_a ? A_MMAJOR : B_MMAJOR || st.own) ? 4 * (u & 15) + mm_k < st.left : 8 * chunk < st.left) {
+                load_to_lds(st.to + i * 1024u, base_of(st, is_a, u), from_of(st, i));
+            } else {
+                slots[st.half * STAGE + i * 64] = zero_u4();
             }
         }
+    };
+    // unit i of a whole stage in all lanes (`lanes` -1) or none (0): without a branch, beside the products
+    auto ask_whole = [&](Stage st, int i, int lanes) {
+        const bool is_a = first_unit + i < A_UNITS;
+        const int u = is_a ? first_unit + i : first_unit + i - A_UNITS;
+        asm volatile("s_mov_b32 exec_lo, %3\n\ts_mov_b32 exec_hi, %3\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, -1" ::"s"(st.to + i * 1024u),
+                     "v"(from_of(st, i)), "s"(base_of(st, is_a, u)), "s"(lanes)
+                     : "memory");
     };
 
     constexpr int SUMS = MODE == HIDDEN_GRADIENTS ? 3 : 2; // 32-wide column blocks of a wave
@@ -355,7 +390,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ff_pieces_kernel(const TilesP
         constexpr int NB = OWN ? 1 : 2;
         bf16x8 a[2][MI], b[2][NB];
         auto fetch = [&](int set, const uint4 *stage, int s, int n) { // fragment n of a quarter's MI + NB
-            const uint4 *columns = stage + SIDE * 8;
+            const uint4 *columns = stage + ROWS * 8;
             if (n < NB) {
                 if constexpr (OWN) {
                     b[set][n] = mm_fragment((const lds_char *)columns, own_mm, s);
@@ -374,47 +409,57 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ff_pieces_kernel(const TilesP
         for (int n = 0; n < MI + NB; ++n) {
             fetch(0, lds + (t & 1) * STAGE, 0, n);
         }
-        for (const int end = t + stages; t < end; ++t) {
-            const uint4 *stage = lds + (t & 1) * STAGE, *other = lds + ((t + 1) & 1) * STAGE;
+        // the products of 16 k, beside them the fragments of the next 16, and with ASK a wave's units of a stage
+        auto quarter = [&](const uint4 *from_stage, int s, auto asks, Stage st, int lanes) {
+            constexpr int STEPS = MI * NB, TOTAL = MI + NB;
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                if (s == 3) { // the next stage is there, and all have read this one; behind the last one what is read is not used
-                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                    if (t + 2 < total) {
-                        ask(t + 2, t & 1);
+            for (int n = 0; n < STEPS; ++n) {
+                const int i = n / NB, j = n % NB;
+                f32x16 &sum = acc[OWN ? 2 : j][i];
+                sum = mfma(b[s & 1][j], a[s & 1][i], sum);
+                asm volatile("" : "+a"(sum)); // not to be moved behind the barrier
+#pragma unroll
+                for (int f = n * TOTAL / STEPS; f < (n + 1) * TOTAL / STEPS; ++f) {
+                    fetch((s + 1) & 1, from_stage, (s + 1) & 3, f);
+                }
+                if constexpr (decltype(asks)::value) {
+#pragma unroll
+                    for (int i = n * UNITS / STEPS; i < (n + 1) * UNITS / STEPS; ++i) {
+                        ask_whole(st, i, lanes);
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int n = 0; n < MI * NB; ++n) {
-                    const int i = n / NB, j = n % NB;
-                    f32x16 &sum = acc[OWN ? 2 : j][i];
-                    sum = mfma(b[s & 1][j], a[s & 1][i], sum);
-                    asm volatile("" : "+a"(sum));
-                    // the next quarter's fragments, one or two beside a product
-                    constexpr int TOTAL = MI + NB, STEPS = MI * NB;
-#pragma unroll
-                    for (int f = n * TOTAL / STEPS; f < (n + 1) * TOTAL / STEPS; ++f) {
-                        fetch((s + 1) & 1, s == 3 ? other : stage, (s + 1) & 3, f);
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
-                }
             }
+        };
+        for (const int end = t + steps; t < end; ++t) {
+            const uint4 *stage = lds + (t & 1) * STAGE, *other = lds + ((t + 1) & 1) * STAGE;
+            const Stage then = stage_of(t + 2, t & 1);
+            __builtin_amdgcn_sched_barrier(0);
+            quarter(stage, 0, std::false_type{}, then, 0);
+            quarter(stage, 1, std::false_type{}, then, 0);
+            quarter(stage, 2, std::false_type{}, then, 0);
+            // the next stage is there, and all have read this one; behind the last one what is read is not used
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            const bool more = t + 2 < total;
+            if (more && then.left < 64) {
+                ask(then);
+            }
+            quarter(other, 3, std::true_type{}, then, __builtin_amdgcn_readfirstlane(more && then.left >= 64 ? -1 : 0));
         }
     };
-    ask(0, 0);
+    ask(stage_of(0, 0));
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (total > 1) {
-        ask(1, 1);
+        ask(stage_of(1, 1));
     }
     run(std::false_type{});
     if constexpr (TWO) {
         run(std::true_type{});
     }
 
-    if constexpr (MODE == WEIGHT_GRADIENTS) {
+    if constexpr (MODE == WEIGHT_GRADIENTS && MI == 2) {
         if (p.splits > 1) { // a share of the sums, lane by lane: [split][tile of all three][wave][MI][2][4][64] of 16 bytes
-            f32x4 *share = reinterpret_cast<f32x4 *>(p.shares) + ((int64_t)blockIdx.x * (WM * WN) + wave) * (MI * 2 * 4 * 64) + lane;
+            f32x4 *share = reinterpret_cast<f32x4 *>(p.shares) + ((int64_t)place * (WM * WN) + member) * (MI * 2 * 4 * 64) + lane;
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
 #pragma unroll
@@ -428,11 +473,39 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ff_pieces_kernel(const TilesP
             return;
         }
     }
+    if constexpr (GROUPS == 2) { // the second group's sums to the first
+        constexpr int PER_WAVE = 2 * MI * 4 * 64;
+        static_assert(WM * WN * PER_WAVE <= GROUPS * 2 * STAGE, "the sums lie where the operands were");
+        __syncthreads(); // what the other waves have read ahead lies there
+        f32x4 *sums = reinterpret_cast<f32x4 *>(all_lds) + member * PER_WAVE + lane;
+        if (group == 1) {
+#pragma unroll
+            for (int n = 0; n < 2 * MI * 4; ++n) {
+                const f32x16 &v = acc[n & 1][n / 8];
+                const int e = n / 2 % 4;
+                sums[n * 64] = f32x4{v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]};
+            }
+        }
+        __syncthreads();
+        if (group == 1) {
+            return;
+        }
+#pragma unroll
+        for (int n = 0; n < 2 * MI * 4; ++n) {
+            const f32x4 v = sums[n * 64];
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+                acc[n & 1][n / 8][4 * (n / 2 % 4) + f] += v[f];
+            }
+        }
+    }
     // results as bf16 through a strip of the LDS of the wave's own, 32 rows by WIDTH columns, out in whole runs of WIDTH
     constexpr int WIDTH = HIDDEN ? 32 : 64, STRIP_LD = WIDTH + 8;
     static_assert(WM * WN * 32 * STRIP_LD * 2 <= 2 * STAGE * 16, "the strips lie where the operands were");
-    __syncthreads(); // what the other waves have read ahead lies there
-    bf16_t *strip = reinterpret_cast<bf16_t *>(lds) + wave * 32 * STRIP_LD;
+    if constexpr (GROUPS == 1) {
+        __syncthreads(); // what the other waves have read ahead lies there
+    }
+    bf16_t *strip = reinterpret_cast<bf16_t *>(lds + GROUPS / 2 * 2 * STAGE) + member * 32 * STRIP_LD; // with two groups, behind the sums
     auto store = [&](bf16_t *c, int64_t ld, int i, auto value) {
 #pragma unroll
         for (int j = 0; j < WIDTH / 32; ++j) {
@@ -512,6 +585,137 @@ __global__ __launch_bounds__(256) void ff_shares_kernel(const TilesParams p)
     }
 }
 
+// ---- few rows, or few tiles: the W waves of a workgroup share the blocks of 64 k ----
+//
+// 16 MB rows by 16 NB columns a workgroup, all of them in every wave (and with GATED of both projections): wave w takes blocks w, w + W, ... and brings
+// them straight into its own part of the LDS, eight rows of 128 bytes a load, DEPTH blocks ahead and without barriers.  The waves' sums meet in the LDS at
+// the end, in one order.
+template <int MODE, int MB, int NB, int W, int DEPTH>
+__global__ __launch_bounds__(64 * W) void ff_split_kernel(const TilesParams p)
+{
+    static_assert(MODE == PLAIN || MODE == GATED, "operands along k");
+    constexpr int SUMS = MODE == GATED ? 2 : 1, LOADS = 2 * (MB + SUMS * NB), SLOTS = 64 * LOADS;
+    static_assert(SUMS * MB * NB <= DEPTH * LOADS, "the sums lie where the operands were");
+    extern __shared__ uint4 lds[]; // [W][DEPTH][SLOTS], and at the end sums [W][SUMS][NB][MB][64]
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 15, q = lane >> 4;
+    const int M = p.M[0], N = p.N[0], NT = (N + 16 * NB - 1) / (16 * NB);
+    const int n0 = (int)(blockIdx.x % (unsigned)NT) * 16 * NB, m0 = (int)(blockIdx.x / (unsigned)NT) * 16 * MB;
+    const int blocks = (p.K + 63) / 64;
+    const int chunk = (lane & 7) ^ (lane >> 3);
+    const bf16_t *const a_tile = p.product[0].a + (int64_t)m0 * p.product[0].a_ld;
+    uint32_t a_from[2 * MB], b_from[2 * NB];
+#pragma unroll
+    for (int u = 0; u < 2 * MB; ++u) {
+        a_from[u] = 2u * ((uint32_t)min(8 * u + (lane >> 3), M - m0 - 1) * (uint32_t)p.product[0].a_ld + 8u * (uint32_t)chunk);
+    }
+#pragma unroll
+    for (int u = 0; u < 2 * NB; ++u) {
+        b_from[u] = 2u * ((uint32_t)min(8 * u + (lane >> 3), N - n0 - 1) * (uint32_t)p.product[0].b_ld + 8u * (uint32_t)chunk);
+    }
+    uint4 *const mine = lds + wave * DEPTH * SLOTS;
+    const uint32_t to = (uint32_t)(uintptr_t)(const lds_char *)mine;
+    auto ask = [&](int b, int slot) {
+        const uint32_t stage = to + (uint32_t)slot * (SLOTS * 16u);
+        if (8 * chunk < p.K - 64 * b) {
+#pragma unroll
+            for (int u = 0; u < 2 * MB; ++u) {
+                load_to_lds(stage + u * 1024u, a_tile + (int64_t)64 * b, a_from[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < 2 * NB * SUMS; ++u) {
+                load_to_lds(stage + (2 * MB + u) * 1024u, p.product[u / (2 * NB)].b + (int64_t)n0 * p.product[0].b_ld + (int64_t)64 * b, b_from[u % (2 * NB)]);
+            }
+        } else { // past the end of a cut block
+#pragma unroll
+            for (int u = 0; u < LOADS; ++u) {
+                mine[slot * SLOTS + u * 64 + lane] = zero_u4();
+            }
+        }
+    };
+    f32x4 acc[SUMS][NB][MB];
+#pragma unroll
+    for (int n = 0; n < SUMS * NB * MB; ++n) {
+        acc[n / (NB * MB)][n / MB % NB][n % MB] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+        if (wave + d * W < blocks) {
+            ask(wave + d * W, d);
+        }
+    }
+    int slot = 0;
+    for (int b = wave; b < blocks; b += W) {
+        if (b + (DEPTH - 1) * W < blocks) {
+            wait_for_loads<(DEPTH - 1) * LOADS>();
+        } else {
+            wait_for_loads<0>();
+        }
+        const uint4 *stage = mine + slot * SLOTS;
+        auto operand_of = [&](int block16, int half) { return as_bf16x8(stage[(16 * block16 + r) * 8 + ((4 * half + q) ^ (r & 7))]); };
+        bf16x8 a[MB][2], w[SUMS * NB][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int j = 0; j < MB; ++j) {
+                a[j][h] = operand_of(j, h);
+            }
+#pragma unroll
+            for (int i = 0; i < SUMS * NB; ++i) {
+                w[i][h] = operand_of(MB + i, h);
+            }
+        }
+        if (b + DEPTH * W < blocks) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the operands are out of the LDS
+            ask(b + DEPTH * W, slot);
+        }
+        slot = slot + 1 < DEPTH ? slot + 1 : 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < SUMS * NB; ++i) {
+#pragma unroll
+                for (int j = 0; j < MB; ++j) {
+                    f32x4 &sum = acc[i / NB][i % NB][j];
+                    sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[i][h], a[j][h], sum, 0, 0, 0);
+                }
+            }
+        }
+    }
+    __syncthreads(); // the sums take the operands' place
+    f32x4 *sums = reinterpret_cast<f32x4 *>(lds);
+#pragma unroll
+    for (int n = 0; n < SUMS * NB * MB; ++n) {
+        sums[(wave * SUMS * NB * MB + n) * 64 + lane] = acc[n / (NB * MB)][n / MB % NB][n % MB];
+    }
+    __syncthreads();
+    for (int t = wave; t < NB * MB; t += W) {
+        f32x4 sum[SUMS];
+#pragma unroll
+        for (int s = 0; s < SUMS; ++s) {
+            sum[s] = sums[(s * NB * MB + t) * 64 + lane];
+#pragma unroll
+            for (int v = 1; v < W; ++v) {
+                sum[s] += sums[((v * SUMS + s) * NB * MB + t) * 64 + lane];
+            }
+        }
+        const int m = m0 + 16 * (t % MB) + r, n = n0 + 16 * (t / MB) + 4 * q;
+        bf16x4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (MODE == GATED) {
+                float none;
+                o[e] = (bf16_t)(activate<false>(sum[0][e], p.activation, none) * sum[1][e]);
+            } else {
+                o[e] = (bf16_t)sum[0][e];
+            }
+        }
+        if (m < M && n < N) { // N is a multiple of 8
+            *reinterpret_cast<bf16x4 *>(p.c[0] + (int64_t)m * p.c_ld[0] + n) = o;
+        }
+    }
+}
+
 // Whether a product's operands fill whole 16-byte pieces: pointers, pitches, and the extents along which rows are contiguous
 bool pieces(const void *ptr, int64_t ld, int64_t contiguous) { return kutacc_hip_aligned16(ptr) && ld % 8 == 0 && contiguous % 8 == 0 && ld < (1 << 23); }
 
@@ -551,41 +755,122 @@ int64_t count_tiles(TilesParams &p, int side, int columns)
     return all;
 }
 
-template <int MODE, int MI, int WM, int WN>
+template <int MODE, int MI, int WM, int WN, int GROUPS>
 int launch_pieces(TilesParams p, hipStream_t stream)
 {
-    constexpr int SIDE = 32 * MI * WM;
+    constexpr int ROWS = 32 * MI * WM, SIDE = 64 * WN;
+    constexpr size_t LDS = (size_t)GROUPS * 2 * (ROWS + SIDE) * 128;
     static size_t configured[KUTACC_DEVICE_SLOTS] = {};
-    const auto kernel = &ff_pieces_kernel<MODE, MI, WM, WN>;
-    const int64_t tiles = count_tiles(p, SIDE, MODE == GATED || MODE == HIDDEN_GRADIENTS ? SIDE / 2 : SIDE), groups = tiles * p.splits;
+    const auto kernel = &ff_pieces_kernel<MODE, MI, WM, WN, GROUPS>;
+    const int64_t tiles = count_tiles(p, ROWS, MODE == GATED || MODE == HIDDEN_GRADIENTS ? SIDE / 2 : SIDE), groups = tiles * p.splits;
     if (groups > INT32_MAX) {
         return KUTACC_HIP_EUNSUPPORTED;
     }
-    if (const hipError_t e = kutacc_opt_in_lds(reinterpret_cast<const void *>(kernel), 2 * 2 * SIDE * 128, configured)) {
+    if (const hipError_t e = kutacc_opt_in_lds(reinterpret_cast<const void *>(kernel), LDS, configured)) {
         return kutacc_hip_status(e);
     }
-    kernel<<<dim3((unsigned)groups), 64 * WM * WN, 2 * 2 * SIDE * 128, stream>>>(p);
-    if (MODE == WEIGHT_GRADIENTS && p.splits > 1) {
+    kernel<<<dim3((unsigned)groups), 64 * WM * WN * GROUPS, LDS, stream>>>(p);
+    if (MODE == WEIGHT_GRADIENTS && MI == 2 && p.splits > 1) {
         ff_shares_kernel<MI, WM, WN><<<dim3((unsigned)(tiles * WM * WN * MI * 2)), 256, 0, stream>>>(p);
     }
     return kutacc_hip_status(hipGetLastError());
 }
 
-bool enough_large(TilesParams p, int columns) { return 4 * count_tiles(p, 256, columns) >= 3 * kutacc_cu_count(); }
+template <int MODE, int MB, int NB, int W, int DEPTH>
+int launch_split(TilesParams p, hipStream_t stream)
+{
+    constexpr size_t LDS = (size_t)W * DEPTH * 2 * (MB + (MODE == GATED ? 2 : 1) * NB) * 1024;
+    static size_t configured[KUTACC_DEVICE_SLOTS] = {};
+    const auto kernel = &ff_split_kernel<MODE, MB, NB, W, DEPTH>;
+    const int64_t groups = count_tiles(p, 16 * MB, 16 * NB);
+    if (groups > INT32_MAX) {
+        return KUTACC_HIP_EUNSUPPORTED;
+    }
+    if (const hipError_t e = kutacc_opt_in_lds(reinterpret_cast<const void *>(kernel), LDS, configured)) {
+        return kutacc_hip_status(e);
+    }
+    kernel<<<dim3((unsigned)groups), 64 * W, LDS, stream>>>(p);
+    return kutacc_hip_status(hipGetLastError());
+}
+
+// whether the weights' gradients make enough tiles of 256 x 256 without a split of their rows
+bool whole_rows(TilesParams p) { return 4 * count_tiles(p, 256, 256) >= 3 * kutacc_cu_count(); }
+
+// A kernel's tile, how many of its workgroups a CU holds, and what a round of them takes for 64 k
+struct Choice {
+    int rows, columns, per_cu;
+    float round;
+};
+// the one that takes the fewest rounds, weighted with what they take
+template <int N>
+int least(TilesParams p, const Choice (&choices)[N])
+{
+    int best = 0;
+    double time = 0;
+    for (int i = 0; i < N; ++i) {
+        const int64_t slots = (int64_t)kutacc_cu_count() * choices[i].per_cu;
+        const double t = (double)((count_tiles(p, choices[i].rows, choices[i].columns) + slots - 1) / slots) * choices[i].round;
+        if (i == 0 || t < time) {
+            best = i, time = t;
+        }
+    }
+    return best;
+}
+
+// The rounds' times are measured, us for 64 k: 4001 x 1024 x 2816, 8192 x 2048 x 8192, 1000 x 1024 x 4096, 128 x 2048 x 8192 (rows x columns x k) and for the
+// gated form 4001 x 2816 x 1024, 8192 x 8192 x 2048, 256 x 4096 x 1024, 64 x 8192 x 2048.
+template <int MODE>
+int launch_whole(const TilesParams &p, hipStream_t stream)
+{
+    if constexpr (MODE == PLAIN) {
+        if (p.M[0] <= 16) {
+            return launch_split<MODE, 1, 1, 16, 2>(p, stream);
+        }
+        constexpr Choice choices[] = {{32, 32, 1, 0.10f}, {32, 64, 1, 0.13f}, {64, 64, 1, 0.23f}, {128, 128, 1, 0.66f}, {128, 128, 2, 1.05f}, {192, 256, 1, 1.41f}, {256, 256, 1, 1.70f}};
+        switch (least(p, choices)) {
+        case 0: return launch_split<MODE, 2, 2, 16, 1>(p, stream);
+        case 1: return launch_split<MODE, 2, 4, 8, 1>(p, stream);
+        case 2: return launch_split<MODE, 4, 4, 8, 1>(p, stream);
+        case 3: return launch_pieces<MODE, 2, 2, 2, 2>(p, stream);
+        case 4: return launch_pieces<MODE, 2, 2, 2, 1>(p, stream);
+        case 5: return launch_pieces<MODE, 3, 2, 4, 1>(p, stream);
+        default: return launch_pieces<MODE, 4, 2, 4, 1>(p, stream);
+        }
+    } else if constexpr (MODE == GATED) {
+        if (p.M[0] <= 16) {
+            return launch_split<MODE, 1, 1, 8, 2>(p, stream);
+        }
+        constexpr Choice choices[] = {{32, 32, 1, 0.23f}, {64, 32, 1, 0.33f}, {128, 64, 2, 1.15f}, {192, 128, 1, 1.45f}, {256, 128, 1, 1.90f}};
+        switch (least(p, choices)) {
+        case 0: return launch_split<MODE, 2, 2, 8, 1>(p, stream);
+        case 1: return launch_split<MODE, 4, 2, 8, 1>(p, stream);
+        case 2: return launch_pieces<MODE, 2, 2, 2, 1>(p, stream);
+        case 3: return launch_pieces<MODE, 3, 2, 4, 1>(p, stream);
+        default: return launch_pieces<MODE, 4, 2, 4, 1>(p, stream);
+        }
+    } else if constexpr (MODE == HIDDEN_GRADIENTS) {
+        constexpr Choice choices[] = {{128, 64, 2, 1.0f}, {192, 128, 1, 1.27f}};
+        return least(p, choices) == 0 ? launch_pieces<MODE, 2, 2, 2, 1>(p, stream) : launch_pieces<MODE, 3, 2, 4, 1>(p, stream);
+    } else if constexpr (MODE == INPUT_GRADIENT) {
+        constexpr Choice choices[] = {{128, 128, 1, 0.61f}, {128, 128, 2, 0.97f}, {256, 256, 1, 1.55f}};
+        switch (least(p, choices)) {
+        case 0: return launch_pieces<MODE, 2, 2, 2, 2>(p, stream);
+        case 1: return launch_pieces<MODE, 2, 2, 2, 1>(p, stream);
+        default: return launch_pieces<MODE, 4, 2, 4, 1>(p, stream);
+        }
+    } else {
+        return p.splits == 1 && whole_rows(p) ? launch_pieces<MODE, 4, 2, 4, 1>(p, stream) : launch_pieces<MODE, 2, 2, 2, 1>(p, stream);
+    }
+}
 
 template <int MODE>
-int launch_tiles(const TilesParams &p, bool any, double flops, const char *name, hipStream_t stream)
+int launch(const TilesParams &p, bool any, double flops, const char *name, hipStream_t stream)
 {
     if (any) {
         return launch_any<MODE>(p, true, flops, name, stream);
     }
     kutacc_prof::KernelTimer t(name, flops, stream);
-    if constexpr (MODE != HIDDEN_GRADIENTS) {
-        if (enough_large(p, MODE == GATED ? 128 : 256)) {
-            return launch_pieces<MODE, 4, 2, 4>(p, stream);
-        }
-    }
-    return launch_pieces<MODE, 2, 2, 2>(p, stream);
+    return launch_whole<MODE>(p, stream);
 }
 
 // How many ways the rows are split for the weights' gradients: 128 x 128 tiles of fewer than two workgroups a CU, into ranges of at least eight stages
@@ -593,19 +878,11 @@ int weight_splits(int64_t rows, int64_t c_o, int64_t c_i)
 {
     TilesParams p = {};
     p.M[0] = p.M[1] = (int)c_i, p.N[0] = p.N[1] = (int)c_o, p.M[2] = (int)c_o, p.N[2] = (int)c_i;
-    if (enough_large(p, 256)) {
+    if (whole_rows(p)) {
         return 1;
     }
     const int64_t tiles = count_tiles(p, 128, 128), stages = (rows + 63) / 64;
     return (int)std::max<int64_t>(1, std::min<int64_t>(2 * kutacc_cu_count() / tiles, stages / 8));
-}
-int launch_weight_gradients(const TilesParams &p, bool any, double flops, const char *name, hipStream_t stream)
-{
-    if (any) {
-        return launch_any<WEIGHT_GRADIENTS>(p, true, flops, name, stream);
-    }
-    kutacc_prof::KernelTimer t(name, flops, stream);
-    return p.splits == 1 && enough_large(p, 256) ? launch_pieces<WEIGHT_GRADIENTS, 4, 2, 4>(p, stream) : launch_pieces<WEIGHT_GRADIENTS, 2, 2, 2>(p, stream);
 }
 int64_t shares_bytes(int64_t rows, int64_t c_o, int64_t c_i)
 {
@@ -633,7 +910,7 @@ int gated_transition(const kutacc_hip_gated_transition_args_t &a, hipStream_t st
     p.M[0] = (int)rows, p.N[0] = (int)c_i, p.K = (int)c_o, p.activation = a.activation;
     const bool widths = c_o % 8 == 0 && c_i % 8 == 0;
     const bool any_in = !widths || !pieces(a.x, a.x_ld, c_o) || !kutacc_hip_aligned16(a.gate_w) || !kutacc_hip_aligned16(a.up_w);
-    if (const int rc = launch_tiles<GATED>(p, any_in, 4.0 * (double)rows * (double)c_o * (double)c_i, "ff_tiles_kernel<gated>", stream)) {
+    if (const int rc = launch<GATED>(p, any_in, 4.0 * (double)rows * (double)c_o * (double)c_i, "gated_transition<gated>", stream)) {
         return rc;
     }
     TilesParams d = {};
@@ -641,7 +918,7 @@ int gated_transition(const kutacc_hip_gated_transition_args_t &a, hipStream_t st
     d.product[0] = {h, (const bf16_t *)a.down_w, h_ld, c_i};
     d.c[0] = (bf16_t *)a.out, d.c_ld[0] = a.out_ld;
     d.M[0] = (int)rows, d.N[0] = (int)c_o, d.K = (int)c_i;
-    return launch_tiles<PLAIN>(d, !widths || !kutacc_hip_aligned16(a.down_w) || !pieces(a.out, a.out_ld, c_o), 2.0 * (double)rows * (double)c_o * (double)c_i, "ff_tiles_kernel<plain>", stream);
+    return launch<PLAIN>(d, !widths || !kutacc_hip_aligned16(a.down_w) || !pieces(a.out, a.out_ld, c_o), 2.0 * (double)rows * (double)c_o * (double)c_i, "gated_transition<plain>", stream);
 }
 
 int64_t gated_transition_backward_workspace(int64_t rows, int64_t c_o, int64_t c_i) { return 3 * align256(2 * rows * padded(c_i)) + shares_bytes(rows, c_o, c_i); }
@@ -662,7 +939,7 @@ int gated_transition_backward(const kutacc_hip_gated_transition_backward_args_t 
     p.product[2] = {dy, wd, a.grad_out_ld, c_i};
     p.c[0] = h, p.c[1] = dg, p.c[2] = du, p.c_ld[0] = p.c_ld[1] = p.c_ld[2] = ld;
     p.M[0] = (int)rows, p.N[0] = (int)c_i, p.K = (int)c_o, p.activation = a.activation;
-    if (const int rc = launch_tiles<HIDDEN_GRADIENTS>(p, !rows_fit || !weights_fit || !kutacc_hip_aligned16(wd), 3 * flops, "ff_tiles_kernel<hidden gradients>", stream)) {
+    if (const int rc = launch<HIDDEN_GRADIENTS>(p, !rows_fit || !weights_fit || !kutacc_hip_aligned16(wd), 3 * flops, "gated_transition<hidden gradients>", stream)) {
         return rc;
     }
     if (a.grad_x != nullptr) {
@@ -672,7 +949,7 @@ int gated_transition_backward(const kutacc_hip_gated_transition_backward_args_t 
         d.product[1] = {du, wu, ld, c_o};
         d.c[0] = (bf16_t *)a.grad_x, d.c_ld[0] = a.grad_x_ld;
         d.M[0] = (int)rows, d.N[0] = (int)c_o, d.K = (int)c_i;
-        if (const int rc = launch_tiles<INPUT_GRADIENT>(d, !weights_fit || !pieces(a.grad_x, a.grad_x_ld, c_o), 2 * flops, "ff_tiles_kernel<input gradient>", stream)) {
+        if (const int rc = launch<INPUT_GRADIENT>(d, !weights_fit || !pieces(a.grad_x, a.grad_x_ld, c_o), 2 * flops, "gated_transition<input gradient>", stream)) {
             return rc;
         }
     }
@@ -692,7 +969,7 @@ int gated_transition_backward(const kutacc_hip_gated_transition_backward_args_t 
     const bool aligned = (!a.grad_gate_w || kutacc_hip_aligned16(a.grad_gate_w)) && (!a.grad_up_w || kutacc_hip_aligned16(a.grad_up_w)) && (!a.grad_down_w || kutacc_hip_aligned16(a.grad_down_w));
     w.splits = weight_splits(rows, c_o, c_i);
     w.shares = reinterpret_cast<float *>(du + each);
-    return count == 0 ? 0 : launch_weight_gradients(w, !rows_fit || !widths || !aligned, count * flops, "ff_tiles_kernel<weight gradients>", stream);
+    return count == 0 ? 0 : launch<WEIGHT_GRADIENTS>(w, !rows_fit || !widths || !aligned, count * flops, "gated_transition<weight gradients>", stream);
 }
 
 } // namespace kutacc_launch

@@ -349,6 +349,24 @@ def test_gated_transition_backward(activation, c_o, c_i):
         assert all(torch.equal(a, r.view) for a, r in zip(first, grads.values())), "other bits the second time"
 
 
+# enough tiles for the kernels of 128, 192 and 256 rows a tile in every product: ragged sides, k that ends within a stage, an odd number of stages for two groups
+@pytest.mark.parametrize("rows,c_o,c_i", [(4001, 264, 2816), (5000, 136, 2816), (8090, 2048, 72), (8090, 1032, 200), (4001, 72, 4096), (130, 1024, 4096), (2100, 512, 520), (1000, 1024, 1096),
+                                          (40000, 64, 136)])
+def test_gated_transition_of_many_tiles(rows, c_o, c_i):
+    w = weights_of(rows, c_o, c_i)
+    gpu, x, dy = [t.cuda() for t in w], cpu_randn(1, rows, c_o), cpu_randn(2, rows, c_o)
+    want = oracle.gated_transition(x, *w, "silu", dy)
+    out = Room(rows, c_o, BF16)
+    ok(capi.GatedTransition(x.cuda(), *gpu, out.view))
+    oracle.close(out.view, want["out"][0], oracle.stored(*want["out"], BF16), "out")
+    out.untouched("out")
+    grads = dict(grad_x=Room(rows, c_o, BF16), grad_gate_w=Room(c_i, c_o, BF16), grad_up_w=Room(c_i, c_o, BF16), grad_down_w=Room(c_o, c_i, BF16))
+    ok(capi.GatedTransitionBackward(x.cuda(), *gpu, dy.cuda(), **{k: r.view for k, r in grads.items()}))
+    for name, r in grads.items():
+        oracle.close(r.view, want[name][0], oracle.stored(*want[name], BF16), name)
+        r.untouched(name)
+
+
 def test_gated_transition_backward_gives_the_gradients_that_are_asked_for():
     rows, c_o, c_i = 90, 128, 192
     w = weights_of(1, c_o, c_i)
