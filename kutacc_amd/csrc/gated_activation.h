@@ -1,0 +1,31 @@
+// The activation of the gated transition: act(v) = v sigmoid(t(v)), for silu t = v, for gelu in its tanh form t = 2 sqrt(2 / pi) (v + 0.044715 v^3).
+// Its derivative is s + v s (1 - s) t'(v) with s = sigmoid(t(v)).
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include "kutacc_hip.h"
+#include "mfma_tiles.h"
+
+namespace kutacc_dev {
+
+constexpr float GELU_SLOPE = 1.5957691216057308f, GELU_CUBE = 0.044715f; // 2 sqrt(2 / pi)
+
+// 2^(this) = exp(-t(v))
+__device__ __forceinline__ float activation_exponent(float v, int activation)
+{
+    return activation == KUTACC_HIP_GELU ? v * fmaf(-LOG2E * GELU_SLOPE * GELU_CUBE, v * v, -LOG2E * GELU_SLOPE) : -LOG2E * v;
+}
+
+// act(v), and its derivative where it is asked for
+template <bool DERIVATIVE>
+__device__ __forceinline__ float activate(float v, int activation, float &derivative)
+{
+    const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(activation_exponent(v, activation))), a = v * s;
+    if constexpr (DERIVATIVE) {
+        const float slope = activation == KUTACC_HIP_GELU ? GELU_SLOPE * fmaf(3.f * GELU_CUBE, v * v, 1.f) : 1.f;
+        derivative = fmaf(a * (1.f - s), slope, s);
+    }
+    return a;
+}
+
+} // namespace kutacc_dev

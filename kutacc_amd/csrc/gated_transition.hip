@@ -12,6 +12,7 @@
 
 #include <algorithm>
 
+#include "gated_activation.h"
 #include "gemm_panels.h"
 #include "launch_internal.h"
 #include "mfma_tiles.h"
@@ -19,27 +20,6 @@
 
 namespace {
 using namespace kutacc_dev;
-
-// ---- the activation ----
-
-constexpr float GELU_SLOPE = 1.5957691216057308f, GELU_CUBE = 0.044715f; // 2 sqrt(2 / pi)
-
-// act(v), and its derivative where it is asked for
-template <bool DERIVATIVE>
-__device__ __forceinline__ float activate(float v, int activation, float &derivative)
-{
-    float t = v, slope = 1.f;
-    if (activation == KUTACC_HIP_GELU) {
-        const float square = v * v;
-        t = GELU_SLOPE * fmaf(GELU_CUBE * square, v, v);
-        slope = GELU_SLOPE * fmaf(3.f * GELU_CUBE, square, 1.f);
-    }
-    const float s = sigmoid_fast(t), a = v * s;
-    if constexpr (DERIVATIVE) {
-        derivative = fmaf(a * (1.f - s), slope, s);
-    }
-    return a;
-}
 
 // ---- every shape ----
 
@@ -210,13 +190,6 @@ __global__ __launch_bounds__(256, MODE == GATED || MODE == HIDDEN_GRADIENTS ? 1 
     } else {
         store(acc[0], p.c[which], p.c_ld[which]);
     }
-}
-
-// a pointer that is the same in all lanes, in scalar registers
-__device__ __forceinline__ const void *same_in_all_lanes(const void *p)
-{
-    const uint64_t v = (uint64_t)p;
-    return (const void *)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v) | (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32)) << 32);
 }
 
 // ---- whole 16-byte pieces: WM x WN waves a workgroup, 32 MI x 64 of the tile a wave: 256 x 256 by 2 x 4 waves or 128 x 128 by 2 x 2 ----
@@ -900,6 +873,9 @@ int64_t gated_transition_workspace(int64_t rows, int64_t c_o, int64_t c_i) { ret
 
 int gated_transition(const kutacc_hip_gated_transition_args_t &a, hipStream_t stream)
 {
+    if (gated_rows_takes(a)) {
+        return gated_rows(a, stream);
+    }
     const int64_t rows = a.rows, c_o = a.c_o, c_i = a.c_i, h_ld = padded(c_i);
     bf16_t *h = (bf16_t *)a.workspace;
     TilesParams p = {};

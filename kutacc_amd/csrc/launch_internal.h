@@ -225,6 +225,10 @@ int quantize_fp8(const void *x, int64_t x_ld, void *out, int64_t out_ld, float *
 // fp8_linear.hip
 int linear_fp8(const kutacc_hip_linear_fp8_args_t &args, hipStream_t stream);
 
+// gated_rows.hip: 64, 128 and 256 channels, the hidden layer on chip; whether it can and is the faster way
+bool gated_rows_takes(const kutacc_hip_gated_transition_args_t &args);
+int gated_rows(const kutacc_hip_gated_transition_args_t &args, hipStream_t stream);
+
 // gated_transition.hip
 int64_t gated_transition_workspace(int64_t rows, int64_t c_o, int64_t c_i);
 int gated_transition(const kutacc_hip_gated_transition_args_t &args, hipStream_t stream);

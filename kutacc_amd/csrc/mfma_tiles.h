@@ -280,6 +280,13 @@ __device__ __forceinline__ void load_to_lds(uint32_t to, const void *from, uint3
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(lane_bytes), "s"(from) : "memory");
 }
 
+// a pointer that is the same in all lanes, in scalar registers
+__device__ __forceinline__ const void *same_in_all_lanes(const void *p)
+{
+    const uint64_t v = (uint64_t)p;
+    return (const void *)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v) | (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32)) << 32);
+}
+
 // until at most N of a wave's loads (and stores) are on their way
 template <int N>
 __device__ __forceinline__ void wait_for_loads()

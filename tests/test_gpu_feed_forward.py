@@ -367,6 +367,20 @@ def test_gated_transition_of_many_tiles(rows, c_o, c_i):
         r.untouched(name)
 
 
+# the hidden layer on chip: fewer waves than a round, several rounds with a ragged last one, one slice of hidden units and several, strided rows
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("rows,c_o,c_i,pad", [(1, 64, 32, 0), (45, 64, 96, 8), (33000, 64, 64, 0), (8200, 128, 32, 0), (8191, 128, 64, 8), (9001, 128, 512, 0), (70001, 128, 96, 0),
+                                              (20500, 256, 32, 0), (20900, 256, 160, 8), (33000, 256, 64, 0)])
+def test_gated_transition_on_chip(activation, rows, c_o, c_i, pad):
+    w = weights_of(rows, c_o, c_i)
+    x = cpu_randn(1, rows, c_o)
+    room = Room(rows, c_o, BF16, c_o + pad)
+    ok(capi.GatedTransition(placed(x, c_o + pad), *(t.cuda() for t in w), room.view, activation))
+    want, off = oracle.gated_transition(x, *w, activation)["out"]
+    oracle.close(room.view, want, oracle.stored(want, off, BF16), "out")
+    room.untouched("out")
+
+
 def test_gated_transition_backward_gives_the_gradients_that_are_asked_for():
     rows, c_o, c_i = 90, 128, 192
     w = weights_of(1, c_o, c_i)
