@@ -16,16 +16,23 @@ __device__ __forceinline__ float activation_exponent(float v, int activation)
     return activation == KUTACC_HIP_GELU ? v * fmaf(-LOG2E * GELU_SLOPE * GELU_CUBE, v * v, -LOG2E * GELU_SLOPE) : -LOG2E * v;
 }
 
+// act(v) of s = sigmoid(t(v)), and its derivative
+__device__ __forceinline__ float activation_of_sigmoid(float v, float s, int activation, float &derivative)
+{
+    const float a = v * s;
+    derivative = fmaf(activation == KUTACC_HIP_GELU ? a * (GELU_SLOPE * fmaf(3.f * GELU_CUBE, v * v, 1.f)) : a, 1.f - s, s);
+    return a;
+}
+
 // act(v), and its derivative where it is asked for
 template <bool DERIVATIVE>
 __device__ __forceinline__ float activate(float v, int activation, float &derivative)
 {
-    const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(activation_exponent(v, activation))), a = v * s;
+    const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(activation_exponent(v, activation)));
     if constexpr (DERIVATIVE) {
-        const float slope = activation == KUTACC_HIP_GELU ? GELU_SLOPE * fmaf(3.f * GELU_CUBE, v * v, 1.f) : 1.f;
-        derivative = fmaf(a * (1.f - s), slope, s);
+        return activation_of_sigmoid(v, s, activation, derivative);
     }
-    return a;
+    return v * s;
 }
 
 } // namespace kutacc_dev

@@ -897,10 +897,17 @@ int gated_transition(const kutacc_hip_gated_transition_args_t &a, hipStream_t st
     return launch<PLAIN>(d, !widths || !kutacc_hip_aligned16(a.down_w) || !pieces(a.out, a.out_ld, c_o), 2.0 * (double)rows * (double)c_o * (double)c_i, "gated_transition<plain>", stream);
 }
 
-int64_t gated_transition_backward_workspace(int64_t rows, int64_t c_o, int64_t c_i) { return 3 * align256(2 * rows * padded(c_i)) + shares_bytes(rows, c_o, c_i); }
+int64_t gated_transition_backward_workspace(int64_t rows, int64_t c_o, int64_t c_i)
+{
+    const int64_t bytes = 3 * align256(2 * rows * padded(c_i)) + shares_bytes(rows, c_o, c_i);
+    return c_o == 64 || c_o == 128 ? std::max(bytes, gated_rows_backward_workspace(rows, c_o, c_i)) : bytes;
+}
 
 int gated_transition_backward(const kutacc_hip_gated_transition_backward_args_t &a, hipStream_t stream)
 {
+    if (gated_rows_backward_takes(a)) {
+        return gated_rows_backward(a, stream);
+    }
     const int64_t rows = a.rows, c_o = a.c_o, c_i = a.c_i, ld = padded(c_i), each = align256(2 * rows * ld) / 2;
     bf16_t *h = (bf16_t *)a.workspace, *dg = h + each, *du = dg + each;
     const bf16_t *x = (const bf16_t *)a.x, *dy = (const bf16_t *)a.grad_out;

@@ -229,6 +229,11 @@ int linear_fp8(const kutacc_hip_linear_fp8_args_t &args, hipStream_t stream);
 bool gated_rows_takes(const kutacc_hip_gated_transition_args_t &args);
 int gated_rows(const kutacc_hip_gated_transition_args_t &args, hipStream_t stream);
 
+// gated_rows_backward.hip: the backward pass of 64 and 128 channels
+bool gated_rows_backward_takes(const kutacc_hip_gated_transition_backward_args_t &args);
+int64_t gated_rows_backward_workspace(int64_t rows, int64_t c_o, int64_t c_i);
+int gated_rows_backward(const kutacc_hip_gated_transition_backward_args_t &args, hipStream_t stream);
+
 // gated_transition.hip
 int64_t gated_transition_workspace(int64_t rows, int64_t c_o, int64_t c_i);
 int gated_transition(const kutacc_hip_gated_transition_args_t &args, hipStream_t stream);

@@ -381,6 +381,47 @@ def test_gated_transition_on_chip(activation, rows, c_o, c_i, pad):
     room.untouched("out")
 
 
+# rows that fill no block of 32, one block a split and several, hidden units that fill no group of 128, strided rows, splits with fewer blocks than the others
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("rows,c_o,c_i,pad", [(1, 64, 32, 0), (31, 128, 32, 8), (32, 64, 256, 0), (65, 128, 160, 8), (2049, 64, 96, 0), (9001, 128, 256, 16), (8191, 64, 320, 0), (12289, 128, 512, 0),
+                                              (33001, 128, 288, 8), (70001, 64, 64, 0)])
+def test_gated_transition_backward_on_chip(activation, rows, c_o, c_i, pad):
+    w = weights_of(rows, c_o, c_i)
+    gpu, x, dy = [t.cuda() for t in w], cpu_randn(1, rows, c_o), cpu_randn(2, rows, c_o)
+    want = oracle.gated_transition(x, *w, activation, dy)
+    grads = dict(grad_x=Room(rows, c_o, BF16, c_o + pad), grad_gate_w=Room(c_i, c_o, BF16), grad_up_w=Room(c_i, c_o, BF16), grad_down_w=Room(c_o, c_i, BF16))
+    call = capi.GatedTransitionBackward(placed(x, c_o + pad), *gpu, placed(dy, c_o + 2 * pad), activation=activation, **{k: r.view for k, r in grads.items()})
+    ok(call)
+    for name, r in grads.items():
+        oracle.close(r.view, want[name][0], oracle.stored(*want[name], BF16), name)
+        r.untouched(name)
+    first = [r.view.clone() for r in grads.values()]
+    ok(call)
+    assert all(torch.equal(a, r.view) for a, r in zip(first, grads.values())), "other bits the second time"
+    for name, r in grads.items():  # each alone
+        room = Room(*r.view.shape, BF16)
+        ok(capi.GatedTransitionBackward(placed(x, c_o + pad), *gpu, placed(dy, c_o + 2 * pad), activation=activation, **{name: room.view}))
+        assert torch.equal(room.view, r.view), name
+        room.untouched(name)
+
+
+def test_gated_transition_backward_keeps_a_bad_row_to_itself():
+    """In the gradient of x; the weights' gradients are not-a-number where the sum over the rows is, the last row's included where its block of 32 is not full."""
+    rows, c_o, c_i = 40, 128, 256
+    w = weights_of(1, c_o, c_i)
+    x, dy = cpu_randn(1, rows, c_o), cpu_randn(2, rows, c_o)
+    dy[rows - 1, 5] = math.nan
+    grads = [Room(rows, c_o, BF16), Room(c_i, c_o, BF16), Room(c_i, c_o, BF16), Room(c_o, c_i, BF16)]
+    ok(capi.GatedTransitionBackward(x.cuda(), *(t.cuda() for t in w), dy.cuda(), *(r.view for r in grads)))
+    want = oracle.gated_transition(x[:-1], *w, "silu", dy[:-1])
+    assert bool(torch.isnan(grads[0].view[-1]).all())
+    oracle.close(grads[0].view[:-1], want["grad_x"][0], oracle.stored(*want["grad_x"], BF16), "the other rows")
+    assert bool(torch.isnan(grads[1].view).all()) and bool(torch.isnan(grads[2].view).all()) and bool(torch.isnan(grads[3].view[5]).all())
+    others = [c for c in range(c_o) if c != 5]
+    want = oracle.gated_transition(x, *w, "silu", torch.nan_to_num(dy))
+    oracle.close(grads[3].view[others], want["grad_down_w"][0][others], oracle.stored(*want["grad_down_w"], BF16)[others], "the other channels of Wd")
+
+
 def test_gated_transition_backward_gives_the_gradients_that_are_asked_for():
     rows, c_o, c_i = 90, 128, 192
     w = weights_of(1, c_o, c_i)
