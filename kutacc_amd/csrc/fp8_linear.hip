@@ -121,38 +121,59 @@ __device__ __forceinline__ TileOrder tile_order(const LinearParams &p, unsigned 
     return TileOrder{(int)(8 * band + in % height), (int)(in / height)};
 }
 
-// ---- few rows, or few tiles: the waves of a workgroup share the blocks of k ----
+// ---- rows of fewer than 16 bytes, or very far apart: the waves of a workgroup share the blocks of k ----
 //
 // 16 MB rows of `out` by 16 NB columns a workgroup, all of them in every wave: wave w takes blocks w, w + W, ... of k, straight from memory
-// into registers (16 rows x 64 contiguous bytes a load, two of which make whole lines), and the waves' sums meet in the LDS at the end, in one
-// order.
+// into registers, and the waves' sums meet in the LDS at the end, in one order.
 struct Piece { // 32 bytes of a row of 128: 16 from 16 q on, and 16 from 64 + 16 q on
     uint4 lo, hi;
 };
 
-// `row`: the row's bytes of this block.  A cut block ends after `left` < 128 bytes; what follows is zero and not read.
-__device__ __forceinline__ uint4 load16_cut(const uint8_t *row, int at, int left)
+// the last 16 - n bytes of v, then zeros
+__device__ __forceinline__ uint4 without_first_bytes(uint4 v, int n)
 {
     union {
         uint4 u;
-        uint8_t b[16];
+        unsigned __int128 v;
+    } c;
+    c.u = v;
+    c.v = n < 16 ? c.v >> (8 * n) : 0;
+    return c.u;
+}
+
+// `row`: the row's bytes of this block, `before` of which lie in front of it.  A cut block ends after `left` < 128 bytes; what follows is zero and not read.
+__device__ __forceinline__ uint4 load16_cut(const uint8_t *row, int64_t before, int at, int left)
+{
+    union {
+        uint4 u;
+        unsigned __int128 v;
     } c;
     c.u = zero_u4();
-    if (at + 16 <= left) {
+    if (at >= left) {
+        return c.u;
+    }
+    const int past = at + 16 - left; // of the 16 bytes
+    if (past <= 0) {
         __builtin_memcpy(&c.u, row + at, 16);
-    } else if (at < left) {
-        for (int i = 0; i < left - at; ++i) {
-            c.b[i] = row[at + i];
+    } else if (before + at >= past) {
+        __builtin_memcpy(&c.u, row + at - past, 16);
+        return without_first_bytes(c.u, past);
+    } else { // a row of fewer than 16 bytes
+#pragma unroll
+        for (int i = 0; i < 15; ++i) {
+            if (at + i < left) {
+                c.v |= (unsigned __int128)row[at + i] << (8 * i);
+            }
         }
     }
     return c.u;
 }
 template <bool CUT>
-__device__ __forceinline__ Piece load_piece(const uint8_t *row, int q, int left)
+__device__ __forceinline__ Piece load_piece(const uint8_t *row, int64_t before, int q, int left)
 {
     Piece p;
     if constexpr (CUT) {
-        p.lo = load16_cut(row, 16 * q, left), p.hi = load16_cut(row, 64 + 16 * q, left);
+        p.lo = load16_cut(row, before, 16 * q, left), p.hi = load16_cut(row, before, 64 + 16 * q, left);
     } else {
         __builtin_memcpy(&p.lo, row + 16 * q, 16);
         __builtin_memcpy(&p.hi, row + 64 + 16 * q, 16);
@@ -160,7 +181,7 @@ __device__ __forceinline__ Piece load_piece(const uint8_t *row, int q, int left)
     return p;
 }
 
-template <typename T, int MB, int NB, int W, int AHEAD>
+template <typename T, int MB, int NB, int W>
 __global__ __launch_bounds__(64 * W) void fp8_any_kernel(const LinearParams p)
 {
     constexpr bool WIDE = std::is_same<T, float>::value || MB == 1; // full fp32 sums, also where memory bounds the time anyway
@@ -197,12 +218,12 @@ __global__ __launch_bounds__(64 * W) void fp8_any_kernel(const LinearParams p)
         const int64_t at = (int64_t)b * FP8_BLOCK;
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-            t.w[i] = load_piece<decltype(cut)::value>(w_row[i] + at, q, p.K - (int)at);
+            t.w[i] = load_piece<decltype(cut)::value>(w_row[i] + at, at, q, p.K - (int)at);
             t.ws[i] = w_scale[i][b];
         }
 #pragma unroll
         for (int j = 0; j < MB; ++j) {
-            t.a[j] = load_piece<decltype(cut)::value>(a_row[j] + at, q, p.K - (int)at);
+            t.a[j] = load_piece<decltype(cut)::value>(a_row[j] + at, at, q, p.K - (int)at);
             t.as[j] = a_scale[j][b];
         }
     };
@@ -240,17 +261,6 @@ __global__ __launch_bounds__(64 * W) void fp8_any_kernel(const LinearParams p)
         }
     };
     int b = wave;
-    for (; b + (AHEAD - 1) * W < whole; b += AHEAD * W) {
-        Block t[AHEAD];
-#pragma unroll
-        for (int d = 0; d < AHEAD; ++d) {
-            load(t[d], b + d * W, std::false_type{});
-        }
-#pragma unroll
-        for (int d = 0; d < AHEAD; ++d) {
-            multiply(t[d]);
-        }
-    }
     for (; b < whole; b += W) {
         Block t;
         load(t, b, std::false_type{});
@@ -282,7 +292,7 @@ __global__ __launch_bounds__(64 * W) void fp8_any_kernel(const LinearParams p)
 
 int64_t tiles_of(const LinearParams &p, int rows, int columns) { return ((int64_t)p.M + rows - 1) / rows * (((int64_t)p.N + columns - 1) / columns); }
 
-template <typename T, int MB, int NB, int W, int AHEAD>
+template <typename T, int MB, int NB, int W>
 int launch_any(LinearParams p, hipStream_t stream)
 {
     const int64_t groups = tiles_of(p, 16 * MB, 16 * NB);
@@ -290,7 +300,7 @@ int launch_any(LinearParams p, hipStream_t stream)
         return KUTACC_HIP_EUNSUPPORTED;
     }
     p.NT = (p.N + 16 * NB - 1) / (16 * NB);
-    fp8_any_kernel<T, MB, NB, W, AHEAD><<<dim3((unsigned)groups), 64 * W, (size_t)W * NB * MB * 1024, stream>>>(p);
+    fp8_any_kernel<T, MB, NB, W><<<dim3((unsigned)groups), 64 * W, (size_t)W * NB * MB * 1024, stream>>>(p);
     return kutacc_hip_status(hipGetLastError());
 }
 
@@ -300,10 +310,14 @@ __device__ __forceinline__ void load_dword_to_lds(uint32_t to, const void *from,
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(lane_bytes), "s"(from) : "memory");
 }
 
-// The same where rows are whole 16-byte pieces: a wave brings its blocks straight into its own part of the LDS, eight rows of 128 bytes a load,
-// DEPTH blocks ahead and without barriers.  (In the order of the operands, 16 bytes of another row in every lane, a load takes the address path some
-// 42 cycles instead of 16.)  Scales come the same way, a lane for each row.
-template <typename T, int MB, int NB, int W, int DEPTH>
+// ---- few rows, or few tiles: the same, but a wave brings its blocks into a part of the LDS of its own ----
+//
+// Eight rows of 128 bytes a load, straight there, DEPTH blocks ahead and without barriers.  (In the order of the operands, 16 bytes of another row in every
+// lane, a load takes the address path some 42 cycles instead of 16.)  Scales come the same way, a lane for each row.  With ANY, where rows are not whole
+// 16-byte pieces, a block passes through registers: it is asked for when the operands of the one before are in theirs, and goes into the LDS behind its
+// products; past a row's end it is as in the tiles below.  (us, so and with the operands' order: 1000 x 200 x 8001 18 and 86, 16 x 3001 x 8001 10 and 22,
+// 1 x 4097 x 4097 7.8 and 10.9, 40 x 3001 x 2001 7.0 and 21.)
+template <typename T, int MB, int NB, int W, int DEPTH, bool ANY>
 __global__ __launch_bounds__(64 * W) void fp8_split_kernel(const LinearParams p)
 {
     constexpr bool WIDE = std::is_same<T, float>::value || MB == 1; // full fp32 sums, also where memory bounds the time anyway
@@ -328,7 +342,40 @@ __global__ __launch_bounds__(64 * W) void fp8_split_kernel(const LinearParams p)
     const float *a_scales = p.a_scales + (int64_t)m0 * p.a_scales_ld, *w_scales = p.w_scales + (int64_t)(n0 / FP8_BLOCK) * p.w_scales_ld;
     uint4 *mine = lds + wave * DEPTH * SLOTS;
     const uint32_t to = (uint32_t)(uintptr_t)(const lds_char *)mine;
+    static_assert(!ANY || DEPTH == 1, "one block is in registers");
+    uint4 held[ANY ? 2 * (MB + NB) : 1];
+    float held_scale;
+    auto past_end = [&](int b) { return max(0, 16 * chunk + 16 - (p.K - b * FP8_BLOCK)); };
+    auto park = [&](int b) {
+        if constexpr (ANY) {
+            reinterpret_cast<float *>(mine + (MB + NB) * 128)[lane] = held_scale;
+            if (p.K - b * FP8_BLOCK >= FP8_BLOCK) {
+#pragma unroll
+                for (int u = 0; u < 2 * (MB + NB); ++u) {
+                    mine[u * 64 + lane] = held[u];
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < 2 * (MB + NB); ++u) {
+                    mine[u * 64 + lane] = without_first_bytes(held[u], past_end(b));
+                }
+            }
+        }
+    };
     auto ask = [&](int b, int slot) {
+        if constexpr (ANY) {
+            const int64_t at = (int64_t)b * FP8_BLOCK - past_end(b);
+            held_scale = *reinterpret_cast<const float *>(reinterpret_cast<const char *>(a_scales + b) + scale_from);
+#pragma unroll
+            for (int u = 0; u < 2 * MB; ++u) {
+                __builtin_memcpy(&held[u], a_tile + at + a_from[u], 16);
+            }
+#pragma unroll
+            for (int u = 0; u < 2 * NB; ++u) {
+                __builtin_memcpy(&held[2 * MB + u], w_tile + at + w_from[u], 16);
+            }
+            return;
+        }
         const uint32_t stage = to + (uint32_t)slot * (SLOTS * 16u);
         load_dword_to_lds(stage + (MB + NB) * 2048u, a_scales + b, scale_from);
         if (16 * chunk < p.K - b * FP8_BLOCK) {
@@ -359,15 +406,18 @@ __global__ __launch_bounds__(64 * W) void fp8_split_kernel(const LinearParams p)
     for (int d = 0; d < DEPTH; ++d) {
         if (wave + d * W < blocks) {
             ask(wave + d * W, d);
+            park(wave + d * W);
         }
     }
     float w_scale = wave < blocks ? w_scales[wave] : 0.f;
     int slot = 0;
     for (int b = wave; b < blocks; b += W) {
-        if (b + (DEPTH - 1) * W < blocks) {
-            wait_for_loads<(DEPTH - 1) * LOADS>();
-        } else {
-            wait_for_loads<0>();
+        if constexpr (!ANY) {
+            if (b + (DEPTH - 1) * W < blocks) {
+                wait_for_loads<(DEPTH - 1) * LOADS>();
+            } else {
+                wait_for_loads<0>();
+            }
         }
         const float ws = w_scale;
         if (b + W < blocks) {
@@ -425,6 +475,9 @@ __global__ __launch_bounds__(64 * W) void fp8_split_kernel(const LinearParams p)
                 }
             }
         }
+        if (b + W < blocks) {
+            park(b + W);
+        }
     }
     __syncthreads(); // the sums take the operands' place
     f32x4 *sums = reinterpret_cast<f32x4 *>(lds);
@@ -447,13 +500,13 @@ __global__ __launch_bounds__(64 * W) void fp8_split_kernel(const LinearParams p)
     }
 }
 
-template <typename T, int MB, int NB, int W, int DEPTH>
+template <typename T, int MB, int NB, int W, int DEPTH, bool ANY>
 int launch_split(LinearParams p, hipStream_t stream)
 {
     static_assert(64 * MB * NB <= DEPTH * ((MB + NB) * 128 + 16), "the sums lie where the operands were");
     constexpr size_t bytes = (size_t)W * DEPTH * ((MB + NB) * 128 + 16) * 16;
     static size_t configured[KUTACC_DEVICE_SLOTS] = {};
-    const auto kernel = &fp8_split_kernel<T, MB, NB, W, DEPTH>;
+    const auto kernel = &fp8_split_kernel<T, MB, NB, W, DEPTH, ANY>;
     const int64_t groups = tiles_of(p, 16 * MB, 16 * NB);
     if (groups > INT32_MAX) {
         return KUTACC_HIP_EUNSUPPORTED;
@@ -475,7 +528,7 @@ int launch_split(LinearParams p, hipStream_t stream)
 constexpr int SPAN = 8; // blocks whose scales are brought at a time
 constexpr size_t tiles_lds(int side) { return 2 * 2 * side * 128 + 2 * SPAN * side * 4 + 2 * 64 * 4; }
 
-template <typename T, int MI, int WM, int WN>
+template <typename T, int MI, int WM, int WN, bool ANY>
 __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(const LinearParams p)
 {
     constexpr bool WIDE = std::is_same<T, float>::value;
@@ -501,9 +554,37 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(const Linear
         from[u] = (uint32_t)min(first + 8 * u + (lane >> 3), rows) * (uint32_t)ld + 16u * (uint32_t)chunk;
     }
     const uint32_t to = (uint32_t)(uintptr_t)(const lds_char *)lds + (brings_a ? 0u : SIDE * 128u) + (uint32_t)first * 128u;
+    // With ANY, where rows are not whole 16-byte pieces, a block passes through registers: asked for a block ahead as well, and put into the LDS before the
+    // barrier that it has to be there at.  Of a cut block a piece past the row's end is the row's last 16 bytes, shifted by as many as are past it.
+    uint4 held[ANY ? 8 : 1];
+    auto past_end = [&](int b) { return max(0, 16 * chunk + 16 - (p.K - b * FP8_BLOCK)); };
+    auto park = [&](int b, int half) {
+        if constexpr (ANY) {
+            uint4 *slot = lds + half * STAGE + (brings_a ? 0 : SIDE * 8) + first * 8 + lane;
+            if (p.K - b * FP8_BLOCK >= FP8_BLOCK) {
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    slot[u * 64] = held[u];
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    slot[u * 64] = without_first_bytes(held[u], past_end(b));
+                }
+            }
+        }
+    };
     auto ask = [&](int b, int half) {
         const uint32_t stage = to + (uint32_t)half * (STAGE * 16u);
         const uint8_t *block = operand + (int64_t)b * FP8_BLOCK;
+        if constexpr (ANY) {
+            block -= past_end(b);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                __builtin_memcpy(&held[u], block + from[u], 16);
+            }
+            return;
+        }
         if (16 * chunk < p.K - b * FP8_BLOCK) {
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
@@ -578,7 +659,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(const Linear
     int place = 0, next = after(block); // where the next block's scales lie; the block after this one
     load_scales(block / SPAN, 0);
     ask(block, 0);
-    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    park(block, 0);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (blocks > 1) {
         if (next / SPAN != block / SPAN) {
             place = 1;
@@ -623,6 +705,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(const Linear
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        if (b + 1 < blocks) {
+            park(next, (b + 1) & 1);
+        }
         // The next block is there, and all have read this one.  (Behind the last block what is read is never used.)
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         take_scales(next, place);
@@ -658,12 +743,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tiles_kernel(const Linear
     }
 }
 
-template <typename T, int MI, int WM, int WN>
+template <typename T, int MI, int WM, int WN, bool ANY>
 int launch_tiles(LinearParams p, hipStream_t stream)
 {
     constexpr int SIDE = 16 * MI * WM;
     static size_t configured[KUTACC_DEVICE_SLOTS] = {};
-    const auto kernel = &fp8_tiles_kernel<T, MI, WM, WN>;
+    const auto kernel = &fp8_tiles_kernel<T, MI, WM, WN, ANY>;
     p.MT = (p.M + SIDE - 1) / SIDE, p.NT = (p.N + SIDE - 1) / SIDE;
     const int64_t tiles = tiles_of(p, SIDE, SIDE);
     if (tiles > INT32_MAX) {
@@ -690,17 +775,39 @@ template <typename T>
 int launch_pieces(const LinearParams &p, hipStream_t stream)
 {
     if (p.M <= 16) {
-        return 2 * tiles_of(p, 16, 64) >= kutacc_cu_count() ? launch_split<T, 1, 4, 8, 1>(p, stream) : launch_split<T, 1, 1, 16, 1>(p, stream);
+        return 2 * tiles_of(p, 16, 64) >= kutacc_cu_count() ? launch_split<T, 1, 4, 8, 1, false>(p, stream) : launch_split<T, 1, 1, 16, 1, false>(p, stream);
     }
     if constexpr (std::is_same<T, bf16_t>::value) { // in fp32 a wave of these has no registers for its widened operands
         if (takes_large_tiles(p, true)) {
-            return launch_tiles<T, 8, 2, 4>(p, stream);
+            return launch_tiles<T, 8, 2, 4, false>(p, stream);
         }
     }
     if (takes_tiles(p, false)) {
-        return launch_tiles<T, 4, 2, 2>(p, stream);
+        return launch_tiles<T, 4, 2, 2, false>(p, stream);
     }
-    return enough(p, 64, 64) ? launch_split<T, 4, 4, 8, 1>(p, stream) : enough(p, 32, 64) ? launch_split<T, 2, 4, 8, 1>(p, stream) : launch_split<T, 2, 2, 16, 1>(p, stream);
+    return enough(p, 64, 64) ? launch_split<T, 4, 4, 8, 1, false>(p, stream) : enough(p, 32, 64) ? launch_split<T, 2, 4, 8, 1, false>(p, stream) : launch_split<T, 2, 2, 16, 1, false>(p, stream);
+}
+
+// Rows on any address, of 16 bytes and more: what passes through registers leaves less of them, so 64 x 64 is not among these, nor with fp32 results 32 x 32;
+// tiles from three for eight CUs on (us, 32 x 32, 32 x 64 and 128 x 128, bf16 results: 40 x 3001 x 2001 7.0, 8.5, 21; 1000 x 200 x 8001 18, 24, 77;
+// 3814 x 112 x 6088 22, 16, 49; 300 x 3001 x 2001 23, 18, 24; 675 x 1751 x 4081 46, 37, 42; 12417 x 128 x 861 27, 20, 13; 4001 x 3001 x 2001 248, 174, 57).
+bool takes_any_tiles(const LinearParams &p) { return p.M > 16 && 8 * tiles_of(p, 128, 128) >= 3 * kutacc_cu_count(); }
+
+template <typename T>
+int launch_bytes(const LinearParams &p, hipStream_t stream)
+{
+    if (p.M <= 16) {
+        return 2 * tiles_of(p, 16, 64) >= kutacc_cu_count() ? launch_split<T, 1, 4, 8, 1, true>(p, stream) : launch_split<T, 1, 1, 16, 1, true>(p, stream);
+    }
+    if (takes_any_tiles(p)) {
+        return launch_tiles<T, 4, 2, 2, true>(p, stream);
+    }
+    if constexpr (std::is_same<T, bf16_t>::value) {
+        if (!enough(p, 32, 64)) {
+            return launch_split<T, 2, 2, 16, 1, true>(p, stream);
+        }
+    }
+    return launch_split<T, 2, 4, 8, 1, true>(p, stream);
 }
 } // namespace
 
@@ -710,12 +817,16 @@ int linear_fp8(const kutacc_hip_linear_fp8_args_t &a, hipStream_t stream)
 {
     const LinearParams p = {(const uint8_t *)a.a, (const uint8_t *)a.w, a.a_scales, a.w_scales, a.bias, a.out, a.a_ld, a.w_ld, a.a_scales_ld,
                             a.w_scales_ld, a.out_ld, (int)a.m, (int)a.n, (int)a.k, 0, 0};
-    // whole 16-byte pieces, and rows of a tile within 32 bits of its first
-    const bool pieces = kutacc_hip_aligned16(a.a) && kutacc_hip_aligned16(a.w) && a.a_ld % 16 == 0 && a.w_ld % 16 == 0 && a.k % 16 == 0 &&
-                        a.a_ld < (1 << 23) && a.w_ld < (1 << 23) && a.a_scales_ld < (1 << 21) && a.w_scales_ld < (1 << 21);
-    const auto run = [&](auto type) { return pieces ? launch_pieces<decltype(type)>(p, stream) : a.m <= 16 ? launch_any<decltype(type), 1, 1, 8, 4>(p, stream) : launch_any<decltype(type), 4, 4, 4, 1>(p, stream); };
-    const char *name = !pieces ? "fp8_any_kernel" : takes_tiles(p, a.dtype == KUTACC_DTYPE_BF16) ? "fp8_tiles_kernel" : "fp8_split_kernel";
-    kutacc_prof::KernelTimer t(name, 2.0 * (double)a.m * (double)a.n * (double)a.k, stream);
+    // rows of a tile within 32 bits of its first; whole 16-byte pieces; at least one piece
+    const bool near = a.a_ld < (1 << 23) && a.w_ld < (1 << 23) && a.a_scales_ld < (1 << 21) && a.w_scales_ld < (1 << 21);
+    const bool pieces = near && kutacc_hip_aligned16(a.a) && kutacc_hip_aligned16(a.w) && a.a_ld % 16 == 0 && a.w_ld % 16 == 0 && a.k % 16 == 0;
+    const bool bytes = near && a.k >= 16;
+    const bool tiles = pieces ? takes_tiles(p, a.dtype == KUTACC_DTYPE_BF16) : bytes && takes_any_tiles(p);
+    const auto run = [&](auto type) {
+        using T = decltype(type);
+        return pieces ? launch_pieces<T>(p, stream) : bytes ? launch_bytes<T>(p, stream) : launch_any<T, 4, 4, 4>(p, stream);
+    };
+    kutacc_prof::KernelTimer t(tiles ? "fp8_tiles_kernel" : pieces || bytes ? "fp8_split_kernel" : "fp8_any_kernel", 2.0 * (double)a.m * (double)a.n * (double)a.k, stream);
     return a.dtype == KUTACC_DTYPE_BF16 ? run(bf16_t{}) : run(float{});
 }
 

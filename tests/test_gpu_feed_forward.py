@@ -274,6 +274,45 @@ def test_linear_fp8_of_rows_on_any_address(m, n, k, pad, offset):
     room.untouched("out")
 
 
+# rows that are no whole 16-byte pieces, in tiles: several spans of scales, one cut block alone, rows of fewer than 16 bytes, a last block of one value
+@pytest.mark.parametrize("out", ["bf16", "fp32"])
+@pytest.mark.parametrize("m,n,k,pad,offset", [(1700, 1500, 2441, 0, 0), (1280, 1100, 7, 0, 0), (1300, 1410, 120, 3, 5), (1201, 1153, 257, 0, 0), (1290, 1164, 384, 1, 0), (1290, 1164, 256, 0, 8),
+                                              (9900, 120, 645, 0, 1)])
+def test_linear_fp8_of_many_rows_on_any_address(out, m, n, k, pad, offset):
+    dt = TYPES[out]
+    a, a_scales, w, w_scales = eight_bits(m + n + k, m, n, k)
+    bias = cpu_randn(5, n, dtype=FP32)
+    room = Room(m, n, dt, n + pad)
+    ok(capi.LinearFp8(placed(a, k + pad, offset), a_scales.cuda(), placed(w, k + pad, offset), w_scales.cuda(), room.view, bias=bias.cuda()))
+    want, off = oracle.linear_fp8(a, a_scales, w, w_scales, bias, dt)
+    oracle.close(room.view, want, oracle.stored(want, off, dt), f"{m} x {n} x {k}")
+    room.untouched("out")
+
+
+# rows of fewer than 16 bytes, of 16 and 17, and a cut block that begins within one; in every form that few rows have
+@pytest.mark.parametrize("out", ["bf16", "fp32"])
+@pytest.mark.parametrize("m,n,k", [(1, 300, 15), (3, 9000, 15), (3, 9000, 17), (16, 8200, 143), (9, 70, 18), (40, 3000, 130), (300, 1100, 129), (700, 900, 19), (30, 70, 2049)])
+def test_linear_fp8_of_few_rows_on_any_address(out, m, n, k):
+    dt = TYPES[out]
+    a, a_scales, w, w_scales = eight_bits(m + n + k, m, n, k)
+    room = Room(m, n, dt)
+    ok(capi.LinearFp8(placed(a, k + 1, 3), a_scales.cuda(), placed(w, None, 1), w_scales.cuda(), room.view))
+    want, off = oracle.linear_fp8(a, a_scales, w, w_scales, None, dt)
+    oracle.close(room.view, want, oracle.stored(want, off, dt), f"{m} x {n} x {k}")
+    room.untouched("out")
+
+
+def test_linear_fp8_of_rows_far_apart():
+    m, n, k, ld = 18, 130, 300, (1 << 23) + 16
+    a, a_scales, w, w_scales = eight_bits(4, m, n, k)
+    memory = torch.zeros(m, ld, device="cuda", dtype=torch.uint8).view(a.dtype)
+    memory[:, :k] = a.cuda()
+    room = Room(m, n, FP32)
+    ok(capi.LinearFp8(memory[:, :k], a_scales.cuda(), w.cuda(), w_scales.cuda(), room.view))
+    want, off = oracle.linear_fp8(a, a_scales, w, w_scales)
+    oracle.close(room.view, want, oracle.stored(want, off, FP32), "out")
+
+
 @pytest.mark.parametrize("m", [3, 200])
 def test_linear_fp8_keeps_a_bad_row_to_itself(m):
     """A row of no numbers, and one with an infinite scale, beside others."""
