@@ -37,7 +37,7 @@ struct TilesParams {
     int64_t c_ld[3];
     int M[3], N[3], tiles[3]; // of the products of WEIGHT_GRADIENTS, which have tiles of their own; else the first alone
     int K, activation;
-    int splits;   // of WEIGHT_GRADIENTS' rows, whose sums then meet in `shares`
+    int splits;   // of k, with WEIGHT_GRADIENTS and INPUT_GRADIENT; their sums then meet in `shares`
     float *shares;
 };
 
@@ -212,6 +212,7 @@ __global__ __launch_bounds__(64 * WM * WN * GROUPS, 2) void ff_pieces_kernel(con
     constexpr bool A_MMAJOR = MODE == WEIGHT_GRADIENTS, B_MMAJOR = MODE == WEIGHT_GRADIENTS || MODE == INPUT_GRADIENT;
     static_assert(!A_MMAJOR || ROWS % 128 == 0, "sub-tiles of M-major operands");
     static_assert(GROUPS == 1 || MODE == PLAIN || MODE == INPUT_GRADIENT, "sums that meet in the LDS");
+    constexpr bool SPLIT = (MODE == WEIGHT_GRADIENTS || MODE == INPUT_GRADIENT) && MI == 2 && GROUPS == 1;
     extern __shared__ uint4 all_lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int group = wave / (WM * WN), member = wave % (WM * WN);
@@ -226,7 +227,7 @@ __global__ __launch_bounds__(64 * WM * WN * GROUPS, 2) void ff_pieces_kernel(con
     }
     int which = 0, split = 0;
     const unsigned place = tile; // of a share of the sums
-    if constexpr (MODE == WEIGHT_GRADIENTS) { // (all tiles of a range of rows, which share them, and then the next range's)
+    if constexpr (MODE == WEIGHT_GRADIENTS || SPLIT) { // (all tiles of a range of k, which share it, and then the next range's)
         const unsigned all = (unsigned)(p.tiles[0] + p.tiles[1] + p.tiles[2]);
         split = __builtin_amdgcn_readfirstlane((int)(tile / all)), tile = (unsigned)__builtin_amdgcn_readfirstlane((int)(tile % all));
         while (which < 2 && tile >= (unsigned)p.tiles[which]) {
@@ -243,7 +244,7 @@ __global__ __launch_bounds__(64 * WM * WN * GROUPS, 2) void ff_pieces_kernel(con
     // stages of the first list of products (and of the second, as many)
     const int all_stages = (p.K + 63) / 64;
     int first_stage = 0, stages = all_stages;
-    if constexpr (MODE == WEIGHT_GRADIENTS) {
+    if constexpr (SPLIT) {
         first_stage = __builtin_amdgcn_readfirstlane((int)((int64_t)all_stages * split / p.splits));
         stages = __builtin_amdgcn_readfirstlane((int)((int64_t)all_stages * (split + 1) / p.splits)) - first_stage;
     }
@@ -430,7 +431,7 @@ __global__ __launch_bounds__(64 * WM * WN * GROUPS, 2) void ff_pieces_kernel(con
         run(std::true_type{});
     }
 
-    if constexpr (MODE == WEIGHT_GRADIENTS && MI == 2) {
+    if constexpr (SPLIT) {
         if (p.splits > 1) { // a share of the sums, lane by lane: [split][tile of all three][wave][MI][2][4][64] of 16 bytes
             f32x4 *share = reinterpret_cast<f32x4 *>(p.shares) + ((int64_t)place * (WM * WN) + member) * (MI * 2 * 4 * 64) + lane;
 #pragma unroll
@@ -528,7 +529,7 @@ __global__ __launch_bounds__(64 * WM * WN * GROUPS, 2) void ff_pieces_kernel(con
     }
 }
 
-// The weights' gradients from their shares: a thread adds four columns of a row over the splits, in one order.
+// The result of split products from its shares: a thread adds four columns of a row over the splits, in one order.
 template <int MI, int WM, int WN>
 __global__ __launch_bounds__(256) void ff_shares_kernel(const TilesParams p)
 {
@@ -743,7 +744,7 @@ int launch_pieces(TilesParams p, hipStream_t stream)
         return kutacc_hip_status(e);
     }
     kernel<<<dim3((unsigned)groups), 64 * WM * WN * GROUPS, LDS, stream>>>(p);
-    if (MODE == WEIGHT_GRADIENTS && MI == 2 && p.splits > 1) {
+    if ((MODE == WEIGHT_GRADIENTS || MODE == INPUT_GRADIENT) && MI == 2 && GROUPS == 1 && p.splits > 1) {
         ff_shares_kernel<MI, WM, WN><<<dim3((unsigned)(tiles * WM * WN * MI * 2)), 256, 0, stream>>>(p);
     }
     return kutacc_hip_status(hipGetLastError());
@@ -825,6 +826,9 @@ int launch_whole(const TilesParams &p, hipStream_t stream)
         constexpr Choice choices[] = {{128, 64, 2, 1.0f}, {192, 128, 1, 1.27f}};
         return least(p, choices) == 0 ? launch_pieces<MODE, 2, 2, 2, 1>(p, stream) : launch_pieces<MODE, 3, 2, 4, 1>(p, stream);
     } else if constexpr (MODE == INPUT_GRADIENT) {
+        if (p.splits > 1) {
+            return launch_pieces<MODE, 2, 2, 2, 1>(p, stream);
+        }
         constexpr Choice choices[] = {{128, 128, 1, 0.61f}, {128, 128, 2, 0.97f}, {256, 256, 1, 1.55f}};
         switch (least(p, choices)) {
         case 0: return launch_pieces<MODE, 2, 2, 2, 2>(p, stream);
@@ -857,10 +861,25 @@ int weight_splits(int64_t rows, int64_t c_o, int64_t c_i)
     const int64_t tiles = count_tiles(p, 128, 128), stages = (rows + 63) / 64;
     return (int)std::max<int64_t>(1, std::min<int64_t>(2 * kutacc_cu_count() / tiles, stages / 8));
 }
+// How many ways the hidden units are split for the gradient of x, where its tiles leave half of the CUs and more without work: into ranges of at least four
+// stages, and only where that saves more than the shares cost, all in us: a stage of both products takes 1.15, a share of a tile 0.033 to write and read, the
+// kernel that adds them 3.  (us, the whole backward pass, unsplit and split: 300 x 512 x 2048 64 and 42, 93 x 512 x 1024 42 and 35, 2 x 2048 x 8192 187 and 96,
+// 1000 x 1024 x 4096 137 and 106, 4000 x 384 x 1536 87 and 85, 5618 x 256 x 1024 70 and 71.)
+int input_splits(int64_t rows, int64_t c_o, int64_t c_i)
+{
+    TilesParams p = {};
+    p.M[0] = (int)rows, p.N[0] = (int)c_o;
+    const int64_t tiles = count_tiles(p, 128, 128), stages = (c_i + 63) / 64;
+    if (2 * tiles > kutacc_cu_count()) {
+        return 1;
+    }
+    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(2 * kutacc_cu_count() / std::max<int64_t>(tiles, 1), stages / 4));
+    return 1.15 * (double)stages * (double)(splits - 1) > (3 + 0.033 * (double)(tiles * splits)) * (double)splits ? (int)splits : 1;
+}
 int64_t shares_bytes(int64_t rows, int64_t c_o, int64_t c_i)
 {
-    const int64_t splits = weight_splits(rows, c_o, c_i);
-    return splits == 1 ? 0 : splits * ((c_i + 127) / 128) * ((c_o + 127) / 128) * 3 * 128 * 128 * 4;
+    const int64_t weights = weight_splits(rows, c_o, c_i), input = input_splits(rows, c_o, c_i), across = (c_o + 127) / 128, tile = 128 * 128 * 4;
+    return std::max(weights == 1 ? 0 : weights * ((c_i + 127) / 128) * across * 3 * tile, input == 1 ? 0 : input * ((rows + 127) / 128) * across * tile);
 }
 
 int64_t padded(int64_t v) { return (v + 31) / 32 * 32; }
@@ -910,6 +929,7 @@ int gated_transition_backward(const kutacc_hip_gated_transition_backward_args_t 
     }
     const int64_t rows = a.rows, c_o = a.c_o, c_i = a.c_i, ld = padded(c_i), each = align256(2 * rows * ld) / 2;
     bf16_t *h = (bf16_t *)a.workspace, *dg = h + each, *du = dg + each;
+    float *shares = reinterpret_cast<float *>(du + each);
     const bf16_t *x = (const bf16_t *)a.x, *dy = (const bf16_t *)a.grad_out;
     const bf16_t *wg = (const bf16_t *)a.gate_w, *wu = (const bf16_t *)a.up_w, *wd = (const bf16_t *)a.down_w;
     const double flops = 2.0 * (double)rows * (double)c_o * (double)c_i;
@@ -927,7 +947,8 @@ int gated_transition_backward(const kutacc_hip_gated_transition_backward_args_t 
     }
     if (a.grad_x != nullptr) {
         TilesParams d = {};
-    d.splits = 1;
+        d.splits = input_splits(rows, c_o, c_i);
+        d.shares = shares;
         d.product[0] = {dg, wg, ld, c_o};
         d.product[1] = {du, wu, ld, c_o};
         d.c[0] = (bf16_t *)a.grad_x, d.c_ld[0] = a.grad_x_ld;
@@ -951,7 +972,7 @@ int gated_transition_backward(const kutacc_hip_gated_transition_backward_args_t 
     add({dy, h, a.grad_out_ld, ld}, a.grad_down_w, c_o, c_i);
     const bool aligned = (!a.grad_gate_w || kutacc_hip_aligned16(a.grad_gate_w)) && (!a.grad_up_w || kutacc_hip_aligned16(a.grad_up_w)) && (!a.grad_down_w || kutacc_hip_aligned16(a.grad_down_w));
     w.splits = weight_splits(rows, c_o, c_i);
-    w.shares = reinterpret_cast<float *>(du + each);
+    w.shares = shares;
     return count == 0 ? 0 : launch<WEIGHT_GRADIENTS>(w, !rows_fit || !widths || !aligned, count * flops, "gated_transition<weight gradients>", stream);
 }
 
