@@ -570,7 +570,7 @@ def run_all(calls, stream=None):
         assert rc == 0, (type(call).__name__, rc)
 
 
-@pytest.mark.parametrize("rows,c,c_i", [(3, 512, 1024), (700, 128, 512), (400, 384, 640)])
+@pytest.mark.parametrize("rows,c,c_i", [(3, 512, 1024), (700, 128, 512), (400, 384, 640), (100, 64, 128), (13000, 128, 512), (200, 131, 259)])
 def test_captured_and_replayed(rows, c, c_i):
     calls, results, x = operators_of_everything(rows, c, c_i, 1)
     run_all(calls)
@@ -610,6 +610,57 @@ def test_two_at_once_on_streams_of_their_own():
     torch.cuda.synchronize()
     for (_, results, _), w in zip(sets, want):
         assert all(torch.equal(a, r.view(torch.uint8)) for a, r in zip(w, results))
+
+
+@pytest.mark.parametrize("c", [128, 127])
+def test_more_elements_than_32_bits_count(c):
+    """The first and the last rows of calls whose operands end past 2^31 elements; the gradient of out is zero but in the last ones."""
+    c_i, last = 32, 40
+    rows = (1 << 31) // c + 3 * last
+    w, gamma = weights_of(7, c, c_i), 1 + 0.1 * cpu_randn(3, c, dtype=FP32)
+    gpu, x_last, dy_last = [t.cuda() for t in w], cpu_randn(1, last, c), cpu_randn(2, last, c)
+    x, dy = torch.zeros(rows, c, device="cuda", dtype=BF16), torch.zeros(rows, c, device="cuda", dtype=BF16)
+    x[:last], x[-last:], dy[-last:] = x_last.cuda(), x_last.cuda(), dy_last.cuda()
+    out, grads = torch.ones_like(x), [torch.empty_like(t) for t in gpu]
+
+    def check(got, want, dtype, what):
+        oracle.close(got, want[0], oracle.stored(want[0], want[1], dtype), what)
+
+    want = oracle.gated_transition(x_last, *w, "silu", dy_last)
+    ok(capi.GatedTransition(x, *gpu, out))
+    check(out[:last], want["out"], BF16, "the first rows")
+    check(out[-last:], want["out"], BF16, "the last rows")
+    assert not bool(out[last:-last].any())
+    ok(capi.GatedTransitionBackward(x, *gpu, dy, out, *grads))
+    check(out[-last:], want["grad_x"], BF16, "grad_x")
+    assert not bool(out[:-last].any())
+    for name, g in zip(("grad_gate_w", "grad_up_w", "grad_down_w"), grads):
+        check(g, want[name], BF16, name)
+
+    s64, y64 = oracle.rms_norm(x_last, gamma, EPS)
+    out8, scales = torch.empty(rows, c, device="cuda", dtype=E4M3), torch.empty(rows, 1, device="cuda")
+    ok(capi.RmsNorm(x, gamma.cuda(), EPS, out=out, out8=out8, scales=scales))
+    near = [torch.empty(last, c, device="cuda", dtype=t.dtype) for t in (out, out8)] + [torch.empty(last, 1, device="cuda")]
+    ok(capi.RmsNorm(x_last.cuda(), gamma.cuda(), EPS, out=near[0], out8=near[1], scales=near[2]))
+    for a, b in zip((out, out8, scales), near):
+        assert torch.equal(a[:last].view(torch.uint8), b.view(torch.uint8)) and torch.equal(a[-last:].view(torch.uint8), b.view(torch.uint8))
+    dgamma, want_dgamma = torch.empty(c, device="cuda"), torch.empty(c, device="cuda")
+    near_dx = torch.empty(last, c, device="cuda", dtype=BF16)
+    ok(capi.RmsNormBackward(x, gamma.cuda(), dy, EPS, grad_x=out, grad_gamma=dgamma))
+    ok(capi.RmsNormBackward(x_last.cuda(), gamma.cuda(), dy_last.cuda(), EPS, grad_x=near_dx, grad_gamma=want_dgamma))
+    assert torch.equal(out[-last:], near_dx) and not bool(out[:-last].any())
+    # sums of 40 products, in two orders
+    bound = 2 * 40 * oracle.ADD * (dy_last.double().abs() * y64.abs() / gamma.double().abs()).sum(0) * (1 + 2 ** -10)
+    assert bool(((dgamma - want_dgamma).double().cpu().abs() <= bound).all())
+
+    w8, w_scales = torch.empty(24, c, device="cuda", dtype=E4M3), torch.empty(1, 1, device="cuda")
+    ok(capi.QuantizeFp8(cpu_randn(9, 24, c).cuda(), w8, w_scales, 128))
+    product, near_product = torch.empty(rows, 24, device="cuda", dtype=BF16), torch.empty(last, 24, device="cuda", dtype=BF16)
+    ok(capi.LinearFp8(out8, scales, w8, w_scales, product))
+    ok(capi.LinearFp8(near[1], near[2], w8, w_scales, near_product))
+    want, off = oracle.linear_fp8(near[1].cpu(), near[2].cpu(), w8.cpu(), w_scales.cpu(), None, BF16)
+    for got in (product[:last], product[-last:], near_product):
+        check(got, (want, off), BF16, "product")
 
 
 def test_calls_of_no_rows_do_nothing():
