@@ -918,12 +918,18 @@ int gated_transition(const kutacc_hip_gated_transition_args_t &a, hipStream_t st
 
 int64_t gated_transition_backward_workspace(int64_t rows, int64_t c_o, int64_t c_i)
 {
-    const int64_t bytes = 3 * align256(2 * rows * padded(c_i)) + shares_bytes(rows, c_o, c_i);
+    int64_t bytes = 3 * align256(2 * rows * padded(c_i)) + shares_bytes(rows, c_o, c_i);
+    if (gated_few_rows_backward_fits(rows, c_o, c_i)) {
+        bytes = std::max(bytes, gated_few_rows_backward_workspace(rows, c_o, c_i));
+    }
     return c_o == 64 || c_o == 128 ? std::max(bytes, gated_rows_backward_workspace(rows, c_o, c_i)) : bytes;
 }
 
 int gated_transition_backward(const kutacc_hip_gated_transition_backward_args_t &a, hipStream_t stream)
 {
+    if (gated_few_rows_backward_takes(a)) {
+        return gated_few_rows_backward(a, stream);
+    }
     if (gated_rows_backward_takes(a)) {
         return gated_rows_backward(a, stream);
     }

@@ -234,6 +234,12 @@ bool gated_rows_backward_takes(const kutacc_hip_gated_transition_backward_args_t
 int64_t gated_rows_backward_workspace(int64_t rows, int64_t c_o, int64_t c_i);
 int gated_rows_backward(const kutacc_hip_gated_transition_backward_args_t &args, hipStream_t stream);
 
+// gated_few_rows_backward.hip: the backward pass of up to 64 rows
+bool gated_few_rows_backward_fits(int64_t rows, int64_t c_o, int64_t c_i);
+int64_t gated_few_rows_backward_workspace(int64_t rows, int64_t c_o, int64_t c_i);
+bool gated_few_rows_backward_takes(const kutacc_hip_gated_transition_backward_args_t &args);
+int gated_few_rows_backward(const kutacc_hip_gated_transition_backward_args_t &args, hipStream_t stream);
+
 // gated_transition.hip
 int64_t gated_transition_workspace(int64_t rows, int64_t c_o, int64_t c_i);
 int gated_transition(const kutacc_hip_gated_transition_args_t &args, hipStream_t stream);

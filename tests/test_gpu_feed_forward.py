@@ -444,9 +444,27 @@ def test_gated_transition_backward_on_chip(activation, rows, c_o, c_i, pad):
         room.untouched(name)
 
 
-def test_gated_transition_backward_keeps_a_bad_row_to_itself():
+# up to 64 rows: one block of 32 and two, full and not; fewer channels than waves share, and as many as the LDS holds
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("rows,c_o,c_i,pad", [(1, 2048, 96, 0), (64, 1024, 1024, 8), (63, 96, 32, 0), (32, 32, 32, 8), (33, 32, 64, 0), (17, 1056, 160, 16), (64, 2048, 32, 0), (2, 160, 4096, 0)])
+def test_gated_transition_backward_of_few_rows(activation, rows, c_o, c_i, pad):
+    w = weights_of(rows, c_o, c_i)
+    gpu, x, dy = [t.cuda() for t in w], cpu_randn(1, rows, c_o), cpu_randn(2, rows, c_o)
+    want = oracle.gated_transition(x, *w, activation, dy)
+    grads = dict(grad_x=Room(rows, c_o, BF16, c_o + pad), grad_gate_w=Room(c_i, c_o, BF16), grad_up_w=Room(c_i, c_o, BF16), grad_down_w=Room(c_o, c_i, BF16))
+    ok(capi.GatedTransitionBackward(placed(x, c_o + pad), *gpu, placed(dy, c_o + 2 * pad), activation=activation, **{k: r.view for k, r in grads.items()}))
+    for name, r in grads.items():
+        oracle.close(r.view, want[name][0], oracle.stored(*want[name], BF16), name)
+        r.untouched(name)
+        room = Room(*r.view.shape, BF16)  # and alone
+        ok(capi.GatedTransitionBackward(placed(x, c_o + pad), *gpu, placed(dy, c_o + 2 * pad), activation=activation, **{name: room.view}))
+        assert torch.equal(room.view, r.view), name
+
+
+@pytest.mark.parametrize("rows", [40, 90])
+def test_gated_transition_backward_keeps_a_bad_row_to_itself(rows):
     """In the gradient of x; the weights' gradients are not-a-number where the sum over the rows is, the last row's included where its block of 32 is not full."""
-    rows, c_o, c_i = 40, 128, 256
+    c_o, c_i = 128, 256
     w = weights_of(1, c_o, c_i)
     x, dy = cpu_randn(1, rows, c_o), cpu_randn(2, rows, c_o)
     dy[rows - 1, 5] = math.nan
