@@ -411,7 +411,9 @@ int by_type(int32_t dtype, F f)
     return dtype == KUTACC_DTYPE_BF16 ? f(bf16_t{}) : f(float{});
 }
 
-// workgroups of the backward pass, each with its share of dgamma
+// Workgroups of the backward pass, each with its share of dgamma.  One alone writes dgamma itself, which saves the second kernel where it has few rounds of
+// rows to go through (us, so and with shares: 2 x 1256 4.7 and 8.1, 8 x 1024 5.3 and 7.3, 16 x 512 (four rounds) 5.4 and 7.3, 3 x 8192 (three) 8.1 and 7.4,
+// 4 x 8192 10.2 and 7.8).
 int64_t backward_groups(int64_t rows, int64_t size)
 {
     int per_group = 1;
@@ -420,6 +422,9 @@ int64_t backward_groups(int64_t rows, int64_t size)
         return 0;
     });
     const int64_t needed = (rows + per_group - 1) / per_group;
+    if (needed <= (size <= 2048 ? 4 : 2)) {
+        return 1;
+    }
     return std::min<int64_t>(needed, (size <= 1024 ? 8 : 2) * (int64_t)kutacc_cu_count());
 }
 } // namespace
@@ -449,7 +454,7 @@ int64_t rms_norm_backward_workspace(int64_t rows, int64_t size) { return backwar
 int rms_norm_backward(const kutacc_hip_rms_norm_backward_args_t &a, hipStream_t stream)
 {
     const int64_t groups = backward_groups(a.rows, a.size);
-    const BackwardParams p = {a.x, a.grad_out, a.grad_sum, a.gamma, a.grad_x, a.grad_gamma != nullptr ? (float *)a.workspace : nullptr,
+    const BackwardParams p = {a.x, a.grad_out, a.grad_sum, a.gamma, a.grad_x, groups == 1 || a.grad_gamma == nullptr ? a.grad_gamma : (float *)a.workspace,
                               a.x_ld, a.grad_out_ld, a.grad_sum_ld, a.grad_x_ld, a.rows, (int)a.size, a.eps};
     const int rc = by_type(a.dtype, [&](auto type) {
         return by_size(a.size, [&](auto tpr, auto nv) {
@@ -459,7 +464,7 @@ int rms_norm_backward(const kutacc_hip_rms_norm_backward_args_t &a, hipStream_t 
             return kutacc_hip_status(hipGetLastError());
         });
     });
-    if (rc != 0 || a.grad_gamma == nullptr) {
+    if (rc != 0 || a.grad_gamma == nullptr || groups == 1) {
         return rc;
     }
     kutacc_prof::KernelTimer t("column_sums_kernel", (double)groups * (double)a.size, stream);

@@ -174,6 +174,18 @@ def test_rms_norm_backward_on_any_address_and_in_place():
     oracle.close(dgamma, want_gamma, off_gamma + 2.0 ** -24 * want_gamma.abs(), "grad_gamma alone")
 
 
+# few enough rows for a workgroup alone, which writes dgamma itself: on any address, and not past its end
+@pytest.mark.parametrize("rows,size", [(1, 5), (3, 130), (4, 1999), (8, 1024), (7, 600), (16, 509), (100, 40), (2, 8193), (2, 16384)])
+def test_rms_norm_backward_of_few_rows(rows, size):
+    x, dy, gamma = cpu_randn(1, rows, size), cpu_randn(2, rows, size), 1 + 0.1 * cpu_randn(4, size, dtype=FP32)
+    want, off, want_gamma, off_gamma = oracle.rms_norm_backward(x, gamma, dy, EPS, None)
+    dx, dgamma = Room(rows, size, BF16), Room(1, size, FP32, size, 1)
+    ok(capi.RmsNormBackward(x.cuda(), gamma.cuda(), dy.cuda(), EPS, grad_x=dx.view, grad_gamma=dgamma.view.view(size)))
+    oracle.close(dx.view, want, oracle.stored(want, off, BF16), "grad_x")
+    oracle.close(dgamma.view.view(size), want_gamma, off_gamma + 2.0 ** -24 * want_gamma.abs(), "grad_gamma")
+    dx.untouched("grad_x"), dgamma.untouched("grad_gamma")
+
+
 def test_rms_norm_backward_against_differences():
     rows, size, step = 3, 40, 1e-6
     x, dy, gamma = cpu_randn(1, rows, size, dtype=FP32), cpu_randn(2, rows, size, dtype=FP32), 1 + 0.1 * cpu_randn(3, size, dtype=FP32)
