@@ -167,8 +167,10 @@ struct BackwardParams {
 };
 
 // A workgroup walks rows, ROWS at a time, and keeps its share of dgamma in registers.  The shares meet in the LDS and then, in another kernel,
-// over the workgroups, always in one order.
-template <typename T, int TPR, int NV>
+// over the workgroups, always in one order.  With AHEAD the next rows are on their way while these are reduced and written, as they lie in memory: values
+// that a load's own branch converts are waited for there.  us, so and with converted values: bf16 with grad_sum, 5696 x 4096 43.9 and 66.8 (floor 38.3),
+// 4238 x 2334 33 and 62, 147456 x 128 35.8 and 37.7 (31.0); fp32 50000 x 256 41.9 (42.0).  TINY: rows of fewer than eight elements.
+template <typename T, int TPR, int NV, bool TINY>
 __global__ __launch_bounds__(threads_of<TPR>()) void rms_norm_backward_kernel(const BackwardParams p)
 {
     constexpr int THREADS = threads_of<TPR>(), ROWS = THREADS / TPR;
@@ -196,22 +198,33 @@ __global__ __launch_bounds__(threads_of<TPR>()) void rms_norm_backward_kernel(co
             share[i][e] = 0.f;
         }
     }
+    const bool adds = p.grad_sum != nullptr;
     struct Row {
-        float x[NV][8], dy[NV][8];
+        RawChunk<T> x[AHEAD ? NV : 1], dy[AHEAD ? NV : 1], ds[AHEAD ? NV : 1];
+        float x32[AHEAD ? 1 : NV][8], dy32[AHEAD ? 1 : NV][8];
         bool there;
         int64_t at;
     } now, next;
     auto load = [&](Row &row, int64_t first) {
         row.there = first + group < p.rows;
-        row.at = row.there ? first + group : 0;
-        const int size = row.there ? p.size : 0;
+        row.at = row.there ? first + group : 0; // a row past the last brings the first one, and leaves nothing
+        const T *x = (const T *)p.x + row.at * p.x_ld, *dy = (const T *)p.grad_out + row.at * p.grad_out_ld;
+        if constexpr (AHEAD && !TINY) {
+            const T *ds = adds ? (const T *)p.grad_sum + row.at * p.grad_sum_ld : dy; // without grad_sum, grad_out once more: a branch would wait for what it brings
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            load_chunk(row.x[i], (const T *)p.x + row.at * p.x_ld, 8 * (TPR * i + t), size);
-        }
+            for (int i = 0; i < NV; ++i) {
+                const int c = 8 * (TPR * i + t);
+                ask_chunk(row.x[i], x, c, p.size), ask_chunk(row.dy[i], dy, c, p.size), ask_chunk(row.ds[i], ds, c, p.size);
+            }
+        } else if constexpr (!AHEAD) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            load_chunk(row.dy[i], (const T *)p.grad_out + row.at * p.grad_out_ld, 8 * (TPR * i + t), size);
+            for (int i = 0; i < NV; ++i) {
+                load_chunk(row.x32[i], x, 8 * (TPR * i + t), p.size);
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                load_chunk(row.dy32[i], dy, 8 * (TPR * i + t), p.size);
+            }
         }
     };
     const int64_t step = (int64_t)gridDim.x * ROWS;
@@ -224,9 +237,21 @@ __global__ __launch_bounds__(threads_of<TPR>()) void rms_norm_backward_kernel(co
         if constexpr (!AHEAD) {
             load(now, first);
         } else if (more) {
-            load(next, first + step); // on its way while this one is reduced and written
+            load(next, first + step);
         }
-        const int size = now.there ? p.size : 0;
+        auto take = [&](float (&x)[8], float (&dy)[8], int i) {
+            const int c = 8 * (TPR * i + t);
+            if constexpr (TINY) {
+                load_chunk(x, (const T *)p.x + now.at * p.x_ld, c, p.size), load_chunk(dy, (const T *)p.grad_out + now.at * p.grad_out_ld, c, p.size);
+            } else if constexpr (AHEAD) {
+                unpack(x, now.x[i], c, p.size), unpack(dy, now.dy[i], c, p.size);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = now.x32[i][e], dy[e] = now.dy32[i][e];
+                }
+            }
+        };
         float squares = 0.f, products = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -234,10 +259,12 @@ __global__ __launch_bounds__(threads_of<TPR>()) void rms_norm_backward_kernel(co
                 load_gamma(gamma[0], i);
             }
             constexpr int KEPT = AHEAD ? 1 : 0;
+            float x[8], dy[8];
+            take(x, dy, i);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                squares = fmaf(now.x[i][e], now.x[i][e], squares);
-                products = fmaf(now.dy[i][e] * gamma[KEPT * i][e], now.x[i][e], products);
+                squares = fmaf(x[e], x[e], squares);
+                products = fmaf(dy[e] * gamma[KEPT * i][e], x[e], products);
             }
         }
         const float n = (float)p.size;
@@ -247,22 +274,25 @@ __global__ __launch_bounds__(threads_of<TPR>()) void rms_norm_backward_kernel(co
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = 8 * (TPR * i + t);
-            float dx[8];
             if constexpr (!AHEAD) {
                 load_gamma(gamma[0], i);
             }
             constexpr int KEPT = AHEAD ? 1 : 0;
-            if (p.grad_sum != nullptr) {
-                load_chunk(dx, (const T *)p.grad_sum + now.at * p.grad_sum_ld, c, size);
+            float x[8], dy[8], dx[8];
+            take(x, dy, i);
+            if (adds && AHEAD && !TINY) {
+                unpack(dx, now.ds[AHEAD ? i : 0], c, p.size);
+            } else if (adds) {
+                load_chunk(dx, (const T *)p.grad_sum + now.at * p.grad_sum_ld, c, p.size);
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float own = r * (now.dy[i][e] * gamma[KEPT * i][e] - now.x[i][e] * pull);
-                dx[e] = p.grad_sum != nullptr ? dx[e] + own : own;
-                share[i][e] = now.there ? fmaf(now.dy[i][e] * now.x[i][e], r, share[i][e]) : share[i][e];
+                const float own = r * (dy[e] * gamma[KEPT * i][e] - x[e] * pull);
+                dx[e] = adds ? dx[e] + own : own;
+                share[i][e] = now.there ? fmaf(dy[e] * x[e], r, share[i][e]) : share[i][e];
             }
             if (p.grad_x != nullptr) {
-                store_chunk(dx, (T *)p.grad_x + now.at * p.grad_x_ld, c, size);
+                store_chunk(dx, (T *)p.grad_x + now.at * p.grad_x_ld, c, now.there ? p.size : 0);
             }
         }
         if (AHEAD && more) {
@@ -411,10 +441,12 @@ int by_type(int32_t dtype, F f)
     return dtype == KUTACC_DTYPE_BF16 ? f(bf16_t{}) : f(float{});
 }
 
-// Workgroups of the backward pass, each with its share of dgamma.  One alone writes dgamma itself, which saves the second kernel where it has few rounds of
-// rows to go through (us, so and with shares: 2 x 1256 4.7 and 8.1, 8 x 1024 5.3 and 7.3, 16 x 512 (four rounds) 5.4 and 7.3, 3 x 8192 (three) 8.1 and 7.4,
-// 4 x 8192 10.2 and 7.8).
-int64_t backward_groups(int64_t rows, int64_t size)
+// Workgroups of the backward pass, each with its share of dgamma: as many as are on the chip at a time.  One alone writes dgamma itself, which saves the second
+// kernel where it has few rounds of rows to go through (us, so and with shares: 2 x 1256 4.7 and 8.1, 8 x 1024 5.3 and 7.3, 16 x 512 (four rounds) 5.4 and 7.3,
+// 3 x 8192 (three) 8.1 and 7.4, 4 x 8192 10.2 and 7.8).  Four for a CU with short rows of bf16, else two (two, four and eight: 147456 x 128 bf16 33.7, 28.9, 31.0,
+// fp32 45, 50, 50; 20000 x 512 20.5, 19.4, 21.6, fp32 28, 32, 33; 10000 x 1024 18.4, 21.4, 24.7), and one where a row's
+// threads fill the CU (one and two: 2000 x 8192 34.4 and 40.2, 700 x 12000 24.3 and 30.7).
+int64_t backward_groups(int64_t rows, int64_t size, bool bf16)
 {
     int per_group = 1;
     (void)by_size(size, [&](auto tpr, auto) {
@@ -425,7 +457,7 @@ int64_t backward_groups(int64_t rows, int64_t size)
     if (needed <= (size <= 2048 ? 4 : 2)) {
         return 1;
     }
-    return std::min<int64_t>(needed, (size <= 1024 ? 8 : 2) * (int64_t)kutacc_cu_count());
+    return std::min<int64_t>(needed, (size <= 512 && bf16 ? 4 : size <= 4096 ? 2 : 1) * (int64_t)kutacc_cu_count());
 }
 } // namespace
 
@@ -449,18 +481,22 @@ int rms_norm(const kutacc_hip_rms_norm_args_t &a, hipStream_t stream)
     });
 }
 
-int64_t rms_norm_backward_workspace(int64_t rows, int64_t size) { return backward_groups(rows, size) * size * (int64_t)sizeof(float); }
+int64_t rms_norm_backward_workspace(int64_t rows, int64_t size) { return backward_groups(rows, size, true) * size * (int64_t)sizeof(float); }
 
 int rms_norm_backward(const kutacc_hip_rms_norm_backward_args_t &a, hipStream_t stream)
 {
-    const int64_t groups = backward_groups(a.rows, a.size);
+    const int64_t groups = backward_groups(a.rows, a.size, a.dtype == KUTACC_DTYPE_BF16);
     const BackwardParams p = {a.x, a.grad_out, a.grad_sum, a.gamma, a.grad_x, groups == 1 || a.grad_gamma == nullptr ? a.grad_gamma : (float *)a.workspace,
                               a.x_ld, a.grad_out_ld, a.grad_sum_ld, a.grad_x_ld, a.rows, (int)a.size, a.eps};
     const int rc = by_type(a.dtype, [&](auto type) {
         return by_size(a.size, [&](auto tpr, auto nv) {
             constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
             kutacc_prof::KernelTimer t("rms_norm_backward_kernel", 12.0 * (double)p.rows * (double)p.size, stream);
-            rms_norm_backward_kernel<decltype(type), TPR, NV><<<dim3((unsigned)groups), threads_of<TPR>(), 0, stream>>>(p);
+            if (TPR == 8 && p.size < 8) {
+                rms_norm_backward_kernel<decltype(type), 8, 1, true><<<dim3((unsigned)groups), threads_of<TPR>(), 0, stream>>>(p);
+            } else {
+                rms_norm_backward_kernel<decltype(type), TPR, NV, false><<<dim3((unsigned)groups), threads_of<TPR>(), 0, stream>>>(p);
+            }
             return kutacc_hip_status(hipGetLastError());
         });
     });

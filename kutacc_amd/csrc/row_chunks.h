@@ -49,6 +49,43 @@ __device__ __forceinline__ void store_chunk(const float (&v)[8], T *row, int at,
     }
 }
 
+// A chunk on its way, as it lies in memory: asked for without a branch, so that nothing waits for it before unpack() does.  Rows of at least eight elements; a
+// chunk past the row's end is read in front of it, and unpack() shifts it into place.
+template <typename T>
+struct RawChunk {
+    uint4 v[sizeof(T) / 2];
+};
+__device__ __forceinline__ int past_end(int at, int size) { return max(0, at + 8 - size); }
+template <typename T>
+__device__ __forceinline__ void ask_chunk(RawChunk<T> &raw, const T *row, int at, int size)
+{
+    __builtin_memcpy(&raw, row + at - past_end(at, size), sizeof(raw));
+}
+template <typename T>
+__device__ __forceinline__ void unpack(float (&v)[8], const RawChunk<T> &raw, int at, int size)
+{
+    T values[8];
+    __builtin_memcpy(values, &raw, sizeof(values));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        v[e] = to_f32(values[e]);
+    }
+    const int past = past_end(at, size);
+    if (size % 8 != 0) {
+#pragma unroll
+        for (int shift = 1; shift < 8; shift *= 2) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] = (past & shift) == 0 ? v[e] : e + shift < 8 ? v[e + shift] : 0.f;
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        v[e] = past < 8 ? v[e] : 0.f;
+    }
+}
+
 // ---- e4m3 (OCP: largest value 448, no infinities) with a scale ----
 
 constexpr int FP8_BLOCK = 128; // values along a row that share a scale
