@@ -422,7 +422,10 @@ typedef struct kutacc_hip_msa_attention_args {
 kutacc_export int64_t kutacc_hip_msa_attention_workspace(int64_t n_seq, int64_t n_res, int64_t nheads, int32_t column);
 kutacc_export int kutacc_hip_msa_attention(const kutacc_hip_msa_attention_args_t *args, void *stream);
 
-/* ---- the feed-forward half of a transformer block (no counterpart in the reference) ---- */
+/* ---- the feed-forward half of a transformer block (no counterpart in the reference) ----
+ *
+ * Calls enqueue their kernels on `stream` and return 0, a hipError_t, KUTACC_HIP_EINVAL or KUTACC_HIP_EUNSUPPORTED.  A first call on a device raises a kernel's
+ * dynamic-LDS limit: make one per shape outside stream capture.  Captured calls can be replayed.  A workspace is one call's at a time. */
 
 /*
  * RMS norm with the residual's addition, row by row:

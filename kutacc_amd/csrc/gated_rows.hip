@@ -5,6 +5,9 @@
 // columns = rows of x): the accumulators of the first two, rounded to bf16, are the operand of the third without leaving the registers.  For that, row i
 // of a slice in the LDS is hidden unit sigma(i) (bits 2 and 3 of i swapped), which makes the eight values a lane holds per k-step consecutive hidden units.
 // The slices come straight into the LDS, into a ring with one barrier a slice.
+//
+// 147456 x 128 -> 512: 64 us, 910 TFLOP/s of the 1380 that a large product reaches here (142 us with the hidden layer in memory).  The matrix pipe works in 37 %
+// of the clocks, the vector issue port in 42 %, both in 18 %: the activation is as much work as the products, and the clock falls under the two together.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -1,6 +1,7 @@
 // The backward pass of the gated transition of 64 and 128 channels: the hidden layer stays on chip, formed once for the gradient of x and once more for those
-// of the weights.  With so few channels that costs less than its way through memory: 65536 rows, 128 -> 512, are 94 GFLOP in place of 69, but h, dg and du,
-// 200 MB written and read again, took 88 us of their own (174 us in all; a kernel that gave the gradient of x and stored them, and products of tiles: 148).
+// of the weights.  With so few channels that costs less than its way through memory: at 65536 rows, 128 -> 512, 94 GFLOP in place of 69, but h, dg and du are
+// 200 MB to write and to read again (us for the whole pass: 110; a kernel that stored them beside the gradient of x, and products of tiles: 88 + 60; products of
+// tiles alone: 174).
 //
 // The gradient of x: a wave owns 32 rows of x and of the gradient of out as operand fragments in registers, and walks the hidden layer in slices of 32 units
 // that come straight into the LDS: g and u from x, dh from the gradient, in 32 bits; what the activation and its derivative make of them is rounded to bf16
