@@ -6,7 +6,7 @@
 // g, u and dh are never rounded: the kernel that forms them holds all of them of one tile at once, and h, dg and du are rounded once, as
 // operands of the products that follow.
 //
-// ff_tiles_kernel covers every shape: 128 x 128 of a result per workgroup of four waves, K in steps of 64 through the LDS, for a list of
+// ff_tiles_kernel covers every shape: 128 x 128 of a result per workgroup of four waves, K in steps of 64 through registers and the LDS, for a list of
 // products that share the tile.
 #include <hip/hip_runtime.h>
 
@@ -44,7 +44,61 @@ struct TilesParams {
 constexpr int TILE = 128, OPERAND_SLOTS = 1024, CT_LD = 136;
 constexpr size_t TILES_LDS = TILE * CT_LD * 2;
 
-template <int MODE, bool ANY>
+// Eight elements of a row that has `size` >= 8, on their way as they lie in memory, without a branch that would wait for them: a piece past the row's end is the row's
+// last eight, and dropped() elements are too many in front.
+__device__ __forceinline__ int dropped(int at, int size) { return max(0, at + 8 - size); }
+__device__ __forceinline__ uint4 ask8(const bf16_t *row, int at, int size) { return load8_any(row - dropped(at, size), (uint32_t)at); }
+// 32 rows by 64 k of a K-major operand, 64 columns by 32 k of an M-major one, as load_kmajor and load_mmajor divide them
+__device__ __forceinline__ PanelRegs ask_kmajor(const bf16_t *base, int64_t ld, int row0, int last_row, int k0, int K, int lane)
+{
+    PanelRegs p;
+    uint4 *dst[4] = {&p.r0, &p.r1, &p.r2, &p.r3};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        *dst[i] = ask8(base + (int64_t)min(row0 + 8 * i + (lane >> 3), last_row) * ld, k0 + (lane & 7) * 8, K);
+    }
+    return p;
+}
+__device__ __forceinline__ PanelRegs ask_mmajor(const bf16_t *base, int64_t ld, int m0, int rows, int k0, int K, int lane)
+{
+    PanelRegs p;
+    uint4 *dst[4] = {&p.r0, &p.r1, &p.r2, &p.r3};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        *dst[i] = ask8(base + (int64_t)min(k0 + 8 * i + mm_row(lane >> 3), K - 1) * ld, m0 + (lane & 7) * 8, rows);
+    }
+    return p;
+}
+// ... and put in order, zeros past K
+__device__ __forceinline__ void settle_kmajor(PanelRegs &p, int k0, int K, int lane)
+{
+    if (k0 + KSTEP > K) {
+        const int drop = min(8, dropped(k0 + (lane & 7) * 8, K));
+        p.r0 = drop_first(p.r0, drop), p.r1 = drop_first(p.r1, drop), p.r2 = drop_first(p.r2, drop), p.r3 = drop_first(p.r3, drop);
+    }
+}
+__device__ __forceinline__ void settle_mmajor(PanelRegs &p, int m0, int rows, int k0, int K, int lane)
+{
+    uint4 *dst[4] = {&p.r0, &p.r1, &p.r2, &p.r3};
+    if (m0 + 64 > rows) {
+        const int drop = min(8, dropped(m0 + (lane & 7) * 8, rows));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            *dst[i] = drop_first(*dst[i], drop);
+        }
+    }
+    if (k0 + 32 > K) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            *dst[i] = k0 + 8 * i + mm_row(lane >> 3) < K ? *dst[i] : zero_u4();
+        }
+    }
+}
+
+// The next step's operands are on their way while this one's are multiplied.  us, so and with branches around the pieces at a row's end: 7829 x 512 x 2046 89
+// and 193, its backward pass 274 and 825 (with rows and hidden units split where tiles are few, as below), 5088 x 124 x 128 41 and 192.  TINY: a width of fewer than
+// eight, element by element.
+template <int MODE, bool TINY>
 __global__ __launch_bounds__(256, MODE == GATED || MODE == HIDDEN_GRADIENTS ? 1 : 2) void ff_tiles_kernel(const TilesParams p)
 {
     constexpr int SUMS = MODE == GATED ? 2 : MODE == HIDDEN_GRADIENTS ? 3 : 1;
@@ -52,14 +106,21 @@ __global__ __launch_bounds__(256, MODE == GATED || MODE == HIDDEN_GRADIENTS ? 1 
     extern __shared__ uint4 lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int r = lane & 31, g = lane >> 5, wm = wave >> 1, wn = wave & 1;
-    int which = 0, tile = blockIdx.x;
-    if constexpr (MODE == WEIGHT_GRADIENTS) {
-        while (which < 2 && tile >= p.tiles[which]) {
-            tile -= p.tiles[which++];
+    constexpr bool SPLIT = MODE == WEIGHT_GRADIENTS || MODE == INPUT_GRADIENT;
+    int which = 0, split = 0;
+    unsigned tile = blockIdx.x;
+    if constexpr (SPLIT) { // (all tiles of a range of k, then the next range's)
+        const unsigned all = (unsigned)(p.tiles[0] + p.tiles[1] + p.tiles[2]);
+        split = (int)(tile / all), tile %= all;
+        while (which < 2 && tile >= (unsigned)p.tiles[which]) {
+            tile -= (unsigned)p.tiles[which++];
         }
     }
-    const int M = p.M[which], N = p.N[which], NT = (N + TILE - 1) / TILE;
-    const int m0 = tile / NT * TILE, n0 = tile % NT * TILE;
+    const int M = p.M[which], N = p.N[which];
+    // the walk of ff_pieces_kernel, as the shares are added in its order
+    const unsigned MT = (unsigned)(M + TILE - 1) / TILE, NT = (unsigned)(N + TILE - 1) / TILE;
+    const unsigned band = tile / (8 * NT), height = min(8u, MT - 8 * band), in = tile - band * 8 * NT;
+    const int m0 = (int)(8 * band + in % height) * TILE, n0 = (int)(in / height) * TILE;
 
     f32x16 acc[SUMS][2][2];
 #pragma unroll
@@ -71,20 +132,31 @@ __global__ __launch_bounds__(256, MODE == GATED || MODE == HIDDEN_GRADIENTS ? 1 
     }
     const int mm_a[2] = {mm_fragment_offset(2 * wm, lane), mm_fragment_offset(2 * wm + 1, lane)};
     const int mm_b[2] = {mm_fragment_offset(2 * wn, lane), mm_fragment_offset(2 * wn + 1, lane)};
-    const int steps = (p.K + KSTEP - 1) / KSTEP;
+    const int all_steps = (p.K + KSTEP - 1) / KSTEP;
+    const int first = SPLIT ? (int)((int64_t)all_steps * split / p.splits) : 0, steps = SPLIT ? (int)((int64_t)all_steps * (split + 1) / p.splits) : all_steps;
 #pragma unroll
     for (int n = 0; n < PRODUCTS; ++n) {
         constexpr bool A_MMAJOR = MODE == WEIGHT_GRADIENTS;
         const bool B_MMAJOR = MODE == INPUT_GRADIENT || MODE == WEIGHT_GRADIENTS || (MODE == HIDDEN_GRADIENTS && n == 2); // a constant in every copy
         const Product &q = p.product[MODE == WEIGHT_GRADIENTS ? which : n];
-        auto fetch_a = [&](int k0) {
-            return A_MMAJOR ? load_mmajor<ANY>(q.a, q.a_ld, m0 + 64 * (wave & 1), M, k0 + 32 * (wave >> 1), p.K, lane)
-                            : load_kmajor<ANY>(q.a, q.a_ld, m0 + 32 * wave, M - 1, k0, p.K, lane);
+        auto fetch = [&](const bf16_t *base, int64_t ld, bool mmajor, int at, int extent, int k0) {
+            if constexpr (TINY) {
+                return mmajor ? load_mmajor<true>(base, ld, at + 64 * (wave & 1), extent, k0 + 32 * (wave >> 1), p.K, lane) : load_kmajor<true>(base, ld, at + 32 * wave, extent - 1, k0, p.K, lane);
+            } else {
+                return mmajor ? ask_mmajor(base, ld, at + 64 * (wave & 1), extent, k0 + 32 * (wave >> 1), p.K, lane) : ask_kmajor(base, ld, at + 32 * wave, extent - 1, k0, p.K, lane);
+            }
         };
-        auto fetch_b = [&](int k0) {
-            return B_MMAJOR ? load_mmajor<ANY>(q.b, q.b_ld, n0 + 64 * (wave & 1), N, k0 + 32 * (wave >> 1), p.K, lane)
-                            : load_kmajor<ANY>(q.b, q.b_ld, n0 + 32 * wave, N - 1, k0, p.K, lane);
+        auto settle = [&](PanelRegs &f, bool mmajor, int at, int extent, int k0) {
+            if constexpr (!TINY) {
+                if (mmajor) {
+                    settle_mmajor(f, at + 64 * (wave & 1), extent, k0 + 32 * (wave >> 1), p.K, lane);
+                } else {
+                    settle_kmajor(f, k0, p.K, lane);
+                }
+            }
         };
+        auto fetch_a = [&](int k0) { return fetch(q.a, q.a_ld, A_MMAJOR, m0, M, k0); };
+        auto fetch_b = [&](int k0) { return fetch(q.b, q.b_ld, B_MMAJOR, n0, N, k0); };
         auto park = [&](uint4 *operand, bool mmajor, const PanelRegs &f) {
             if (mmajor) {
                 store_mmajor(operand, 64 * (wave & 1), 32 * (wave >> 1), lane, f);
@@ -93,8 +165,10 @@ __global__ __launch_bounds__(256, MODE == GATED || MODE == HIDDEN_GRADIENTS ? 1 
             }
         };
         f32x16(&sum)[2][2] = acc[SUMS == 1 ? 0 : n];
-        PanelRegs ra = fetch_a(0), rb = fetch_b(0);
-        for (int kt = 0; kt < steps; ++kt) {
+        PanelRegs ra = fetch_a(first * KSTEP), rb = fetch_b(first * KSTEP);
+        for (int kt = first; kt < steps; ++kt) {
+            settle(ra, A_MMAJOR, m0, M, kt * KSTEP);
+            settle(rb, B_MMAJOR, n0, N, kt * KSTEP);
             __syncthreads(); // the stage is no longer being read
             park(lds, A_MMAJOR, ra);
             park(lds + OPERAND_SLOTS, B_MMAJOR, rb);
@@ -122,6 +196,17 @@ __global__ __launch_bounds__(256, MODE == GATED || MODE == HIDDEN_GRADIENTS ? 1 
         }
     }
 
+    if constexpr (SPLIT) {
+        if (p.splits > 1) { // a share of the sums, as ff_pieces_kernel leaves it
+            f32x4 *share = reinterpret_cast<f32x4 *>(p.shares) + ((int64_t)blockIdx.x * 4 + wave) * (2 * 2 * 4 * 64) + lane;
+#pragma unroll
+            for (int n = 0; n < 16; ++n) {
+                const f32x16 &v = acc[0][n / 8][n / 4 % 2];
+                share[n * 64] = f32x4{v[4 * (n % 4)], v[4 * (n % 4) + 1], v[4 * (n % 4) + 2], v[4 * (n % 4) + 3]};
+            }
+            return;
+        }
+    }
     // results as bf16 through the LDS, out as whole rows of 256 bytes
     bf16_t *ct = reinterpret_cast<bf16_t *>(lds);
     auto store = [&](const f32x16 (&v)[2][2], bf16_t *c, int64_t ld) {
@@ -559,7 +644,17 @@ __global__ __launch_bounds__(256) void ff_shares_kernel(const TilesParams p)
     const int n = (int)(of / height) * SIDE + 64 * (wave % WN) + 32 * j + 8 * e + 4 * (lane >> 5);
     if (m < M && n < N) {
         const bf16x4 o = {(bf16_t)sum[0], (bf16_t)sum[1], (bf16_t)sum[2], (bf16_t)sum[3]};
-        *reinterpret_cast<bf16x4 *>(p.c[which] + (int64_t)m * p.c_ld[which] + n) = o;
+        bf16_t *const to = p.c[which] + (int64_t)m * p.c_ld[which] + n;
+        if (n + 4 <= N) {
+            __builtin_memcpy(to, &o, sizeof(o));
+        } else {
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+                if (n + f < N) {
+                    to[f] = o[f];
+                }
+            }
+        }
     }
 }
 
@@ -700,7 +795,7 @@ bool pieces(const void *ptr, int64_t ld, int64_t contiguous) { return kutacc_hip
 int64_t tiles_of(int64_t m, int64_t n) { return (m + TILE - 1) / TILE * ((n + TILE - 1) / TILE); }
 
 template <int MODE>
-int launch_any(TilesParams p, bool any, double flops, const char *name, hipStream_t stream)
+int launch_any(TilesParams p, double flops, const char *name, hipStream_t stream)
 {
     static size_t configured[2][KUTACC_DEVICE_SLOTS] = {};
     int64_t blocks = 0;
@@ -712,12 +807,19 @@ int launch_any(TilesParams p, bool any, double flops, const char *name, hipStrea
         }
         p.tiles[i] = (int)tiles;
     }
-    const auto kernel = any ? &ff_tiles_kernel<MODE, true> : &ff_tiles_kernel<MODE, false>;
-    if (const hipError_t e = kutacc_opt_in_lds(reinterpret_cast<const void *>(kernel), TILES_LDS, configured[any])) {
+    const bool tiny = std::min(p.N[0], MODE == WEIGHT_GRADIENTS ? p.M[0] : p.K) < 8; // contiguous extents
+    const auto kernel = tiny ? &ff_tiles_kernel<MODE, true> : &ff_tiles_kernel<MODE, false>;
+    if (const hipError_t e = kutacc_opt_in_lds(reinterpret_cast<const void *>(kernel), TILES_LDS, configured[tiny])) {
         return kutacc_hip_status(e);
     }
     kutacc_prof::KernelTimer t(name, flops, stream);
-    kernel<<<dim3((unsigned)blocks), 256, TILES_LDS, stream>>>(p);
+    if (blocks * p.splits > INT32_MAX) {
+        return KUTACC_HIP_EUNSUPPORTED;
+    }
+    kernel<<<dim3((unsigned)(blocks * p.splits)), 256, TILES_LDS, stream>>>(p);
+    if ((MODE == WEIGHT_GRADIENTS || MODE == INPUT_GRADIENT) && p.splits > 1) {
+        ff_shares_kernel<2, 2, 2><<<dim3((unsigned)(blocks * 16)), 256, 0, stream>>>(p);
+    }
     return kutacc_hip_status(hipGetLastError());
 }
 
@@ -748,8 +850,10 @@ int launch_pieces(TilesParams p, hipStream_t stream)
         return kutacc_hip_status(e);
     }
     kernel<<<dim3((unsigned)groups), 64 * WM * WN * GROUPS, LDS, stream>>>(p);
-    if ((MODE == WEIGHT_GRADIENTS || MODE == INPUT_GRADIENT) && MI == 2 && GROUPS == 1 && p.splits > 1) {
-        ff_shares_kernel<MI, WM, WN><<<dim3((unsigned)(tiles * WM * WN * MI * 2)), 256, 0, stream>>>(p);
+    if constexpr ((MODE == WEIGHT_GRADIENTS || MODE == INPUT_GRADIENT) && MI == 2 && GROUPS == 1) {
+        if (p.splits > 1) {
+            ff_shares_kernel<MI, WM, WN><<<dim3((unsigned)(tiles * WM * WN * MI * 2)), 256, 0, stream>>>(p);
+        }
     }
     return kutacc_hip_status(hipGetLastError());
 }
@@ -848,7 +952,7 @@ template <int MODE>
 int launch(const TilesParams &p, bool any, double flops, const char *name, hipStream_t stream)
 {
     if (any) {
-        return launch_any<MODE>(p, true, flops, name, stream);
+        return launch_any<MODE>(p, flops, name, stream);
     }
     kutacc_prof::KernelTimer t(name, flops, stream);
     return launch_whole<MODE>(p, stream);

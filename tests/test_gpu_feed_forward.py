@@ -402,7 +402,9 @@ def test_gated_transition_backward(activation, c_o, c_i):
 
 # enough tiles for the kernels of 128, 192 and 256 rows a tile in every product: ragged sides, k that ends within a stage, an odd number of stages for two groups
 @pytest.mark.parametrize("rows,c_o,c_i", [(4001, 264, 2816), (5000, 136, 2816), (8090, 2048, 72), (8090, 1032, 200), (4001, 72, 4096), (130, 1024, 4096), (2100, 512, 520), (1000, 1024, 1096),
-                                          (40000, 64, 136)])
+                                          (40000, 64, 136),
+                                          # ... and of widths that are no whole pieces, split by rows and by hidden units, odd ones and of few columns
+                                          (5088, 124, 130), (2113, 77, 131), (1500, 515, 1030), (70, 70, 1001), (1100, 9, 4100), (3000, 1027, 12)])
 def test_gated_transition_of_many_tiles(rows, c_o, c_i):
     w = weights_of(rows, c_o, c_i)
     gpu, x, dy = [t.cuda() for t in w], cpu_randn(1, rows, c_o), cpu_randn(2, rows, c_o)
