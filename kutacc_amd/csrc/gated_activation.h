@@ -35,4 +35,7 @@ __device__ __forceinline__ float activate(float v, int activation, float &deriva
     return v * s;
 }
 
+// what the rounding of v to r left; of a result past bf16's range nothing, as infinity less infinity is no number
+__device__ __forceinline__ bf16_t rounding_rest(float v, bf16_t r) { return (bf16_t)(fabsf((float)r) <= 3.4e38f ? v - (float)r : 0.f); }
+
 } // namespace kutacc_dev

@@ -317,11 +317,11 @@ namespace kutacc_launch {
 
 // 64, 128 and 256 channels, and rows enough: a wave's chain through the hidden layer takes its time however few there are (us, here and with the hidden
 // layer in memory: 128 -> 512 5000 rows 15.0 14.1, 12000 15.7 22.7, 147456 66 142; 128 -> 2048 8000 rows 46 39, 12000 47 60; 256 -> 1024 20000 rows 64 60,
-// 40000 76 104, 195072 284 476; 64 -> 256 100 rows 7.1 9.0, 40000 10.7 30.4).
+// 40000 76 104, 195072 284 476; 64 -> 256 100 rows 7.1 9.0, 40000 10.7 30.4; 64 -> 512 60 rows 11.2 7.8).
 bool gated_rows_takes(const kutacc_hip_gated_transition_args_t &a)
 {
     const int64_t row_blocks = (a.rows + 31) / 32, cus = kutacc_cu_count();
-    return (a.c_o == 64 || (a.c_o == 128 && row_blocks >= cus) || (a.c_o == 256 && 2 * row_blocks >= 5 * cus)) && a.c_i % 32 == 0 && row_blocks <= ((int64_t)1 << 31) &&
+    return ((a.c_o == 64 && a.rows > 64) || (a.c_o == 128 && row_blocks >= cus) || (a.c_o == 256 && 2 * row_blocks >= 5 * cus)) && a.c_i % 32 == 0 && row_blocks <= ((int64_t)1 << 31) &&
            a.c_i <= (1 << 24) && a.x_ld % 8 == 0 && a.out_ld % 8 == 0 && kutacc_hip_aligned16(a.x) && kutacc_hip_aligned16(a.out) && kutacc_hip_aligned16(a.gate_w) &&
            kutacc_hip_aligned16(a.up_w) && kutacc_hip_aligned16(a.down_w);
 }

@@ -663,9 +663,14 @@ __global__ __launch_bounds__(256) void ff_shares_kernel(const TilesParams p)
 // 16 MB rows by 16 NB columns a workgroup, all of them in every wave (and with GATED of both projections): wave w takes blocks w, w + W, ... and brings
 // them straight into its own part of the LDS, eight rows of 128 bytes a load, DEPTH blocks ahead and without barriers.  The waves' sums meet in the LDS at
 // the end, in one order.  Memory bounds it: 3 x 2048 -> 8192 GATED 12.9 us, 5.2 TB/s, PLAIN 9.6, 3.5.
-template <int MODE, int MB, int NB, int W, int DEPTH>
+//
+// With WITH_REST half of the MB blocks of rows are what the rounding of the others left, product 1's: few enough results are bound by launches, and keep the
+// hidden layer to 16 bits almost for nothing (3 x 128 -> 512 7.3 us and 7.1): a result's error is then that of its own rounding, 1.65e-3 in place of 2.35e-3.
+template <int MODE, int MB, int NB, int W, int DEPTH, bool WITH_REST = false>
 __global__ __launch_bounds__(64 * W) void ff_split_kernel(const TilesParams p)
 {
+    constexpr int ROW_BLOCKS = WITH_REST ? MB / 2 : MB;
+    static_assert(!WITH_REST || (MODE == PLAIN && MB % 2 == 0), "the hidden layer is the product's operand");
     static_assert(MODE == PLAIN || MODE == GATED, "operands along k");
     constexpr int SUMS = MODE == GATED ? 2 : 1, LOADS = 2 * (MB + SUMS * NB), SLOTS = 64 * LOADS;
     static_assert(SUMS * MB * NB <= DEPTH * LOADS, "the sums lie where the operands were");
@@ -673,14 +678,15 @@ __global__ __launch_bounds__(64 * W) void ff_split_kernel(const TilesParams p)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, q = lane >> 4;
     const int M = p.M[0], N = p.N[0], NT = (N + 16 * NB - 1) / (16 * NB);
-    const int n0 = (int)(blockIdx.x % (unsigned)NT) * 16 * NB, m0 = (int)(blockIdx.x / (unsigned)NT) * 16 * MB;
+    const int n0 = (int)(blockIdx.x % (unsigned)NT) * 16 * NB, m0 = (int)(blockIdx.x / (unsigned)NT) * 16 * ROW_BLOCKS;
     const int blocks = (p.K + 63) / 64;
     const int chunk = (lane & 7) ^ (lane >> 3);
     const bf16_t *const a_tile = p.product[0].a + (int64_t)m0 * p.product[0].a_ld;
+    [[maybe_unused]] const bf16_t *const rest_tile = p.product[1].a + (int64_t)m0 * p.product[0].a_ld;
     uint32_t a_from[2 * MB], b_from[2 * NB];
 #pragma unroll
     for (int u = 0; u < 2 * MB; ++u) {
-        a_from[u] = 2u * ((uint32_t)min(8 * u + (lane >> 3), M - m0 - 1) * (uint32_t)p.product[0].a_ld + 8u * (uint32_t)chunk);
+        a_from[u] = 2u * ((uint32_t)min(8 * (u % (2 * ROW_BLOCKS)) + (lane >> 3), M - m0 - 1) * (uint32_t)p.product[0].a_ld + 8u * (uint32_t)chunk);
     }
 #pragma unroll
     for (int u = 0; u < 2 * NB; ++u) {
@@ -693,7 +699,7 @@ __global__ __launch_bounds__(64 * W) void ff_split_kernel(const TilesParams p)
         if (8 * chunk < p.K - 64 * b) {
 #pragma unroll
             for (int u = 0; u < 2 * MB; ++u) {
-                load_to_lds(stage + u * 1024u, a_tile + (int64_t)64 * b, a_from[u]);
+                load_to_lds(stage + u * 1024u, (u < 2 * ROW_BLOCKS ? a_tile : rest_tile) + (int64_t)64 * b, a_from[u]);
             }
 #pragma unroll
             for (int u = 0; u < 2 * NB * SUMS; ++u) {
@@ -762,29 +768,40 @@ __global__ __launch_bounds__(64 * W) void ff_split_kernel(const TilesParams p)
         sums[(wave * SUMS * NB * MB + n) * 64 + lane] = acc[n / (NB * MB)][n / MB % NB][n % MB];
     }
     __syncthreads();
-    for (int t = wave; t < NB * MB; t += W) {
+    for (int t = wave; t < NB * ROW_BLOCKS; t += W) {
         f32x4 sum[SUMS];
 #pragma unroll
         for (int s = 0; s < SUMS; ++s) {
-            sum[s] = sums[(s * NB * MB + t) * 64 + lane];
+            const int at = s * NB * MB + t / ROW_BLOCKS * MB + t % ROW_BLOCKS;
+            sum[s] = sums[at * 64 + lane];
 #pragma unroll
             for (int v = 1; v < W; ++v) {
-                sum[s] += sums[((v * SUMS + s) * NB * MB + t) * 64 + lane];
+                sum[s] += sums[(v * SUMS * NB * MB + at) * 64 + lane];
+            }
+            if constexpr (WITH_REST) {
+#pragma unroll
+                for (int v = 0; v < W; ++v) {
+                    sum[s] += sums[(v * SUMS * NB * MB + at + ROW_BLOCKS) * 64 + lane];
+                }
             }
         }
-        const int m = m0 + 16 * (t % MB) + r, n = n0 + 16 * (t / MB) + 4 * q;
-        bf16x4 o;
+        const int m = m0 + 16 * (t % ROW_BLOCKS) + r, n = n0 + 16 * (t / ROW_BLOCKS) + 4 * q;
+        bf16x4 o, rest;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
+            float v = sum[0][e];
             if constexpr (MODE == GATED) {
                 float none;
-                o[e] = (bf16_t)(activate<false>(sum[0][e], p.activation, none) * sum[1][e]);
-            } else {
-                o[e] = (bf16_t)sum[0][e];
+                v = activate<false>(v, p.activation, none) * sum[1][e];
             }
+            o[e] = (bf16_t)v;
+            rest[e] = rounding_rest(v, o[e]);
         }
         if (m < M && n < N) { // N is a multiple of 8
             *reinterpret_cast<bf16x4 *>(p.c[0] + (int64_t)m * p.c_ld[0] + n) = o;
+            if (MODE == GATED && p.c[1] != nullptr) {
+                *reinterpret_cast<bf16x4 *>(p.c[1] + (int64_t)m * p.c_ld[0] + n) = rest;
+            }
         }
     }
 }
@@ -858,13 +875,13 @@ int launch_pieces(TilesParams p, hipStream_t stream)
     return kutacc_hip_status(hipGetLastError());
 }
 
-template <int MODE, int MB, int NB, int W, int DEPTH>
+template <int MODE, int MB, int NB, int W, int DEPTH, bool WITH_REST = false>
 int launch_split(TilesParams p, hipStream_t stream)
 {
     constexpr size_t LDS = (size_t)W * DEPTH * 2 * (MB + (MODE == GATED ? 2 : 1) * NB) * 1024;
     static size_t configured[KUTACC_DEVICE_SLOTS] = {};
-    const auto kernel = &ff_split_kernel<MODE, MB, NB, W, DEPTH>;
-    const int64_t groups = count_tiles(p, 16 * MB, 16 * NB);
+    const auto kernel = &ff_split_kernel<MODE, MB, NB, W, DEPTH, WITH_REST>;
+    const int64_t groups = count_tiles(p, WITH_REST ? 8 * MB : 16 * MB, 16 * NB);
     if (groups > INT32_MAX) {
         return KUTACC_HIP_EUNSUPPORTED;
     }
@@ -905,6 +922,9 @@ template <int MODE>
 int launch_whole(const TilesParams &p, hipStream_t stream)
 {
     if constexpr (MODE == PLAIN) {
+        if (p.product[1].a != nullptr) {
+            return p.M[0] <= 16 ? launch_split<MODE, 2, 1, 8, 2, true>(p, stream) : launch_split<MODE, 4, 2, 8, 1, true>(p, stream);
+        }
         if (p.M[0] <= 16) {
             return launch_split<MODE, 1, 1, 16, 2>(p, stream);
         }
@@ -921,6 +941,9 @@ int launch_whole(const TilesParams &p, hipStream_t stream)
     } else if constexpr (MODE == GATED) {
         if (p.M[0] <= 16) {
             return launch_split<MODE, 1, 1, 8, 2>(p, stream);
+        }
+        if (p.c[1] != nullptr) {
+            return launch_split<MODE, 2, 2, 8, 1>(p, stream);
         }
         constexpr Choice choices[] = {{32, 32, 1, 0.23f}, {64, 32, 1, 0.33f}, {128, 64, 2, 1.15f}, {192, 128, 1, 1.45f}, {256, 128, 1, 1.90f}};
         switch (least(p, choices)) {
@@ -994,11 +1017,14 @@ int64_t shares_bytes(int64_t rows, int64_t c_o, int64_t c_i)
 
 int64_t padded(int64_t v) { return (v + 31) / 32 * 32; }
 int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
+
+// results few enough to keep what the rounding of the hidden layer leaves
+bool keeps_rest(int64_t rows, int64_t c_o) { return rows <= 64 && rows * c_o <= 4096; }
 } // namespace
 
 namespace kutacc_launch {
 
-int64_t gated_transition_workspace(int64_t rows, int64_t c_o, int64_t c_i) { return align256(2 * rows * padded(c_i)); }
+int64_t gated_transition_workspace(int64_t rows, int64_t c_o, int64_t c_i) { return (keeps_rest(rows, c_o) ? 2 : 1) * align256(2 * rows * padded(c_i)); }
 
 int gated_transition(const kutacc_hip_gated_transition_args_t &a, hipStream_t stream)
 {
@@ -1015,15 +1041,19 @@ int gated_transition(const kutacc_hip_gated_transition_args_t &a, hipStream_t st
     p.M[0] = (int)rows, p.N[0] = (int)c_i, p.K = (int)c_o, p.activation = a.activation;
     const bool widths = c_o % 8 == 0 && c_i % 8 == 0;
     const bool any_in = !widths || !pieces(a.x, a.x_ld, c_o) || !kutacc_hip_aligned16(a.gate_w) || !kutacc_hip_aligned16(a.up_w);
+    const bool any_out = !widths || !kutacc_hip_aligned16(a.down_w) || !pieces(a.out, a.out_ld, c_o);
+    bf16_t *const rest = keeps_rest(rows, c_o) && !any_in && !any_out ? h + align256(2 * rows * h_ld) / 2 : nullptr;
+    p.c[1] = rest;
     if (const int rc = launch<GATED>(p, any_in, 4.0 * (double)rows * (double)c_o * (double)c_i, "gated_transition<gated>", stream)) {
         return rc;
     }
     TilesParams d = {};
     d.splits = 1;
     d.product[0] = {h, (const bf16_t *)a.down_w, h_ld, c_i};
+    d.product[1] = {rest, (const bf16_t *)a.down_w, h_ld, c_i};
     d.c[0] = (bf16_t *)a.out, d.c_ld[0] = a.out_ld;
     d.M[0] = (int)rows, d.N[0] = (int)c_o, d.K = (int)c_i;
-    return launch<PLAIN>(d, !widths || !kutacc_hip_aligned16(a.down_w) || !pieces(a.out, a.out_ld, c_o), 2.0 * (double)rows * (double)c_o * (double)c_i, "gated_transition<plain>", stream);
+    return launch<PLAIN>(d, any_out, 2.0 * (double)rows * (double)c_o * (double)c_i, "gated_transition<plain>", stream);
 }
 
 int64_t gated_transition_backward_workspace(int64_t rows, int64_t c_o, int64_t c_i)

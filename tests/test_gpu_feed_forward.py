@@ -422,7 +422,7 @@ def test_gated_transition_of_many_tiles(rows, c_o, c_i):
 
 # the hidden layer on chip: fewer waves than a round, several rounds with a ragged last one, one slice of hidden units and several, strided rows
 @pytest.mark.parametrize("activation", ["silu", "gelu"])
-@pytest.mark.parametrize("rows,c_o,c_i,pad", [(1, 64, 32, 0), (45, 64, 96, 8), (33000, 64, 64, 0), (8200, 128, 32, 0), (8191, 128, 64, 8), (9001, 128, 512, 0), (70001, 128, 96, 0),
+@pytest.mark.parametrize("rows,c_o,c_i,pad", [(1, 64, 32, 0), (45, 64, 96, 8), (65, 64, 32, 0), (109, 64, 96, 8), (33000, 64, 64, 0), (8200, 128, 32, 0), (8191, 128, 64, 8), (9001, 128, 512, 0), (70001, 128, 96, 0),
                                               (20500, 256, 32, 0), (20900, 256, 160, 8), (33000, 256, 64, 0)])
 def test_gated_transition_on_chip(activation, rows, c_o, c_i, pad):
     w = weights_of(rows, c_o, c_i)
@@ -518,6 +518,20 @@ def test_gated_transition_of_large_values(activation):
     ok(capi.GatedTransitionBackward(x.cuda(), *gpu, dy.cuda(), *(r.view for r in grads), activation=activation))
     for name, r in zip(("grad_x", "grad_gate_w", "grad_up_w", "grad_down_w"), grads):
         oracle.close(r.view, want[name][0], oracle.stored(*want[name], BF16), name)
+
+
+# few results, whose hidden layer keeps what its rounding leaves: a rounding within 2^-8 of a rest within 2^-8 of the value, in place of the first alone
+@pytest.mark.parametrize("rows,c_o,c_i", [(1, 128, 512), (16, 256, 520), (17, 64, 256), (64, 64, 128), (1, 4096, 64), (2, 2048, 72), (33, 120, 1000)])
+def test_gated_transition_of_few_results_rounds_once(rows, c_o, c_i):
+    w = weights_of(rows, c_o, c_i)
+    x = cpu_randn(1, rows, c_o)
+    out = torch.empty(rows, c_o, device="cuda", dtype=BF16)
+    ok(capi.GatedTransition(x.cuda(), *(t.cuda() for t in w), out))
+    want, off = oracle.gated_transition(x, *w, "silu")["out"]
+    h = torch.nn.functional.silu(x.double() @ w[0].double().T) * (x.double() @ w[1].double().T)
+    off = off - (2.0 ** -8 - 2.0 ** -16) * (h.abs() @ w[2].double().abs().T)
+    assert bool((off > 0).all())
+    oracle.close(out, want, oracle.stored(want, off, BF16), "out")
 
 
 @pytest.mark.parametrize("rows,c_o,c_i", [(40, 128, 256), (40, 96, 160)])
