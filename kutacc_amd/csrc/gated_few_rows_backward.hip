@@ -2,9 +2,10 @@
 //
 // A workgroup of eight waves owns 32 hidden units.  First g, u and dh of all rows: the waves share the channels, operands straight into registers but the
 // columns of Wd, which leave the LDS by its transposing reads; their sums meet in the LDS, in one order.  What the activation and its derivative make of them is
-// rounded to bf16 once and stays in the LDS: h, dg and du of 32 units, and for the gradient of x, whose few values have nothing to average over, what the
-// rounding of dg and du left: 16 bits of them, at no cost here.  Then the waves go through the channels in blocks of 32, each with its own: the units' rows
-// of the three weights' gradients are whole, as the rows are few enough to be contracted at once, and the gradient of x is a share of 32 units, in fp32.
+// rounded to bf16 once and stays in the LDS: h, dg and du of 32 units, and what that rounding left, for results that have few values or are sums of few rows,
+// and so little to average over: 16 bits of them, almost for nothing here (us, with rests and without: 25 x 128 x 512 10.2 and 9.9).  Then the waves go through
+// the channels in blocks of 32, each with its own: the units' rows of the three weights' gradients are whole, as the rows are few enough to be contracted at once,
+// and the gradient of x is a share of 32 units, in fp32.
 // What bounds it are those trips and the code itself, which is run once: 6 us at 25 x 128 -> 512, of which the operands of the first products take 1.5, the sums and
 // the activation 1.5 (2.7 as straight-line code), the blocks of channels 2.5.  us for the whole pass, this and the kernels for any number of rows: 25 x 128 x 512
 // 9.9 and 26, 3 x 256 x 1024 11 and 28, 50 x 256 x 896 17 and 30, 16 x 512 x 2048 19 and 35, 64 x 512 x 2048 29 and 35, 64 x 1024 x 4096 (34 MB of shares) 53 and 52.
@@ -41,13 +42,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void gated_few_rows_backward_kernel(
     constexpr int PARTS = WAVES / MB;                         // ways that the channels are split in the first products
     constexpr int ROWS_KB = 2 * MB;                           // of 64-byte rows: two loads for 32
     constexpr int OWN = (2 * ROWS_KB + 4) * 1024;             // a wave's blocks of x and the gradient, Wg and Wu
-    extern __shared__ uint4 lds[];                            // [h, dg, du, the rest of dg and du: ROWS_KB each], then the columns of Wd, then the sums, then the waves' blocks
+    extern __shared__ uint4 lds[];                            // [h, dg, du, the rests of dg, du and h: ROWS_KB each], then the columns of Wd, then the sums, then the waves' blocks
     lds_char *const bytes = (lds_char *)lds;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 31, g = lane >> 5;
     const int unit0 = (int)blockIdx.x * UNITS;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(const lds_char *)lds;
-    constexpr int REST = 5 * ROWS_KB * 1024; // where what follows h, dg, du and what the rounding of dg and du left begins
+    constexpr bool ALL_RESTS = MB == 1;                              // of two blocks of rows the weights' gradients do without: no registers
+    constexpr int REST = (ALL_RESTS ? 6 : 5) * ROWS_KB * 1024;       // where what follows h, dg, du and what their rounding left begins
     // this lane's 16 bytes of 16 rows of 64 bytes, `ld` elements apart
     auto lane_bytes = [&](int64_t ld, int row0, int last) { return 2u * ((uint32_t)min(row0 + (lane >> 2), last) * (uint32_t)ld + 8u * (uint32_t)((lane & 3) ^ ((lane >> 4) & 3))); };
     const int a4 = (lane & 15) >> 2, half16 = (lane >> 4) & 1, quad = lane & 3;
@@ -119,15 +121,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void gated_few_rows_backward_kernel(
             v[0] += from[0], v[1] += from[512], v[2] += from[1024];
         }
         const bool valid = at_row < p.rows; // rows past the last are zeros, and so is all they give
-        two_bf16 h, dg, du, dg_rest, du_rest;
+        two_bf16 h, dg, du, h_rest, dg_rest, du_rest;
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
             float slope;
             const float a = activate<true>(v[0][f], ACTIVATION, slope);
-            h[f] = (bf16_t)(valid ? a * v[1][f] : 0.f);
-            const float dg32 = valid ? v[2][f] * v[1][f] * slope : 0.f, du32 = valid ? v[2][f] * a : 0.f;
-            dg[f] = (bf16_t)dg32, du[f] = (bf16_t)du32;
-            dg_rest[f] = rounding_rest(dg32, dg[f]), du_rest[f] = rounding_rest(du32, du[f]);
+            const float h32 = valid ? a * v[1][f] : 0.f, dg32 = valid ? v[2][f] * v[1][f] * slope : 0.f, du32 = valid ? v[2][f] * a : 0.f;
+            h[f] = (bf16_t)h32, dg[f] = (bf16_t)dg32, du[f] = (bf16_t)du32;
+            h_rest[f] = rounding_rest(h32, h[f]), dg_rest[f] = rounding_rest(dg32, dg[f]), du_rest[f] = rounding_rest(du32, du[f]);
         }
         const int to = at_row * 64 + ((e ^ ((at_row >> 2) & 3)) * 16) + g * 8 + half * 4; // units 8 e + 4 g + 2 half ..
         *(__attribute__((address_space(3))) two_bf16 *)(bytes + to) = h;
@@ -135,15 +136,22 @@ __global__ __launch_bounds__(64 * WAVES, 2) void gated_few_rows_backward_kernel(
         *(__attribute__((address_space(3))) two_bf16 *)(bytes + 2 * ROWS_KB * 1024 + to) = du;
         *(__attribute__((address_space(3))) two_bf16 *)(bytes + 3 * ROWS_KB * 1024 + to) = dg_rest;
         *(__attribute__((address_space(3))) two_bf16 *)(bytes + 4 * ROWS_KB * 1024 + to) = du_rest;
+        if constexpr (ALL_RESTS) {
+            *(__attribute__((address_space(3))) two_bf16 *)(bytes + 5 * ROWS_KB * 1024 + to) = h_rest;
+        }
     }
     __syncthreads();
 
     // ---- the gradients, 32 channels at a time ----
     bf16x8 h_t[ROWS_KB], dg_t[ROWS_KB], du_t[ROWS_KB]; // k along the rows
+    bf16x8 h_rest_t[ALL_RESTS ? ROWS_KB : 1], dg_rest_t[ALL_RESTS ? ROWS_KB : 1], du_rest_t[ALL_RESTS ? ROWS_KB : 1];
     bf16x8 dg[MB][2], du[MB][2], dg_rest[MB][2], du_rest[MB][2]; // k along the units
 #pragma unroll
     for (int k = 0; k < ROWS_KB; ++k) {
         h_t[k] = transposed(k * 1024), dg_t[k] = transposed((ROWS_KB + k) * 1024), du_t[k] = transposed((2 * ROWS_KB + k) * 1024);
+        if constexpr (ALL_RESTS) {
+            dg_rest_t[k] = transposed((3 * ROWS_KB + k) * 1024), du_rest_t[k] = transposed((4 * ROWS_KB + k) * 1024), h_rest_t[k] = transposed((5 * ROWS_KB + k) * 1024);
+        }
     }
 #pragma unroll
     for (int m = 0; m < MB; ++m) {
@@ -178,6 +186,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void gated_few_rows_backward_kernel(
             gate_g = mfma(x_t, dg_t[k], gate_g);
             up_g = mfma(x_t, du_t[k], up_g);
             down_g = mfma(h_t[k], dy_t, down_g);
+            if constexpr (ALL_RESTS) {
+                gate_g = mfma(x_t, dg_rest_t[k], gate_g);
+                up_g = mfma(x_t, du_rest_t[k], up_g);
+                down_g = mfma(h_rest_t[k], dy_t, down_g);
+            }
         }
 #pragma unroll
         for (int m = 0; m < MB; ++m) {
@@ -254,7 +267,7 @@ hipError_t launch(const FewRowsParams &p, hipStream_t stream)
 {
     static size_t configured[KUTACC_DEVICE_SLOTS] = {};
     const auto kernel = &gated_few_rows_backward_kernel<MB, ACTIVATION>;
-    constexpr size_t OPERANDS = 5 * 2 * MB * 1024, SUMS = WAVES * 12 * 1024, BLOCKS = WAVES * (4 * MB + 4) * 1024;
+    constexpr size_t OPERANDS = (MB == 1 ? 6 : 5) * 2 * MB * 1024, SUMS = WAVES * 12 * 1024, BLOCKS = WAVES * (4 * MB + 4) * 1024;
     const size_t bytes = OPERANDS + std::max({SUMS, BLOCKS, (size_t)p.c_o * 64});
     if (const hipError_t e = kutacc_opt_in_lds(reinterpret_cast<const void *>(kernel), bytes, configured)) {
         return e;
