@@ -779,9 +779,15 @@ __global__ __launch_bounds__(64 * W) void ff_split_kernel(const TilesParams p)
                 sum[s] += sums[(v * SUMS * NB * MB + at) * 64 + lane];
             }
             if constexpr (WITH_REST) {
+                f32x4 rests = sums[(at + ROW_BLOCKS) * 64 + lane];
 #pragma unroll
-                for (int v = 0; v < W; ++v) {
-                    sum[s] += sums[(v * SUMS * NB * MB + at + ROW_BLOCKS) * 64 + lane];
+                for (int v = 1; v < W; ++v) {
+                    rests += sums[(v * SUMS * NB * MB + at + ROW_BLOCKS) * 64 + lane];
+                }
+                // an infinity among the weights makes the sum what it is: a rest of the other sign, or of zero, would make it no number
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sum[s][e] = __builtin_isfinite(sum[s][e]) ? sum[s][e] + rests[e] : sum[s][e];
                 }
             }
         }
