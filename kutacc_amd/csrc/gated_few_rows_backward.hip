@@ -180,32 +180,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void gated_few_rows_backward_kernel(
             lds[own / 16 + i] = zero_u4(), lds[own / 16 + 64 * ROWS_KB + i] = zero_u4();
         }
         f32x16 gate_g = zero16(), up_g = zero16(), down_g = zero16(), x_g[MB];
+        bf16x8 x_t[ALL_RESTS ? ROWS_KB : 1], dy_t[ALL_RESTS ? ROWS_KB : 1], gate_t[2], up_t[2];
 #pragma unroll
         for (int k = 0; k < ROWS_KB; ++k) {
-            const bf16x8 x_t = transposed(own + k * 1024), dy_t = transposed(own + (ROWS_KB + k) * 1024);
-            gate_g = mfma(x_t, dg_t[k], gate_g);
-            up_g = mfma(x_t, du_t[k], up_g);
-            down_g = mfma(h_t[k], dy_t, down_g);
-            if constexpr (ALL_RESTS) {
-                gate_g = mfma(x_t, dg_rest_t[k], gate_g);
-                up_g = mfma(x_t, du_rest_t[k], up_g);
-                down_g = mfma(h_rest_t[k], dy_t, down_g);
-            }
-        }
-#pragma unroll
-        for (int m = 0; m < MB; ++m) {
-            x_g[m] = zero16();
-        }
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const bf16x8 gate_t = transposed(own + (2 * ROWS_KB + s) * 1024), up_t = transposed(own + (2 * ROWS_KB + 2 + s) * 1024);
-#pragma unroll
-            for (int m = 0; m < MB; ++m) {
-                x_g[m] = mfma(gate_t, dg[m][s], x_g[m]);
-                x_g[m] = mfma(up_t, du[m][s], x_g[m]);
-                x_g[m] = mfma(gate_t, dg_rest[m][s], x_g[m]);
-                x_g[m] = mfma(up_t, du_rest[m][s], x_g[m]);
-            }
+            constexpr int KEPT = ALL_RESTS ? 1 : 0;
+            x_t[KEPT * k] = transposed(own + k * 1024), dy_t[KEPT * k] = transposed(own + (ROWS_KB + k) * 1024);
+            gate_g = mfma(x_t[KEPT * k], dg_t[k], gate_g);
+            up_g = mfma(x_t[KEPT * k], du_t[k], up_g);
+            down_g = mfma(h_t[k], dy_t[KEPT * k], down_g);
         }
         // channels c0 + 8 e + 4 g .. of unit or row r; units 8 e + 4 g .. of channel c0 + r
         auto store = [&](bf16_t *to, const f32x16 &v) {
@@ -214,15 +196,92 @@ __global__ __launch_bounds__(64 * WAVES, 2) void gated_few_rows_backward_kernel(
                 *reinterpret_cast<bf16x4 *>(to + 8 * e) = bf16x4{(bf16_t)v[4 * e], (bf16_t)v[4 * e + 1], (bf16_t)v[4 * e + 2], (bf16_t)v[4 * e + 3]};
             }
         };
-        const int64_t of_unit = (int64_t)(unit0 + r) * p.c_o + c0 + 4 * g;
-        if (p.grad_gate_w != nullptr) {
-            store(p.grad_gate_w + of_unit, gate_g);
+        auto store_weights = [&]() {
+            const int64_t of_unit = (int64_t)(unit0 + r) * p.c_o + c0 + 4 * g;
+            if (p.grad_gate_w != nullptr) {
+                store(p.grad_gate_w + of_unit, gate_g);
+            }
+            if (p.grad_up_w != nullptr) {
+                store(p.grad_up_w + of_unit, up_g);
+            }
+            if (p.grad_down_w != nullptr) {
+                store(p.grad_down_w + (int64_t)(c0 + r) * p.c_i + unit0 + 4 * g, down_g);
+            }
+        };
+        if constexpr (!ALL_RESTS) { // now: beside what follows they would not all have registers
+            store_weights();
         }
-        if (p.grad_up_w != nullptr) {
-            store(p.grad_up_w + of_unit, up_g);
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+            x_g[m] = zero16();
         }
-        if (p.grad_down_w != nullptr) {
-            store(p.grad_down_w + (int64_t)(c0 + r) * p.c_i + unit0 + 4 * g, down_g);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            gate_t[s] = transposed(own + (2 * ROWS_KB + s) * 1024), up_t[s] = transposed(own + (2 * ROWS_KB + 2 + s) * 1024);
+#pragma unroll
+            for (int m = 0; m < MB; ++m) {
+                x_g[m] = mfma(gate_t[s], dg[m][s], x_g[m]);
+                x_g[m] = mfma(up_t[s], du[m][s], x_g[m]);
+            }
+        }
+        // What the rounding left, on top.  An infinity among the other operands makes a sum what it is: a rest of the other sign, or of zero, would make it no
+        // number.  So where a block has a sum that is not finite, its rests' sums are formed apart, and added to those that are.
+        float finite = 0.f; // else no number
+        auto look = [&](const f32x16 &v) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                finite = fmaf(v[e], 0.f, finite);
+            }
+        };
+        auto rests_of_x = [&](int m, f32x16 &to) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                to = mfma(gate_t[s], dg_rest[m][s], to);
+                to = mfma(up_t[s], du_rest[m][s], to);
+            }
+        };
+        [[maybe_unused]] auto rests_of_weights = [&](int which, f32x16 &to) {
+            if constexpr (ALL_RESTS) {
+#pragma unroll
+                for (int k = 0; k < ROWS_KB; ++k) {
+                    to = which == 0 ? mfma(x_t[k], dg_rest_t[k], to) : which == 1 ? mfma(x_t[k], du_rest_t[k], to) : mfma(h_rest_t[k], dy_t[k], to);
+                }
+            }
+        };
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+            look(x_g[m]);
+        }
+        if constexpr (ALL_RESTS) {
+            look(gate_g), look(up_g), look(down_g);
+        }
+        if (__builtin_expect(__any(finite != 0.f) == 0, 1)) {
+#pragma unroll
+            for (int m = 0; m < MB; ++m) {
+                rests_of_x(m, x_g[m]);
+            }
+            rests_of_weights(0, gate_g), rests_of_weights(1, up_g), rests_of_weights(2, down_g);
+        } else {
+            auto add = [&](f32x16 &sum, const f32x16 &rests) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    sum[e] = __builtin_isfinite(sum[e]) ? sum[e] + rests[e] : sum[e];
+                }
+            };
+#pragma unroll
+            for (int m = 0; m < MB; ++m) {
+                f32x16 rests = zero16();
+                rests_of_x(m, rests);
+                add(x_g[m], rests);
+            }
+            if constexpr (ALL_RESTS) {
+                f32x16 rests[3] = {zero16(), zero16(), zero16()};
+                rests_of_weights(0, rests[0]), rests_of_weights(1, rests[1]), rests_of_weights(2, rests[2]);
+                add(gate_g, rests[0]), add(up_g, rests[1]), add(down_g, rests[2]);
+            }
+        }
+        if constexpr (ALL_RESTS) {
+            store_weights();
         }
         if (p.grad_x != nullptr) {
 #pragma unroll

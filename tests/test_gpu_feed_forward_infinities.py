@@ -52,3 +52,16 @@ def test_gated_transition_keeps_infinities(rows, c_o, c_i, place, activation):
     out = Room(rows, c_o, BF16)
     ok(capi.GatedTransition(x.cuda(), *(t.cuda() for t in w), out.view, activation))
     same(out.view, want, "out")
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("place", ["gate_w", "up_w", "down_w", "grad_out"])
+@pytest.mark.parametrize("rows,c_o,c_i", [s for s in SHAPES if s not in ((65, 64, 64), (100, 64, 96), (9001, 128, 96))])
+def test_gated_transition_backward_keeps_infinities(rows, c_o, c_i, place, activation):
+    x, w, dy = operands(rows, c_o, c_i)
+    put_infinity(place, w, dy)
+    want = oracle.gated_transition(x, *w, activation, dy)
+    grads = dict(grad_x=Room(rows, c_o, BF16), grad_gate_w=Room(c_i, c_o, BF16), grad_up_w=Room(c_i, c_o, BF16), grad_down_w=Room(c_o, c_i, BF16))
+    ok(capi.GatedTransitionBackward(x.cuda(), *(t.cuda() for t in w), dy.cuda(), activation=activation, **{k: r.view for k, r in grads.items()}))
+    for name, r in grads.items():
+        same(r.view, want[name][0], name)
