@@ -401,6 +401,13 @@ __global__ __launch_bounds__(256, 1) void gated_weight_gradients_kernel(const Ba
     }
     __builtin_amdgcn_sched_barrier(0);
     step(0, 0, 0, std::false_type{});
+    if (valid < 32) { // the first block's rows past the last: of zeros, but an infinity among the weights makes no numbers of these
+#pragma unroll
+        for (int e = 0; e < 16; ++e) { // (row i of a product is row sigma(i) of the block)
+            const int i = 8 * (e / 4) + 4 * g + e % 4, row = (i & 19) | ((i & 4) << 1) | ((i & 8) >> 1);
+            gate[e] = row < valid ? gate[e] : 0.f, up[e] = row < valid ? up[e] : 0.f, dh[e] = row < valid ? dh[e] : 0.f;
+        }
+    }
     int stage = 0;
     for (int j = 1; j < blocks; ++j) {
         const int before = stage;
