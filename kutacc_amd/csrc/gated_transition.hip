@@ -812,7 +812,8 @@ __global__ __launch_bounds__(64 * W) void ff_split_kernel(const TilesParams p)
     }
 }
 
-// Whether a product's operands fill whole 16-byte pieces: pointers, pitches, and the extents along which rows are contiguous
+// Whether a product's operands fill whole 16-byte pieces: pointers, pitches, and the extents along which rows are contiguous.  Rows of a tile have to lie within
+// 32 bits of bytes from its first, up to 255 pitches on; ff_tiles_kernel has no such bound.
 bool pieces(const void *ptr, int64_t ld, int64_t contiguous) { return kutacc_hip_aligned16(ptr) && ld % 8 == 0 && contiguous % 8 == 0 && ld < (1 << 23); }
 
 int64_t tiles_of(int64_t m, int64_t n) { return (m + TILE - 1) / TILE * ((n + TILE - 1) / TILE); }
@@ -1046,8 +1047,8 @@ int gated_transition(const kutacc_hip_gated_transition_args_t &a, hipStream_t st
     p.c[0] = h, p.c_ld[0] = h_ld;
     p.M[0] = (int)rows, p.N[0] = (int)c_i, p.K = (int)c_o, p.activation = a.activation;
     const bool widths = c_o % 8 == 0 && c_i % 8 == 0;
-    const bool any_in = !widths || !pieces(a.x, a.x_ld, c_o) || !kutacc_hip_aligned16(a.gate_w) || !kutacc_hip_aligned16(a.up_w);
-    const bool any_out = !widths || !kutacc_hip_aligned16(a.down_w) || !pieces(a.out, a.out_ld, c_o);
+    const bool any_in = !widths || !pieces(a.x, a.x_ld, c_o) || !pieces(a.gate_w, c_o, c_o) || !pieces(a.up_w, c_o, c_o);
+    const bool any_out = !widths || !pieces(h, h_ld, c_i) || !pieces(a.down_w, c_i, c_i) || !pieces(a.out, a.out_ld, c_o);
     bf16_t *const rest = keeps_rest(rows, c_o) && !any_in && !any_out ? h + align256(2 * rows * h_ld) / 2 : nullptr;
     p.c[1] = rest;
     if (const int rc = launch<GATED>(p, any_in, 4.0 * (double)rows * (double)c_o * (double)c_i, "gated_transition<gated>", stream)) {
@@ -1085,8 +1086,8 @@ int gated_transition_backward(const kutacc_hip_gated_transition_backward_args_t 
     const bf16_t *x = (const bf16_t *)a.x, *dy = (const bf16_t *)a.grad_out;
     const bf16_t *wg = (const bf16_t *)a.gate_w, *wu = (const bf16_t *)a.up_w, *wd = (const bf16_t *)a.down_w;
     const double flops = 2.0 * (double)rows * (double)c_o * (double)c_i;
-    const bool rows_fit = pieces(x, a.x_ld, c_o) && pieces(dy, a.grad_out_ld, c_o), widths = c_o % 8 == 0 && c_i % 8 == 0;
-    const bool weights_fit = widths && kutacc_hip_aligned16(wg) && kutacc_hip_aligned16(wu);
+    const bool rows_fit = pieces(x, a.x_ld, c_o) && pieces(dy, a.grad_out_ld, c_o), hidden_fit = c_o % 8 == 0 && pieces(h, ld, c_i);
+    const bool weights_fit = hidden_fit && pieces(wg, c_o, c_o) && pieces(wu, c_o, c_o);
     TilesParams p = {};
     p.splits = 1;
     p.product[0] = {x, wg, a.x_ld, c_o};
@@ -1094,7 +1095,7 @@ int gated_transition_backward(const kutacc_hip_gated_transition_backward_args_t 
     p.product[2] = {dy, wd, a.grad_out_ld, c_i};
     p.c[0] = h, p.c[1] = dg, p.c[2] = du, p.c_ld[0] = p.c_ld[1] = p.c_ld[2] = ld;
     p.M[0] = (int)rows, p.N[0] = (int)c_i, p.K = (int)c_o, p.activation = a.activation;
-    if (const int rc = launch<HIDDEN_GRADIENTS>(p, !rows_fit || !weights_fit || !kutacc_hip_aligned16(wd), 3 * flops, "gated_transition<hidden gradients>", stream)) {
+    if (const int rc = launch<HIDDEN_GRADIENTS>(p, !rows_fit || !weights_fit || !pieces(wd, c_i, c_i), 3 * flops, "gated_transition<hidden gradients>", stream)) {
         return rc;
     }
     if (a.grad_x != nullptr) {
@@ -1125,7 +1126,7 @@ int gated_transition_backward(const kutacc_hip_gated_transition_backward_args_t 
     const bool aligned = (!a.grad_gate_w || kutacc_hip_aligned16(a.grad_gate_w)) && (!a.grad_up_w || kutacc_hip_aligned16(a.grad_up_w)) && (!a.grad_down_w || kutacc_hip_aligned16(a.grad_down_w));
     w.splits = weight_splits(rows, c_o, c_i);
     w.shares = shares;
-    return count == 0 ? 0 : launch<WEIGHT_GRADIENTS>(w, !rows_fit || !widths || !aligned, count * flops, "gated_transition<weight gradients>", stream);
+    return count == 0 ? 0 : launch<WEIGHT_GRADIENTS>(w, !rows_fit || !hidden_fit || !aligned, count * flops, "gated_transition<weight gradients>", stream);
 }
 
 } // namespace kutacc_launch
