@@ -16,11 +16,12 @@ __device__ __forceinline__ float activation_exponent(float v, int activation)
     return activation == KUTACC_HIP_GELU ? v * fmaf(-LOG2E * GELU_SLOPE * GELU_CUBE, v * v, -LOG2E * GELU_SLOPE) : -LOG2E * v;
 }
 
-// act(v) of s = sigmoid(t(v)), and its derivative
+// act(v) of s = sigmoid(t(v)), and its derivative.  From |v| = 100 on s is 0 or 1, and so is the derivative: gelu's t'(v) stays what it is there, or a large v, times
+// its square, would be an infinity times the zero of 1 - s.
 __device__ __forceinline__ float activation_of_sigmoid(float v, float s, int activation, float &derivative)
 {
-    const float a = v * s;
-    derivative = fmaf(activation == KUTACC_HIP_GELU ? a * (GELU_SLOPE * fmaf(3.f * GELU_CUBE, v * v, 1.f)) : a, 1.f - s, s);
+    const float a = v * s, rest = 1.f - s;
+    derivative = activation == KUTACC_HIP_GELU ? fmaf(a * rest, fmaf(3.f * GELU_CUBE * GELU_SLOPE, fminf(v * v, 1e4f), GELU_SLOPE), s) : fmaf(a, rest, s);
     return a;
 }
 
