@@ -270,7 +270,7 @@ __global__ __launch_bounds__(threads_of<TPR>()) void rms_norm_backward_kernel(co
         const float n = (float)p.size;
         row_sums<TPR>(squares, products, waves);
         const float r = 1.0f / sqrtf(squares / n + p.eps);
-        const float pull = r * r * (products / n);
+        const float pull = r * (r * (products / n)); // (r^2 may be past 2^128 where x r^2 is not)
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = 8 * (TPR * i + t);

@@ -4,7 +4,7 @@ import torch
 
 import feed_forward_oracle as oracle
 from kutacc_amd import capi
-from test_gpu_feed_forward import BF16, Room, cpu_randn, ok
+from test_gpu_feed_forward import BF16, FP32, Room, cpu_randn, ok
 from test_gpu_feed_forward_infinities import operands, same
 
 pytestmark = pytest.mark.gpu
@@ -44,3 +44,24 @@ def test_gated_transition_of_gates_far_from_zero(rows, c_o, c_i, scale, activati
     ok(capi.GatedTransitionBackward(x.cuda(), *gpu, dy.cuda(), activation=activation, **{k: r.view for k, r in grads.items()}))
     for name, r in grads.items():
         same(r.view, want[name][0], name)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("rows,size", [(3, 7), (5, 64), (9, 300), (4, 2051), (3, 8200)])
+def test_rms_norm_of_rows_near_zero_without_eps(dtype, rows, size):
+    """Values around 2^-66: 1 / mean(x^2) is past 32 bits, and all results are not."""
+    x, dy, gamma = cpu_randn(1, rows, size, scale=2.0 ** -66, dtype=dtype), cpu_randn(2, rows, size, dtype=dtype), 1 + 0.1 * cpu_randn(3, size, dtype=FP32)
+    # squares below 2^-126 have steps of 2^-149: the sum of squares is off by size 2^-150 beside some size 2^-132, the factor of a row by half of 2^-18 of itself, and a
+    # result by three such factors at most (r, and the r^2 of the pull), beside what the oracle counts
+    rows_off = 3 * 2.0 ** -18
+    out, dx, dgamma = Room(rows, size, dtype), Room(rows, size, dtype), Room(1, size, FP32)
+    ok(capi.RmsNorm(x.cuda(), gamma.cuda(), 0.0, out=out.view))
+    _, y = oracle.rms_norm(x, gamma, 0.0)
+    oracle.close(out.view, y, oracle.stored(y, y.abs() * (oracle.norm_slack(size) + rows_off), dtype), "out")
+    ok(capi.RmsNormBackward(x.cuda(), gamma.cuda(), dy.cuda(), 0.0, grad_x=dx.view, grad_gamma=dgamma.view[0]))
+    want, off, want_gamma, off_gamma = oracle.rms_norm_backward(x, gamma, dy, 0.0)
+    r = 1 / torch.sqrt((x.double() ** 2).mean(1, keepdim=True))
+    h = dy.double() * gamma.double()
+    terms = r * (h.abs() + x.double().abs() * r * r * (h * x.double()).abs().mean(1, keepdim=True))
+    oracle.close(dx.view, want, oracle.stored(want, off + rows_off * terms, dtype), "grad_x")
+    oracle.close(dgamma.view[0], want_gamma, off_gamma + (rows_off + 2.0 ** -24) * (dy.double() * x.double() * r).abs().sum(0), "grad_gamma")
