@@ -25,7 +25,7 @@
 namespace {
 using namespace kutacc_dev;
 
-constexpr int UNITS = 32, WAVES = 8;
+constexpr int UNITS = 32, WAVES = 8, MAX_CHANNELS = 2048; // (of channels, what leaves the LDS room for the columns of Wd)
 
 struct FewRowsParams {
     const bf16_t *x, *grad_out, *gate_w, *up_w, *down_w;
@@ -328,7 +328,8 @@ hipError_t launch(const FewRowsParams &p, hipStream_t stream)
     const auto kernel = &gated_few_rows_backward_kernel<MB, ACTIVATION>;
     constexpr size_t OPERANDS = (MB == 1 ? 6 : 5) * 2 * MB * 1024, SUMS = WAVES * 12 * 1024, BLOCKS = WAVES * (4 * MB + 4) * 1024;
     const size_t bytes = OPERANDS + std::max({SUMS, BLOCKS, (size_t)p.c_o * 64});
-    if (const hipError_t e = kutacc_opt_in_lds(reinterpret_cast<const void *>(kernel), bytes, configured)) {
+    // opted in for the widest rows at once, not for these: a later call with wider ones must not have to, in a capture or beside another thread's first call
+    if (const hipError_t e = kutacc_opt_in_lds(reinterpret_cast<const void *>(kernel), OPERANDS + std::max({SUMS, BLOCKS, (size_t)MAX_CHANNELS * 64}), configured)) {
         return e;
     }
     kernel<<<dim3((unsigned)(p.c_i / UNITS)), 64 * WAVES, bytes, stream>>>(p);
@@ -338,10 +339,10 @@ hipError_t launch(const FewRowsParams &p, hipStream_t stream)
 
 namespace kutacc_launch {
 
-// widths in blocks of 32, as many channels as leave the LDS room for the columns of Wd, and shares of no more than 16 MB
+// widths in blocks of 32, and shares of no more than 16 MB
 bool gated_few_rows_backward_fits(int64_t rows, int64_t c_o, int64_t c_i)
 {
-    return rows > 0 && rows <= 64 && c_o > 0 && c_i > 0 && c_o % 32 == 0 && c_i % 32 == 0 && c_o <= 2048 && c_i < (1 << 23) && gated_few_rows_backward_workspace(rows, c_o, c_i) <= (16 << 20);
+    return rows > 0 && rows <= 64 && c_o > 0 && c_i > 0 && c_o % 32 == 0 && c_i % 32 == 0 && c_o <= MAX_CHANNELS && c_i < (1 << 23) && gated_few_rows_backward_workspace(rows, c_o, c_i) <= (16 << 20);
 }
 
 int64_t gated_few_rows_backward_workspace(int64_t rows, int64_t c_o, int64_t c_i) { return c_i / UNITS * rows * c_o * 4; }
