@@ -424,8 +424,9 @@ kutacc_export int kutacc_hip_msa_attention(const kutacc_hip_msa_attention_args_t
 
 /* ---- the feed-forward half of a transformer block (no counterpart in the reference) ----
  *
- * Calls enqueue their kernels on `stream` and return 0, a hipError_t, KUTACC_HIP_EINVAL or KUTACC_HIP_EUNSUPPORTED.  A first call on a device raises a kernel's
- * dynamic-LDS limit: make one per shape outside stream capture.  Captured calls can be replayed.  A workspace is one call's at a time. */
+ * Calls enqueue their kernels on `stream` and return 0, a hipError_t, KUTACC_HIP_EINVAL or KUTACC_HIP_EUNSUPPORTED (a shape that has no kernel, or a product of more
+ * tiles than a launch has threads for, 2^32: results of some 2^38 values, or one row of 2^29).  A first call on a device raises a kernel's dynamic-LDS limit: make
+ * one per shape outside stream capture.  Captured calls can be replayed.  A workspace is one call's at a time. */
 
 /*
  * RMS norm with the residual's addition, row by row:

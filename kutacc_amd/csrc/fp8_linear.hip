@@ -296,7 +296,7 @@ template <typename T, int MB, int NB, int W>
 int launch_any(LinearParams p, hipStream_t stream)
 {
     const int64_t groups = tiles_of(p, 16 * MB, 16 * NB);
-    if (groups > INT32_MAX) {
+    if (!kutacc_grid_fits(groups, 64 * W)) {
         return KUTACC_HIP_EUNSUPPORTED;
     }
     p.NT = (p.N + 16 * NB - 1) / (16 * NB);
@@ -508,7 +508,7 @@ int launch_split(LinearParams p, hipStream_t stream)
     static size_t configured[KUTACC_DEVICE_SLOTS] = {};
     const auto kernel = &fp8_split_kernel<T, MB, NB, W, DEPTH, ANY>;
     const int64_t groups = tiles_of(p, 16 * MB, 16 * NB);
-    if (groups > INT32_MAX) {
+    if (!kutacc_grid_fits(groups, 64 * W)) {
         return KUTACC_HIP_EUNSUPPORTED;
     }
     p.NT = (p.N + 16 * NB - 1) / (16 * NB);
@@ -752,7 +752,7 @@ int launch_tiles(LinearParams p, hipStream_t stream)
     const auto kernel = &fp8_tiles_kernel<T, MI, WM, WN, ANY>;
     p.MT = (p.M + SIDE - 1) / SIDE, p.NT = (p.N + SIDE - 1) / SIDE;
     const int64_t tiles = tiles_of(p, SIDE, SIDE);
-    if (tiles > INT32_MAX) {
+    if (!kutacc_grid_fits(tiles, 64 * WM * WN)) {
         return KUTACC_HIP_EUNSUPPORTED;
     }
     if (const hipError_t e = kutacc_opt_in_lds(reinterpret_cast<const void *>(kernel), tiles_lds(SIDE), configured)) {

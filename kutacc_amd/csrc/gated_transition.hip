@@ -826,20 +826,28 @@ int launch_any(TilesParams p, double flops, const char *name, hipStream_t stream
     for (int i = 0; i < 3; ++i) {
         const int64_t tiles = tiles_of(p.M[i], p.N[i]);
         blocks += tiles;
-        if (blocks > INT32_MAX) {
-            return KUTACC_HIP_EUNSUPPORTED;
+        p.tiles[i] = (int)std::min<int64_t>(tiles, INT32_MAX);
+    }
+    if (MODE == WEIGHT_GRADIENTS && p.M[1] != 0 && !kutacc_grid_fits(blocks * p.splits, 256)) { // one by one
+        for (int i = 0; i < 3 && p.M[i] != 0; ++i) {
+            TilesParams one = p;
+            one.product[0] = p.product[i], one.c[0] = p.c[i], one.c_ld[0] = p.c_ld[i], one.M[0] = p.M[i], one.N[0] = p.N[i];
+            one.M[1] = one.M[2] = 0;
+            if (const int rc = launch_any<MODE>(one, flops / 3, name, stream)) {
+                return rc;
+            }
         }
-        p.tiles[i] = (int)tiles;
+        return 0;
     }
     const bool tiny = std::min(p.N[0], MODE == WEIGHT_GRADIENTS ? p.M[0] : p.K) < 8; // contiguous extents
     const auto kernel = tiny ? &ff_tiles_kernel<MODE, true> : &ff_tiles_kernel<MODE, false>;
     if (const hipError_t e = kutacc_opt_in_lds(reinterpret_cast<const void *>(kernel), TILES_LDS, configured[tiny])) {
         return kutacc_hip_status(e);
     }
-    kutacc_prof::KernelTimer t(name, flops, stream);
-    if (blocks * p.splits > INT32_MAX) {
+    if (!kutacc_grid_fits(blocks * p.splits, 256)) {
         return KUTACC_HIP_EUNSUPPORTED;
     }
+    kutacc_prof::KernelTimer t(name, flops, stream);
     kernel<<<dim3((unsigned)(blocks * p.splits)), 256, TILES_LDS, stream>>>(p);
     if ((MODE == WEIGHT_GRADIENTS || MODE == INPUT_GRADIENT) && p.splits > 1) {
         ff_shares_kernel<2, 2, 2><<<dim3((unsigned)(blocks * 16)), 256, 0, stream>>>(p);
@@ -867,7 +875,7 @@ int launch_pieces(TilesParams p, hipStream_t stream)
     static size_t configured[KUTACC_DEVICE_SLOTS] = {};
     const auto kernel = &ff_pieces_kernel<MODE, MI, WM, WN, GROUPS>;
     const int64_t tiles = count_tiles(p, ROWS, MODE == GATED || MODE == HIDDEN_GRADIENTS ? SIDE / 2 : SIDE), groups = tiles * p.splits;
-    if (groups > INT32_MAX) {
+    if (!kutacc_grid_fits(groups, 64 * WM * WN * GROUPS)) {
         return KUTACC_HIP_EUNSUPPORTED;
     }
     if (const hipError_t e = kutacc_opt_in_lds(reinterpret_cast<const void *>(kernel), LDS, configured)) {
@@ -889,7 +897,7 @@ int launch_split(TilesParams p, hipStream_t stream)
     static size_t configured[KUTACC_DEVICE_SLOTS] = {};
     const auto kernel = &ff_split_kernel<MODE, MB, NB, W, DEPTH, WITH_REST>;
     const int64_t groups = count_tiles(p, WITH_REST ? 8 * MB : 16 * MB, 16 * NB);
-    if (groups > INT32_MAX) {
+    if (!kutacc_grid_fits(groups, 64 * W)) {
         return KUTACC_HIP_EUNSUPPORTED;
     }
     if (const hipError_t e = kutacc_opt_in_lds(reinterpret_cast<const void *>(kernel), LDS, configured)) {
@@ -902,21 +910,21 @@ int launch_split(TilesParams p, hipStream_t stream)
 // whether the weights' gradients make enough tiles of 256 x 256 without a split of their rows
 bool whole_rows(TilesParams p) { return 4 * count_tiles(p, 256, 256) >= 3 * kutacc_cu_count(); }
 
-// A kernel's tile, how many of its workgroups a CU holds, and what a round of them takes for 64 k
+// A kernel's tile, its threads, how many of its workgroups a CU holds, and what a round of them takes for 64 k
 struct Choice {
-    int rows, columns, per_cu;
+    int rows, columns, threads, per_cu;
     float round;
 };
-// the one that takes the fewest rounds, weighted with what they take
+// of those that can be started, the one that takes the fewest rounds, weighted with what they take
 template <int N>
 int least(TilesParams p, const Choice (&choices)[N])
 {
     int best = 0;
     double time = 0;
     for (int i = 0; i < N; ++i) {
-        const int64_t slots = (int64_t)kutacc_cu_count() * choices[i].per_cu;
-        const double t = (double)((count_tiles(p, choices[i].rows, choices[i].columns) + slots - 1) / slots) * choices[i].round;
-        if (i == 0 || t < time) {
+        const int64_t tiles = count_tiles(p, choices[i].rows, choices[i].columns), slots = (int64_t)kutacc_cu_count() * choices[i].per_cu;
+        const double t = (double)((tiles + slots - 1) / slots) * choices[i].round;
+        if (kutacc_grid_fits(tiles, choices[i].threads) && (time == 0 || t < time)) {
             best = i, time = t;
         }
     }
@@ -935,7 +943,7 @@ int launch_whole(const TilesParams &p, hipStream_t stream)
         if (p.M[0] <= 16) {
             return launch_split<MODE, 1, 1, 16, 2>(p, stream);
         }
-        constexpr Choice choices[] = {{32, 32, 1, 0.10f}, {32, 64, 1, 0.13f}, {64, 64, 1, 0.23f}, {128, 128, 1, 0.66f}, {128, 128, 2, 1.05f}, {192, 256, 1, 1.41f}, {256, 256, 1, 1.70f}};
+        constexpr Choice choices[] = {{32, 32, 1024, 1, 0.10f}, {32, 64, 512, 1, 0.13f}, {64, 64, 512, 1, 0.23f}, {128, 128, 512, 1, 0.66f}, {128, 128, 256, 2, 1.05f}, {192, 256, 512, 1, 1.41f}, {256, 256, 512, 1, 1.70f}};
         switch (least(p, choices)) {
         case 0: return launch_split<MODE, 2, 2, 16, 1>(p, stream);
         case 1: return launch_split<MODE, 2, 4, 8, 1>(p, stream);
@@ -952,7 +960,7 @@ int launch_whole(const TilesParams &p, hipStream_t stream)
         if (p.c[1] != nullptr) {
             return launch_split<MODE, 2, 2, 8, 1>(p, stream);
         }
-        constexpr Choice choices[] = {{32, 32, 1, 0.23f}, {64, 32, 1, 0.33f}, {128, 64, 2, 1.15f}, {192, 128, 1, 1.45f}, {256, 128, 1, 1.90f}};
+        constexpr Choice choices[] = {{32, 32, 512, 1, 0.23f}, {64, 32, 512, 1, 0.33f}, {128, 64, 256, 2, 1.15f}, {192, 128, 512, 1, 1.45f}, {256, 128, 512, 1, 1.90f}};
         switch (least(p, choices)) {
         case 0: return launch_split<MODE, 2, 2, 8, 1>(p, stream);
         case 1: return launch_split<MODE, 4, 2, 8, 1>(p, stream);
@@ -961,13 +969,13 @@ int launch_whole(const TilesParams &p, hipStream_t stream)
         default: return launch_pieces<MODE, 4, 2, 4, 1>(p, stream);
         }
     } else if constexpr (MODE == HIDDEN_GRADIENTS) {
-        constexpr Choice choices[] = {{128, 64, 2, 1.0f}, {192, 128, 1, 1.27f}};
+        constexpr Choice choices[] = {{128, 64, 256, 2, 1.0f}, {192, 128, 512, 1, 1.27f}};
         return least(p, choices) == 0 ? launch_pieces<MODE, 2, 2, 2, 1>(p, stream) : launch_pieces<MODE, 3, 2, 4, 1>(p, stream);
     } else if constexpr (MODE == INPUT_GRADIENT) {
         if (p.splits > 1) {
             return launch_pieces<MODE, 2, 2, 2, 1>(p, stream);
         }
-        constexpr Choice choices[] = {{128, 128, 1, 0.61f}, {128, 128, 2, 0.97f}, {256, 256, 1, 1.55f}};
+        constexpr Choice choices[] = {{128, 128, 512, 1, 0.61f}, {128, 128, 256, 2, 0.97f}, {256, 256, 512, 1, 1.55f}};
         switch (least(p, choices)) {
         case 0: return launch_pieces<MODE, 2, 2, 2, 2>(p, stream);
         case 1: return launch_pieces<MODE, 2, 2, 2, 1>(p, stream);
@@ -1047,7 +1055,7 @@ int gated_transition(const kutacc_hip_gated_transition_args_t &a, hipStream_t st
     p.c[0] = h, p.c_ld[0] = h_ld;
     p.M[0] = (int)rows, p.N[0] = (int)c_i, p.K = (int)c_o, p.activation = a.activation;
     const bool widths = c_o % 8 == 0 && c_i % 8 == 0;
-    const bool any_in = !widths || !pieces(a.x, a.x_ld, c_o) || !pieces(a.gate_w, c_o, c_o) || !pieces(a.up_w, c_o, c_o);
+    const bool any_in = !widths || !pieces(h, h_ld, c_i) || !pieces(a.x, a.x_ld, c_o) || !pieces(a.gate_w, c_o, c_o) || !pieces(a.up_w, c_o, c_o);
     const bool any_out = !widths || !pieces(h, h_ld, c_i) || !pieces(a.down_w, c_i, c_i) || !pieces(a.out, a.out_ld, c_o);
     bf16_t *const rest = keeps_rest(rows, c_o) && !any_in && !any_out ? h + align256(2 * rows * h_ld) / 2 : nullptr;
     p.c[1] = rest;

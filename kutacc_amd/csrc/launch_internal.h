@@ -68,6 +68,9 @@ static inline int kutacc_cu_count()
     return kutacc_device_attribute(hipDeviceAttributeMultiprocessorCount, 256, table);
 }
 
+// Whether workgroups along x can be started: below 2^31 of them and 2^32 threads
+static inline bool kutacc_grid_fits(int64_t blocks, int threads) { return blocks <= INT32_MAX && blocks * threads <= (int64_t)UINT32_MAX; }
+
 namespace kutacc_launch {
 
 // generic_kernels.hip

@@ -465,18 +465,24 @@ namespace kutacc_launch {
 
 int rms_norm(const kutacc_hip_rms_norm_args_t &a, hipStream_t stream)
 {
-    const NormParams p = {a.x, a.residual, a.sum, a.out, (uint8_t *)a.out8, a.gamma, a.scales,
-                          a.x_ld, a.residual_ld, a.sum_ld, a.out_ld, a.out8_ld, a.scales_ld, a.rows, (int)a.size, a.eps};
     return by_type(a.dtype, [&](auto type) {
         return by_size(a.size, [&](auto tpr, auto nv) {
-            constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, THREADS = threads_of<TPR>();
-            const int64_t blocks = (p.rows + THREADS / TPR - 1) / (THREADS / TPR);
-            if (blocks > INT32_MAX) {
-                return KUTACC_HIP_EUNSUPPORTED;
+            using T = decltype(type);
+            constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, THREADS = threads_of<TPR>(), PER_GROUP = THREADS / TPR;
+            constexpr int64_t MOST = (int64_t)(UINT32_MAX / THREADS) * PER_GROUP; // rows of a launch
+            kutacc_prof::KernelTimer t("rms_norm_kernel", 8.0 * (double)a.rows * (double)a.size, stream);
+            for (int64_t first = 0; first < a.rows; first += MOST) {
+                const auto from = [&](auto *rows, int64_t ld) { return rows != nullptr ? rows + first * ld : nullptr; };
+                const int64_t rows = std::min(a.rows - first, MOST);
+                const NormParams p = {from((const T *)a.x, a.x_ld), from((const T *)a.residual, a.residual_ld), from((T *)a.sum, a.sum_ld), from((T *)a.out, a.out_ld),
+                                      from((uint8_t *)a.out8, a.out8_ld), a.gamma, from(a.scales, a.scales_ld),
+                                      a.x_ld, a.residual_ld, a.sum_ld, a.out_ld, a.out8_ld, a.scales_ld, rows, (int)a.size, a.eps};
+                rms_norm_kernel<T, TPR, NV><<<dim3((unsigned)((rows + PER_GROUP - 1) / PER_GROUP)), THREADS, 0, stream>>>(p);
+                if (const hipError_t e = hipGetLastError()) {
+                    return kutacc_hip_status(e);
+                }
             }
-            kutacc_prof::KernelTimer t("rms_norm_kernel", 8.0 * (double)p.rows * (double)p.size, stream);
-            rms_norm_kernel<decltype(type), TPR, NV><<<dim3((unsigned)blocks), THREADS, 0, stream>>>(p);
-            return kutacc_hip_status(hipGetLastError());
+            return 0;
         });
     });
 }
@@ -512,19 +518,23 @@ int quantize_fp8(const void *x, int64_t x_ld, void *out, int64_t out_ld, float *
                  int32_t block_rows, int32_t dtype, hipStream_t stream)
 {
     const int across = (int)((size + FP8_BLOCK - 1) / FP8_BLOCK);
-    const QuantizeParams p = {x, (uint8_t *)out, scales, x_ld, out_ld, scales_ld, rows, (int)size, across};
-    const int64_t blocks = block_rows == 1 ? (rows * across + 15) / 16 : (rows + FP8_BLOCK - 1) / FP8_BLOCK * across;
-    if (blocks > INT32_MAX) {
-        return KUTACC_HIP_EUNSUPPORTED;
-    }
+    const int64_t groups = UINT32_MAX / 256, most = block_rows == 1 ? groups * 16 / across : groups / across * FP8_BLOCK; // rows of a launch
     return by_type(dtype, [&](auto type) {
+        using T = decltype(type);
         kutacc_prof::KernelTimer t("quantize_fp8_kernel", (double)rows * (double)size, stream);
-        if (block_rows == 1) {
-            quantize_fp8_kernel<decltype(type), 1><<<dim3((unsigned)blocks), 256, 0, stream>>>(p);
-        } else {
-            quantize_fp8_kernel<decltype(type), FP8_BLOCK><<<dim3((unsigned)blocks), 256, 0, stream>>>(p);
+        for (int64_t first = 0; first < rows; first += most) {
+            const int64_t count = std::min(rows - first, most);
+            const QuantizeParams p = {(const T *)x + first * x_ld, (uint8_t *)out + first * out_ld, scales + first / block_rows * scales_ld, x_ld, out_ld, scales_ld, count, (int)size, across};
+            if (block_rows == 1) {
+                quantize_fp8_kernel<T, 1><<<dim3((unsigned)((count * across + 15) / 16)), 256, 0, stream>>>(p);
+            } else {
+                quantize_fp8_kernel<T, FP8_BLOCK><<<dim3((unsigned)((count + FP8_BLOCK - 1) / FP8_BLOCK * across)), 256, 0, stream>>>(p);
+            }
+            if (const hipError_t e = hipGetLastError()) {
+                return kutacc_hip_status(e);
+            }
         }
-        return kutacc_hip_status(hipGetLastError());
+        return 0;
     });
 }
 

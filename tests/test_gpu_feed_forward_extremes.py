@@ -4,7 +4,7 @@ import torch
 
 import feed_forward_oracle as oracle
 from kutacc_amd import capi
-from test_gpu_feed_forward import BF16, FP32, Room, cpu_randn, ok
+from test_gpu_feed_forward import BF16, E4M3, EPS, FP32, Room, cpu_randn, ok, weights_of
 from test_gpu_feed_forward_infinities import operands, same
 
 pytestmark = pytest.mark.gpu
@@ -65,3 +65,60 @@ def test_rms_norm_of_rows_near_zero_without_eps(dtype, rows, size):
     terms = r * (h.abs() + x.double().abs() * r * r * (h * x.double()).abs().mean(1, keepdim=True))
     oracle.close(dx.view, want, oracle.stored(want, off + rows_off * terms, dtype), "grad_x")
     oracle.close(dgamma.view[0], want_gamma, off_gamma + (rows_off + 2.0 ** -24) * (dy.double() * x.double() * r).abs().sum(0), "grad_gamma")
+
+
+def edges(rows, around):
+    """The first and the last rows, and those on either side of `around`."""
+    return torch.cat([torch.arange(40), torch.arange(around - 40, around + 40), torch.arange(rows - 40, rows)])
+
+
+def test_rms_norm_of_more_rows_than_a_launch_has_threads():
+    """Eight threads a row: the second of two launches begins behind (2^32 - 1) / 256 workgroups of 32 rows."""
+    part = (2 ** 32 - 1) // 256 * 32
+    rows, size = part + 1000, 2
+    picked = edges(rows, part)
+    x, gamma = cpu_randn(1, len(picked), size), 1 + 0.1 * cpu_randn(2, size, dtype=FP32)
+    gx, out = torch.zeros(rows, size, device="cuda", dtype=BF16), torch.full((rows, size), 77.0, device="cuda", dtype=BF16)
+    gx[picked] = x.cuda()
+    out8, scales = torch.full((rows, size), 0x33, device="cuda", dtype=torch.uint8).view(E4M3), torch.full((rows, 1), 77.0, device="cuda")
+    ok(capi.RmsNorm(gx, gamma.cuda(), EPS, out=out, out8=out8, scales=scales))
+    near = [torch.empty(len(picked), size, device="cuda", dtype=t) for t in (BF16, E4M3)] + [torch.empty(len(picked), 1, device="cuda")]
+    ok(capi.RmsNorm(x.cuda(), gamma.cuda(), EPS, out=near[0], out8=near[1], scales=near[2]))
+    for got, want in zip((out, out8, scales), near):
+        assert torch.equal(got.view(torch.uint8)[picked.cuda()], want.view(torch.uint8))
+    _, y = oracle.rms_norm(x, gamma, EPS)
+    oracle.close(near[0], y, oracle.stored(y, y.abs() * oracle.norm_slack(size), BF16) + 1e-40, "out")
+    assert int(out.count_nonzero()) == int(near[0].count_nonzero()) and int(out8.view(torch.uint8).count_nonzero()) == int(near[1].view(torch.uint8).count_nonzero())
+    assert int((scales == 2.0 ** -126).sum()) == rows - len(picked)
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantiser_of_more_rows_than_a_launch_has_threads(block_rows):
+    """16 threads a row, or two a row of a block of 128."""
+    part = (2 ** 32 - 1) // 256 * (16 if block_rows == 1 else 128)
+    rows, size = part + 1000, 1
+    picked = edges(rows, part)
+    x = torch.zeros(rows, size, dtype=BF16, device="cuda")
+    x[picked] = cpu_randn(1, len(picked), size).cuda()
+    out, scales = torch.full((rows, size), 0x33, device="cuda", dtype=torch.uint8).view(E4M3), torch.full((-(-rows // block_rows), 1), 77.0, device="cuda")
+    ok(capi.QuantizeFp8(x, out, scales, block_rows))
+    blocks = torch.unique(picked // block_rows)
+    for b in blocks.tolist():
+        at = slice(b * block_rows, min((b + 1) * block_rows, rows))
+        want_q, want_s = oracle.quantise(x[at], block_rows)
+        assert torch.equal(scales[b].cpu(), want_s[0]) and torch.equal(out[at].cpu().float(), want_q.float()), b
+    assert int((scales == 2.0 ** -126).sum()) == scales.numel() - len(blocks) and int(out.view(torch.uint8).count_nonzero()) == int(x.count_nonzero())
+
+
+def test_gated_transition_of_more_rows_than_small_tiles_have_threads():
+    """134 million rows of eight channels: 2^32 threads in tiles of 32 rows, which would be chosen."""
+    rows, c = (1 << 27) + 333, 8
+    picked = edges(rows, 1 << 27)
+    w, x = weights_of(3, c, c), cpu_randn(1, len(picked), c)
+    gx, out = torch.zeros(rows, c, device="cuda", dtype=BF16), torch.full((rows, c), 77.0, device="cuda", dtype=BF16)
+    gx[picked] = x.cuda()
+    ok(capi.GatedTransition(gx, *(t.cuda() for t in w), out))
+    want, off = oracle.gated_transition(x, *w, "silu")["out"]
+    oracle.close(out[picked.cuda()], want, oracle.stored(want, off, BF16), "out")
+    out[picked.cuda()] = 0
+    assert not bool(out.any())
