@@ -650,11 +650,23 @@ def _dense(t, shape, dtype, what):
     return t.data_ptr()
 
 
-def _one_device(*tensors):
-    """All on one device: the library's calls run on the current one."""
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) != 1:
-        raise ValueError(f"operands on {sorted(map(str, devices))}")
+class _DeviceCall:
+    """A call on tensors of one device, which has to be the current one where the call is made: there the library launches."""
+
+    def _on(self, *tensors):
+        import torch
+        devices = {t.device for t in tensors if t is not None}
+        if len(devices) != 1:
+            raise ValueError(f"operands on {sorted(map(str, devices))}")
+        (device,) = devices
+        # with one GPU in sight its tensors are on the current device
+        self.checked_device = None if device.type == "cuda" and torch.cuda.device_count() == 1 else device
+
+    def _check_device(self):
+        if self.checked_device is not None:
+            import torch
+            if self.checked_device.type != "cuda" or self.checked_device.index != torch.cuda.current_device():
+                raise ValueError(f"operands on {self.checked_device}, which is not the current GPU")
 
 
 def _workspace(nbytes, device):
@@ -664,14 +676,14 @@ def _workspace(nbytes, device):
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
-class RmsNorm:
+class RmsNorm(_DeviceCall):
     """One kutacc_hip_rms_norm call on device tensors: x, residual, sum and out [rows, size] in bf16 or fp32, gamma fp32 [size], out8
     [rows, size] in torch.float8_e4m3fn with scales fp32 [rows, ceil(size / 128)].  Rows contiguous, any row stride.  Each but x may be None, not
     all results.  `run()` returns the library's code."""
 
     def __init__(self, x, gamma, eps=1e-6, residual=None, sum=None, out=None, out8=None, scales=None):
         import torch
-        _one_device(x, gamma, residual, sum, out, out8, scales)
+        self._on(x, gamma, residual, sum, out, out8, scales)
         self.keep = (x, gamma, residual, sum, out, out8, scales)
         a = HipRmsNormArgs()
         a.rows, a.size = x.shape
@@ -686,16 +698,17 @@ class RmsNorm:
         self.args = a
 
     def run(self, stream_ptr=None) -> int:
+        self._check_device()
         return lib().kutacc_hip_rms_norm(ctypes.byref(self.args), stream_ptr)
 
 
-class RmsNormBackward:
+class RmsNormBackward(_DeviceCall):
     """One kutacc_hip_rms_norm_backward call: x (what was normalised), grad_out, grad_sum and grad_x [rows, size], gamma and grad_gamma fp32
     [size].  Owns the workspace."""
 
     def __init__(self, x, gamma, grad_out, eps=1e-6, grad_sum=None, grad_x=None, grad_gamma=None):
         import torch
-        _one_device(x, gamma, grad_out, grad_sum, grad_x, grad_gamma)
+        self._on(x, gamma, grad_out, grad_sum, grad_x, grad_gamma)
         a = HipRmsNormBackwardArgs()
         a.rows, a.size = x.shape
         a.dtype, a.eps = _torch_dtype_code(x), eps
@@ -711,32 +724,34 @@ class RmsNormBackward:
         self.args = a
 
     def run(self, stream_ptr=None) -> int:
+        self._check_device()
         return lib().kutacc_hip_rms_norm_backward(ctypes.byref(self.args), stream_ptr)
 
 
-class QuantizeFp8:
+class QuantizeFp8(_DeviceCall):
     """One kutacc_hip_quantize_fp8 call: x [rows, size] in bf16 or fp32 -> out in torch.float8_e4m3fn and fp32 scales for blocks of `block_rows` (1:
     activations, 128: weights) by 128."""
 
     def __init__(self, x, out, scales, block_rows=1):
         import torch
-        _one_device(x, out, scales)
+        self._on(x, out, scales)
         rows, size = x.shape
         self.keep = (x, out, scales)
         self.args = (*_rows(x, x.shape, (torch.bfloat16, torch.float32), "x"), *_rows(out, x.shape, torch.float8_e4m3fn, "out"),
                      *_rows(scales, (-(-rows // block_rows), -(-size // 128)), torch.float32, "scales"), rows, size, block_rows, _torch_dtype_code(x))
 
     def run(self, stream_ptr=None) -> int:
+        self._check_device()
         return lib().kutacc_hip_quantize_fp8(*self.args, stream_ptr)
 
 
-class LinearFp8:
+class LinearFp8(_DeviceCall):
     """One kutacc_hip_linear_fp8 call: a [m, k] and w [n, k] in torch.float8_e4m3fn, a_scales [m, ceil(k / 128)] and w_scales [ceil(n / 128),
     ceil(k / 128)], bias [n] fp32, out [m, n] in bf16 or fp32."""
 
     def __init__(self, a, a_scales, w, w_scales, out, bias=None):
         import torch
-        _one_device(a, a_scales, w, w_scales, out, bias)
+        self._on(a, a_scales, w, w_scales, out, bias)
         self.keep = (a, a_scales, w, w_scales, out, bias)
         g = HipLinearFp8Args()
         (g.m, g.k), g.n, g.dtype = a.shape, w.shape[0], _torch_dtype_code(out)
@@ -750,16 +765,17 @@ class LinearFp8:
         self.args = g
 
     def run(self, stream_ptr=None) -> int:
+        self._check_device()
         return lib().kutacc_hip_linear_fp8(ctypes.byref(self.args), stream_ptr)
 
 
-class GatedTransition:
+class GatedTransition(_DeviceCall):
     """One kutacc_hip_gated_transition call: x and out [rows, c_o], gate_w and up_w [c_i, c_o], down_w [c_o, c_i], all bf16; activation "silu" or
     "gelu".  Owns the workspace."""
 
     def __init__(self, x, gate_w, up_w, down_w, out, activation="silu"):
         import torch
-        _one_device(x, gate_w, up_w, down_w, out)
+        self._on(x, gate_w, up_w, down_w, out)
         bf16 = torch.bfloat16
         a = HipGatedTransitionArgs()
         (a.rows, a.c_o), a.c_i, a.dtype, a.activation = x.shape, gate_w.shape[0], K_BF16, ACTIVATIONS[activation]
@@ -773,16 +789,17 @@ class GatedTransition:
         self.args = a
 
     def run(self, stream_ptr=None) -> int:
+        self._check_device()
         return lib().kutacc_hip_gated_transition(ctypes.byref(self.args), stream_ptr)
 
 
-class GatedTransitionBackward:
+class GatedTransitionBackward(_DeviceCall):
     """One kutacc_hip_gated_transition_backward call: the gradients of x and of the three weights (each may be None, not all) from grad_out and
     the forward pass's inputs.  Owns the workspace."""
 
     def __init__(self, x, gate_w, up_w, down_w, grad_out, grad_x=None, grad_gate_w=None, grad_up_w=None, grad_down_w=None, activation="silu"):
         import torch
-        _one_device(x, gate_w, up_w, down_w, grad_out, grad_x, grad_gate_w, grad_up_w, grad_down_w)
+        self._on(x, gate_w, up_w, down_w, grad_out, grad_x, grad_gate_w, grad_up_w, grad_down_w)
         bf16 = torch.bfloat16
         a = HipGatedTransitionBackwardArgs()
         (a.rows, a.c_o), a.c_i, a.dtype, a.activation = x.shape, gate_w.shape[0], K_BF16, ACTIVATIONS[activation]
@@ -799,4 +816,5 @@ class GatedTransitionBackward:
         self.args = a
 
     def run(self, stream_ptr=None) -> int:
+        self._check_device()
         return lib().kutacc_hip_gated_transition_backward(ctypes.byref(self.args), stream_ptr)

@@ -46,3 +46,37 @@ def test_transition_owner_refuses_wrong_tensors():
         capi.GatedTransition(x, wide, wide, tall, e(4, 64), activation="relu")
     with pytest.raises(ValueError):
         capi.GatedTransitionBackward(x, wide, wide, tall, e(4, 64), grad_gate_w=tall)
+
+
+def owners():
+    f32 = torch.float32
+    x, wide, tall, q, scales = e(4, 64), e(96, 64), e(64, 96), e(4, 64, dtype=E4M3), e(4, 1, dtype=f32)
+    return [capi.RmsNorm(x, None, out=e(4, 64)), capi.RmsNormBackward(x, None, e(4, 64), grad_x=e(4, 64)), capi.QuantizeFp8(x, q, scales),
+            capi.LinearFp8(q, scales, e(96, 64, dtype=E4M3), e(1, 1, dtype=f32), e(4, 96)), capi.GatedTransition(x, wide, wide, tall, e(4, 64)),
+            capi.GatedTransitionBackward(x, wide, wide, tall, e(4, 64), grad_x=e(4, 64))]
+
+
+def test_owners_of_host_tensors_do_not_run(monkeypatch):
+    """Nothing reaches the library, which would take the addresses for a device's."""
+    calls = owners()
+    monkeypatch.setattr(capi, "lib", lambda: pytest.fail("the library was called"))
+    for call in calls:
+        with pytest.raises(ValueError, match="not the current GPU"):
+            call.run()
+
+
+def test_owners_run_on_their_own_device_alone(monkeypatch):
+    calls = owners()
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *args: 0
+
+    monkeypatch.setattr(capi, "lib", Library)
+    for call in calls:
+        call.checked_device = torch.device("cuda", 0)
+        with pytest.raises(ValueError, match="cuda:0"):
+            call.run()
+        call.checked_device = torch.device("cuda", 1)
+        assert call.run() == 0
