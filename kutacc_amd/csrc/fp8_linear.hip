@@ -312,17 +312,17 @@ __device__ __forceinline__ void load_dword_to_lds(uint32_t to, const void *from,
 
 // ---- few rows, or few tiles: the same, but a wave brings its blocks into a part of the LDS of its own ----
 //
-// Eight rows of 128 bytes a load, straight there, DEPTH blocks ahead and without barriers.  (In the order of the operands, 16 bytes of another row in every
-// lane, a load takes the address path some 42 cycles instead of 16.)  Scales come the same way, a lane for each row.  With ANY, where rows are not whole
+// Eight rows of 128 bytes a load, straight there, the next block while this one is multiplied, and without barriers.  (In the order of the operands, 16 bytes of
+// another row in every lane, a load takes the address path some 42 cycles instead of 16.)  Scales come the same way, a lane for each row.  With ANY, where rows are not whole
 // 16-byte pieces, a block passes through registers: it is asked for when the operands of the one before are in theirs, and goes into the LDS behind its
 // products; past a row's end it is as in the tiles below.  (us, so and with the operands' order: 1000 x 200 x 8001 18 and 86, 16 x 3001 x 8001 10 and 22,
 // 1 x 4097 x 4097 7.8 and 10.9, 40 x 3001 x 2001 7.0 and 21.)
-template <typename T, int MB, int NB, int W, int DEPTH, bool ANY>
+template <typename T, int MB, int NB, int W, bool ANY>
 __global__ __launch_bounds__(64 * W) void fp8_split_kernel(const LinearParams p)
 {
     constexpr bool WIDE = std::is_same<T, float>::value || MB == 1; // full fp32 sums, also where memory bounds the time anyway
-    constexpr int SLOTS = (MB + NB) * 128 + 16, LOADS = 2 * (MB + NB) + 1; // of a block: operands and 64 scales
-    extern __shared__ uint4 lds[]; // [W][DEPTH][SLOTS], and at the end sums [W][NB][MB][64]
+    constexpr int SLOTS = (MB + NB) * 128 + 16; // of a block: operands and 64 scales
+    extern __shared__ uint4 lds[];              // [W][SLOTS], and at the end sums [W][NB][MB][64]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, q = lane >> 4;
     const int n0 = (int)(blockIdx.x % (unsigned)p.NT) * 16 * NB, m0 = (int)(blockIdx.x / (unsigned)p.NT) * 16 * MB;
@@ -340,9 +340,8 @@ __global__ __launch_bounds__(64 * W) void fp8_split_kernel(const LinearParams p)
     }
     const uint32_t scale_from = 4u * (uint32_t)min(lane, min(16 * MB, p.M - m0) - 1) * (uint32_t)p.a_scales_ld;
     const float *a_scales = p.a_scales + (int64_t)m0 * p.a_scales_ld, *w_scales = p.w_scales + (int64_t)(n0 / FP8_BLOCK) * p.w_scales_ld;
-    uint4 *mine = lds + wave * DEPTH * SLOTS;
+    uint4 *mine = lds + wave * SLOTS;
     const uint32_t to = (uint32_t)(uintptr_t)(const lds_char *)mine;
-    static_assert(!ANY || DEPTH == 1, "one block is in registers");
     uint4 held[ANY ? 2 * (MB + NB) : 1];
     float held_scale;
     auto past_end = [&](int b) { return max(0, 16 * chunk + 16 - (p.K - b * FP8_BLOCK)); };
@@ -362,7 +361,7 @@ __global__ __launch_bounds__(64 * W) void fp8_split_kernel(const LinearParams p)
             }
         }
     };
-    auto ask = [&](int b, int slot) {
+    auto ask = [&](int b) {
         if constexpr (ANY) {
             const int64_t at = (int64_t)b * FP8_BLOCK - past_end(b);
             held_scale = *reinterpret_cast<const float *>(reinterpret_cast<const char *>(a_scales + b) + scale_from);
@@ -376,7 +375,7 @@ __global__ __launch_bounds__(64 * W) void fp8_split_kernel(const LinearParams p)
             }
             return;
         }
-        const uint32_t stage = to + (uint32_t)slot * (SLOTS * 16u);
+        const uint32_t stage = (uint32_t)__builtin_amdgcn_readfirstlane((int)to); // (known to be the same in all lanes, the compiler keeps its sums in vector registers)
         load_dword_to_lds(stage + (MB + NB) * 2048u, a_scales + b, scale_from);
         if (16 * chunk < p.K - b * FP8_BLOCK) {
 #pragma unroll
@@ -390,7 +389,7 @@ __global__ __launch_bounds__(64 * W) void fp8_split_kernel(const LinearParams p)
         } else { // of a cut block, past the end
 #pragma unroll
             for (int u = 0; u < 2 * (MB + NB); ++u) {
-                mine[slot * SLOTS + u * 64 + lane] = zero_u4();
+                mine[u * 64 + lane] = zero_u4();
             }
         }
     };
@@ -402,31 +401,22 @@ __global__ __launch_bounds__(64 * W) void fp8_split_kernel(const LinearParams p)
             acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
     }
-#pragma unroll
-    for (int d = 0; d < DEPTH; ++d) {
-        if (wave + d * W < blocks) {
-            ask(wave + d * W, d);
-            park(wave + d * W);
-        }
+    if (wave < blocks) {
+        ask(wave);
+        park(wave);
     }
     float w_scale = wave < blocks ? w_scales[wave] : 0.f;
-    int slot = 0;
     for (int b = wave; b < blocks; b += W) {
         if constexpr (!ANY) {
-            if (b + (DEPTH - 1) * W < blocks) {
-                wait_for_loads<(DEPTH - 1) * LOADS>();
-            } else {
-                wait_for_loads<0>();
-            }
+            wait_for_loads<0>();
         }
         const float ws = w_scale;
         if (b + W < blocks) {
             w_scale = w_scales[b + W];
         }
-        const uint4 *stage = mine + slot * SLOTS;
-        const float *scales = reinterpret_cast<const float *>(stage + (MB + NB) * 128);
+        const float *scales = reinterpret_cast<const float *>(mine + (MB + NB) * 128);
         auto operand_of = [&](int block16) {
-            const uint4 *row = stage + (16 * block16 + r) * 8;
+            const uint4 *row = mine + (16 * block16 + r) * 8;
             return fp8_operand(row[q ^ (r & 7)], row[(4 + q) ^ (r & 7)]);
         };
         i32x8 w8[NB], a8[MB];
@@ -440,11 +430,10 @@ __global__ __launch_bounds__(64 * W) void fp8_split_kernel(const LinearParams p)
             a8[j] = operand_of(j);
             scale[j] = scales[16 * j + r] * ws;
         }
-        if (b + DEPTH * W < blocks) {
+        if (b + W < blocks) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the operands are out of the LDS
-            ask(b + DEPTH * W, slot);
+            ask(b + W);
         }
-        slot = slot + 1 < DEPTH ? slot + 1 : 0;
         typename std::conditional<WIDE, WideOperand, i32x8>::type w[NB], a;
         auto take = [&](auto &to, i32x8 v) {
             if constexpr (WIDE) {
@@ -500,13 +489,13 @@ __global__ __launch_bounds__(64 * W) void fp8_split_kernel(const LinearParams p)
     }
 }
 
-template <typename T, int MB, int NB, int W, int DEPTH, bool ANY>
+template <typename T, int MB, int NB, int W, bool ANY>
 int launch_split(LinearParams p, hipStream_t stream)
 {
-    static_assert(64 * MB * NB <= DEPTH * ((MB + NB) * 128 + 16), "the sums lie where the operands were");
-    constexpr size_t bytes = (size_t)W * DEPTH * ((MB + NB) * 128 + 16) * 16;
+    static_assert(64 * MB * NB <= (MB + NB) * 128 + 16, "the sums lie where the operands were");
+    constexpr size_t bytes = (size_t)W * ((MB + NB) * 128 + 16) * 16;
     static size_t configured[KUTACC_DEVICE_SLOTS] = {};
-    const auto kernel = &fp8_split_kernel<T, MB, NB, W, DEPTH, ANY>;
+    const auto kernel = &fp8_split_kernel<T, MB, NB, W, ANY>;
     const int64_t groups = tiles_of(p, 16 * MB, 16 * NB);
     if (!kutacc_grid_fits(groups, 64 * W)) {
         return KUTACC_HIP_EUNSUPPORTED;
@@ -776,7 +765,7 @@ template <typename T>
 int launch_pieces(const LinearParams &p, hipStream_t stream)
 {
     if (p.M <= 16) {
-        return 2 * tiles_of(p, 16, 64) >= kutacc_cu_count() ? launch_split<T, 1, 4, 8, 1, false>(p, stream) : launch_split<T, 1, 1, 16, 1, false>(p, stream);
+        return 2 * tiles_of(p, 16, 64) >= kutacc_cu_count() ? launch_split<T, 1, 4, 8, false>(p, stream) : launch_split<T, 1, 1, 16, false>(p, stream);
     }
     if constexpr (std::is_same<T, bf16_t>::value) { // in fp32 a wave of these has no registers for its widened operands
         if (takes_large_tiles(p, true)) {
@@ -786,7 +775,7 @@ int launch_pieces(const LinearParams &p, hipStream_t stream)
     if (takes_tiles(p, false)) {
         return launch_tiles<T, 4, 2, 2, false>(p, stream);
     }
-    return enough(p, 64, 64) ? launch_split<T, 4, 4, 8, 1, false>(p, stream) : enough(p, 32, 64) ? launch_split<T, 2, 4, 8, 1, false>(p, stream) : launch_split<T, 2, 2, 16, 1, false>(p, stream);
+    return enough(p, 64, 64) ? launch_split<T, 4, 4, 8, false>(p, stream) : enough(p, 32, 64) ? launch_split<T, 2, 4, 8, false>(p, stream) : launch_split<T, 2, 2, 16, false>(p, stream);
 }
 
 // Rows on any address, of 16 bytes and more: what passes through registers leaves less of them, so 64 x 64 is not among these, nor with fp32 results 32 x 32;
@@ -798,17 +787,17 @@ template <typename T>
 int launch_bytes(const LinearParams &p, hipStream_t stream)
 {
     if (p.M <= 16) {
-        return 2 * tiles_of(p, 16, 64) >= kutacc_cu_count() ? launch_split<T, 1, 4, 8, 1, true>(p, stream) : launch_split<T, 1, 1, 16, 1, true>(p, stream);
+        return 2 * tiles_of(p, 16, 64) >= kutacc_cu_count() ? launch_split<T, 1, 4, 8, true>(p, stream) : launch_split<T, 1, 1, 16, true>(p, stream);
     }
     if (takes_any_tiles(p)) {
         return launch_tiles<T, 4, 2, 2, true>(p, stream);
     }
     if constexpr (std::is_same<T, bf16_t>::value) {
         if (!enough(p, 32, 64)) {
-            return launch_split<T, 2, 2, 16, 1, true>(p, stream);
+            return launch_split<T, 2, 2, 16, true>(p, stream);
         }
     }
-    return launch_split<T, 2, 4, 8, 1, true>(p, stream);
+    return launch_split<T, 2, 4, 8, true>(p, stream);
 }
 } // namespace
 
