@@ -21,7 +21,11 @@ __device__ __forceinline__ float activation_exponent(float v, int activation)
 __device__ __forceinline__ float activation_of_sigmoid(float v, float s, int activation, float &derivative)
 {
     const float a = v * s, rest = 1.f - s;
-    derivative = activation == KUTACC_HIP_GELU ? fmaf(a * rest, fmaf(3.f * GELU_CUBE * GELU_SLOPE, fminf(v * v, 1e4f), GELU_SLOPE), s) : fmaf(a, rest, s);
+    if (__builtin_constant_p(activation) && activation != KUTACC_HIP_GELU) {
+        derivative = fmaf(a, rest, s);
+    } else { // (with one expression for both, where the kernel is told which)
+        derivative = fmaf(a * rest, activation == KUTACC_HIP_GELU ? fmaf(3.f * GELU_CUBE * GELU_SLOPE, fminf(v * v, 1e4f), GELU_SLOPE) : 1.f, s);
+    }
     return a;
 }
 
