@@ -122,3 +122,19 @@ def test_gated_transition_of_more_rows_than_small_tiles_have_threads():
     oracle.close(out[picked.cuda()], want, oracle.stored(want, off, BF16), "out")
     out[picked.cuda()] = 0
     assert not bool(out.any())
+
+
+@pytest.mark.parametrize("size", [64, 300, 4100])
+def test_rms_norm_of_rows_whose_squares_pass_32_bits(size):
+    """As the header has it: zeros, and of the backward pass what came by other ways; the rows beside them as always."""
+    x, dy, ds = cpu_randn(1, 5, size), cpu_randn(2, 5, size), cpu_randn(3, 5, size)
+    x[2] = (x[2].float() * 2.0 ** 70).to(BF16)
+    out, dx = Room(5, size, BF16), Room(5, size, BF16)
+    ok(capi.RmsNorm(x.cuda(), None, EPS, out=out.view))
+    ok(capi.RmsNormBackward(x.cuda(), None, dy.cuda(), EPS, grad_sum=ds.cuda(), grad_x=dx.view))
+    assert not bool(out.view[2].any()) and torch.equal(dx.view[2].cpu(), ds[2])
+    others = [0, 1, 3, 4]
+    _, y = oracle.rms_norm(x[others], None, EPS)
+    oracle.close(out.view[others], y, oracle.stored(y, y.abs() * oracle.norm_slack(size), BF16), "out")
+    want, off, _, _ = oracle.rms_norm_backward(x[others], None, dy[others], EPS, ds[others])
+    oracle.close(dx.view[others], want, oracle.stored(want, off, BF16), "grad_x")
