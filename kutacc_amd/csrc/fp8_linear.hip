@@ -513,7 +513,7 @@ int launch_split(LinearParams p, hipStream_t stream)
 // Operands come straight into the LDS (a wave's 64 lanes bring eight rows of 128 bytes a load), a block of 128 k a stage, two stages: a block
 // is asked for when the one before the last has been read by all.  The sums of a block are added to a wave's 128 by vector
 // instructions, which cannot reach the accumulation registers: more than 128 a wave would not fit beside its operands.
-// Two waves a SIMD: one multiplies while the other scales.  8192 x 4096 x 8192: 254 us, 2160 TFLOP/s (a large library product: 2690): the matrix pipe works in
+// Two waves a SIMD: one multiplies while the other scales.  8192 x 4096 x 8192: 262 us, 2100 TFLOP/s (a large library product: 2690): the matrix pipe works in
 // 47 % of the clocks, the vector issue port in 35 %, four multiply-adds a product.
 constexpr int SPAN = 8; // blocks whose scales are brought at a time
 constexpr size_t tiles_lds(int side) { return 2 * 2 * side * 128 + 2 * SPAN * side * 4 + 2 * 64 * 4; }

@@ -3,12 +3,12 @@
 // A workgroup of eight waves owns 32 hidden units.  First g, u and dh of all rows: the waves share the channels, operands straight into registers but the
 // columns of Wd, which leave the LDS by its transposing reads; their sums meet in the LDS, in one order.  What the activation and its derivative make of them is
 // rounded to bf16 once and stays in the LDS: h, dg and du of 32 units, and what that rounding left, for results that have few values or are sums of few rows,
-// and so little to average over: 16 bits of them, almost for nothing here (us, with rests and without: 25 x 128 x 512 10.2 and 9.9).  Then the waves go through
+// and so little to average over: 16 bits of them, for little here (us, with rests and without: 25 x 128 x 512 10.3 and 9.8, 16 x 512 x 2048 20.6 and 19.7).  Then the waves go through
 // the channels in blocks of 32, each with its own: the units' rows of the three weights' gradients are whole, as the rows are few enough to be contracted at once,
 // and the gradient of x is a share of 32 units, in fp32.
-// What bounds it are those trips and the code itself, which is run once: 6 us at 25 x 128 -> 512, of which the operands of the first products take 1.5, the sums and
+// What bounds it are those trips and the code itself, which is run once: some 6 us at 25 x 128 -> 512, of which the operands of the first products take 1.5, the sums and
 // the activation 1.5 (2.7 as straight-line code), the blocks of channels 2.5.  us for the whole pass, this and the kernels for any number of rows: 25 x 128 x 512
-// 9.9 and 26, 3 x 256 x 1024 11 and 28, 50 x 256 x 896 17 and 30, 16 x 512 x 2048 19 and 35, 64 x 512 x 2048 29 and 35, 64 x 1024 x 4096 (34 MB of shares) 53 and 52.
+// 10.3 and 26, 3 x 256 x 1024 11.6 and 28, 50 x 256 x 896 16.9 and 30, 16 x 512 x 2048 20.6 and 35, 64 x 512 x 2048 28 and 35, 64 x 1024 x 4096 (34 MB of shares) 53 and 51.
 //
 // All blocks in the LDS are rows of 64 bytes, their four 16-byte slots XOR-ed with bits 2 and 3 of the row's number: 16 rows are 1 KB, which one load of 64 lanes
 // brings.  Of such 16 rows a transposing read gives the fragment with k along the rows, column (lane & 31).

@@ -6,8 +6,9 @@
 // of a slice in the LDS is hidden unit sigma(i) (bits 2 and 3 of i swapped), which makes the eight values a lane holds per k-step consecutive hidden units.
 // The slices come straight into the LDS, into a ring with one barrier a slice.
 //
-// 147456 x 128 -> 512: 64 us, 910 TFLOP/s of the 1380 that a large product reaches here (142 us with the hidden layer in memory).  The matrix pipe works in 37 %
-// of the clocks, the vector issue port in 42 %, both in 18 %: the activation is as much work as the products, and the clock falls under the two together.
+// 147456 x 128 -> 512: 65.7 us, 880 TFLOP/s of the 1380 that a large product reaches here (142 us with the hidden layer in memory).  The matrix pipe works in 37 %
+// of the clocks, the vector issue port in 42 %, both in 19 %, and neither in 40 %: a SIMD has two waves, which wait for 28 % of their time, at a slice's barrier among
+// others.  The activation is as much work as the products, and the clock falls under the two together.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

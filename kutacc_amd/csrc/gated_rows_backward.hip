@@ -1,6 +1,6 @@
 // The backward pass of the gated transition of 64 and 128 channels: the hidden layer stays on chip, formed once for the gradient of x and once more for those
 // of the weights.  With so few channels that costs less than its way through memory: at 65536 rows, 128 -> 512, 94 GFLOP in place of 69, but h, dg and du are
-// 200 MB to write and to read again (us for the whole pass: 110; a kernel that stored them beside the gradient of x, and products of tiles: 88 + 60; products of
+// 200 MB to write and to read again (us for the whole pass: 112; a kernel that stored them beside the gradient of x, and products of tiles: 88 + 60; products of
 // tiles alone: 174).
 //
 // The gradient of x: a wave owns 32 rows of x and of the gradient of out as operand fragments in registers, and walks the hidden layer in slices of 32 units
@@ -199,7 +199,7 @@ __global__ __launch_bounds__(64 * WAVES, GROUPS * WAVES / 4) void gated_input_gr
 // way round (MFMA columns = hidden units): rounded to bf16, h, dg and du are operands of products that contract over the rows, whose other operands leave the
 // LDS by the transposing reads.  Nothing of the hidden layer goes to memory.  The sums of 32 units, three times 32 x 128, are 192 registers and the weights 96:
 // one wave a SIMD, whose products run beside its own activation.  The rows are split over as many workgroups as there are CUs, each with a share of the sums:
-// 65536 rows, 128 -> 512: 60 us and 9 for adding the shares (50 MB).  Without activation and LDS reads it would take 48: the products
+// 65536 rows, 128 -> 512: 59 us and 8 for adding the shares (50 MB).  Without activation and LDS reads it would take 48: the products
 // themselves, at the rate that they reach here, bound it.
 template <int CO, int ACTIVATION>
 __global__ __launch_bounds__(256, 1) void gated_weight_gradients_kernel(const BackwardParams p)

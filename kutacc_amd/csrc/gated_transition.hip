@@ -287,8 +287,8 @@ __global__ __launch_bounds__(256, MODE == GATED || MODE == HIDDEN_GRADIENTS ? 1 
 // A tile of GATED is SIDE rows of x by SIDE / 2 hidden units: of every 64 columns 32 are of the gate and 32 of the other projection, so that a wave
 // holds both of the same hidden units.  HIDDEN_GRADIENTS then multiplies dy with SIDE / 2 columns of down_w into sums of their own.
 //
-// 4001 x 1024 -> 2816: GATED 54 us (860 TFLOP/s), PLAIN 31 (750); 4096 x 1024 -> 4096: hidden gradients 148 (695), gradient of x 77 (900), of the weights 97
-// (1060); a large library product reaches 1380.  The matrix pipe works in 30 to 44 % of the clocks: the two waves of a SIMD run in step, so that neither hides the
+// 4001 x 1024 -> 2816, 81 us: GATED 52 (890 TFLOP/s), PLAIN 29 (800); 4096 x 1024 -> 4096, backward, 322: hidden gradients 146 (710), gradient of x 77 (890), of the
+// weights 99 (1040); a large library product reaches 1380.  (A call's time, and its kernels' shares of that in a trace.)  The matrix pipe works in 30 to 44 % of the clocks: the two waves of a SIMD run in step, so that neither hides the
 // other's barriers, nor a tile's activation and results another tile's products.
 template <int MODE, int MI, int WM, int WN, int GROUPS>
 __global__ __launch_bounds__(64 * WM * WN * GROUPS, 2) void ff_pieces_kernel(const TilesParams p)
@@ -662,10 +662,10 @@ __global__ __launch_bounds__(256) void ff_shares_kernel(const TilesParams p)
 //
 // 16 MB rows by 16 NB columns a workgroup, all of them in every wave (and with GATED of both projections): wave w takes blocks w, w + W, ... and brings
 // them straight into its own part of the LDS, eight rows of 128 bytes a load, DEPTH blocks ahead and without barriers.  The waves' sums meet in the LDS at
-// the end, in one order.  Memory bounds it: 3 x 2048 -> 8192 GATED 12.9 us, 5.2 TB/s, PLAIN 9.6, 3.5.
+// the end, in one order.  Memory bounds it: 3 x 2048 -> 8192, 24.7 us: GATED 14.9, 4.5 TB/s, PLAIN 9.8, 3.4.
 //
 // With WITH_REST half of the MB blocks of rows are what the rounding of the others left, product 1's: few enough results are bound by launches, and keep the
-// hidden layer to 16 bits almost for nothing (3 x 128 -> 512 7.3 us and 7.1): a result's error is then that of its own rounding, 1.65e-3 in place of 2.35e-3.
+// hidden layer to 16 bits almost for nothing (3 x 128 -> 512 7.2 us and 7.1): a result's error is then that of its own rounding, 1.65e-3 in place of 2.35e-3.
 template <int MODE, int MB, int NB, int W, int DEPTH, bool WITH_REST = false>
 __global__ __launch_bounds__(64 * W) void ff_split_kernel(const TilesParams p)
 {

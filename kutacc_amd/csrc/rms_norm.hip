@@ -9,7 +9,7 @@
 // All sums are fp32, and y is formed from s before its rounding to storage.  Memory bounds them: a row is read once, held in
 // registers (8 values a lane and chunk) over its reduction, and written once.  TPR threads share a row, each with NV chunks, chunk
 // TPR i + thread: whole lines a load, and the 16 lanes whose chunks make up a block of 128 are neighbours, so that a scale costs four DPP
-// steps.  8191 x 4096 with a residual and an 8-bit result: 46 us, 5.1 TB/s; backward 147456 x 128: 34.5 us, 4.4 TB/s.
+// steps.  8191 x 4096 with a residual and an 8-bit result: 46.5 us, 5.1 TB/s; backward 147456 x 128: 34.6 us, 4.4 TB/s.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
