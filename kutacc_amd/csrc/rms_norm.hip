@@ -352,7 +352,8 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(const float *partial,
 }
 
 // Blocks of BLOCK_ROWS x 128 values with a scale each: 16 lanes a row of a block, and 256 threads a block of 128 rows (8 rows each)
-// or 16 blocks of one row.
+// or 16 blocks of one row.  Memory bounds blocks of 128 rows, 8192 x 8192 of bf16 42.8 us, 4.7 TB/s, of fp32 59.5 us, 5.6 TB/s; with one row a thread has a
+// single load on its way, and two divisions of 64 bits in front of it: 65.7 us, 3.1 TB/s, and 67.1 us, 5.0 TB/s.
 struct QuantizeParams {
     const void *x;
     uint8_t *out;
