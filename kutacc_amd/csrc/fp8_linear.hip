@@ -7,7 +7,7 @@
 // The matrix instructions for 8-bit operands add up to 16 neighbouring products at a time in about 14 bits below the largest of them (measured: a
 // product of 2^-14 beside one of 1 is lost, beyond those 16 one of 2^-23 is kept).  2-norm relative 1.5e-5 for normally distributed operands: a
 // hundredth of the rounding of a bf16 result, but not fp32.  Results in fp32 take their operands as bf16, which hold every e4m3 value
-// exactly, at half the rate: 4e-9 so.
+// exactly, at half the rate (8192 x 4096 x 8192 522 us, 1050 TFLOP/s): 4e-9 so.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
