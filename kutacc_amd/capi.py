@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import sys
 
 import numpy as np
 
@@ -651,7 +652,10 @@ def _dense(t, shape, dtype, what):
 
 
 class _DeviceCall:
-    """A call on tensors of one device, which has to be the current one where the call is made: there the library launches."""
+    """A call on tensors of one device, which has to be the current one where the call is made: there the library launches.  A workspace that it owns goes back to
+    PyTorch's allocator with it, which is told of the streams that the call may still run on: what it gives the memory to next waits for them."""
+
+    workspace = None
 
     def _on(self, *tensors):
         import torch
@@ -661,12 +665,28 @@ class _DeviceCall:
         (device,) = devices
         # with one GPU in sight its tensors are on the current device
         self.checked_device = None if device.type == "cuda" and torch.cuda.device_count() == 1 else device
+        self.streams = set()
 
-    def _check_device(self):
+    def _enter(self, stream_ptr):
         if self.checked_device is not None:
             import torch
             if self.checked_device.type != "cuda" or self.checked_device.index != torch.cuda.current_device():
                 raise ValueError(f"operands on {self.checked_device}, which is not the current GPU")
+        self.streams.add(stream_ptr)
+
+    def __del__(self):
+        if self.workspace is None or not self.workspace.is_cuda or sys.is_finalizing():
+            return
+        import torch
+        capturing = torch.cuda.is_current_stream_capturing()  # then streams are not to be asked
+        for ptr in self.streams:
+            ptr = lib().kutacc_hip_get_stream() if ptr is None else getattr(ptr, "value", ptr)
+            stream = torch.cuda.ExternalStream(ptr or 0, self.workspace.device)
+            try:
+                if capturing or not stream.query():
+                    self.workspace.record_stream(stream)
+            except RuntimeError:  # a stream that is no more has finished its work
+                pass
 
 
 def _workspace(nbytes, device):
@@ -698,7 +718,7 @@ class RmsNorm(_DeviceCall):
         self.args = a
 
     def run(self, stream_ptr=None) -> int:
-        self._check_device()
+        self._enter(stream_ptr)
         return lib().kutacc_hip_rms_norm(ctypes.byref(self.args), stream_ptr)
 
 
@@ -724,7 +744,7 @@ class RmsNormBackward(_DeviceCall):
         self.args = a
 
     def run(self, stream_ptr=None) -> int:
-        self._check_device()
+        self._enter(stream_ptr)
         return lib().kutacc_hip_rms_norm_backward(ctypes.byref(self.args), stream_ptr)
 
 
@@ -741,7 +761,7 @@ class QuantizeFp8(_DeviceCall):
                      *_rows(scales, (-(-rows // block_rows), -(-size // 128)), torch.float32, "scales"), rows, size, block_rows, _torch_dtype_code(x))
 
     def run(self, stream_ptr=None) -> int:
-        self._check_device()
+        self._enter(stream_ptr)
         return lib().kutacc_hip_quantize_fp8(*self.args, stream_ptr)
 
 
@@ -765,7 +785,7 @@ class LinearFp8(_DeviceCall):
         self.args = g
 
     def run(self, stream_ptr=None) -> int:
-        self._check_device()
+        self._enter(stream_ptr)
         return lib().kutacc_hip_linear_fp8(ctypes.byref(self.args), stream_ptr)
 
 
@@ -789,7 +809,7 @@ class GatedTransition(_DeviceCall):
         self.args = a
 
     def run(self, stream_ptr=None) -> int:
-        self._check_device()
+        self._enter(stream_ptr)
         return lib().kutacc_hip_gated_transition(ctypes.byref(self.args), stream_ptr)
 
 
@@ -816,5 +836,5 @@ class GatedTransitionBackward(_DeviceCall):
         self.args = a
 
     def run(self, stream_ptr=None) -> int:
-        self._check_device()
+        self._enter(stream_ptr)
         return lib().kutacc_hip_gated_transition_backward(ctypes.byref(self.args), stream_ptr)

@@ -80,3 +80,48 @@ def test_owners_run_on_their_own_device_alone(monkeypatch):
             call.run()
         call.checked_device = torch.device("cuda", 1)
         assert call.run() == 0
+
+
+@pytest.mark.parametrize("capturing", [False, True])
+@pytest.mark.parametrize("streams", [[], [0x7000], [0x7000, 0x8000, 0x7000], [None]])
+def test_a_workspace_that_goes_waits_for_its_streams(monkeypatch, streams, capturing):
+    """PyTorch's allocator is told of each stream on which the call may still run, once; None is the library's own.  Streams that have finished, or are no more, it need not
+    know, and none is asked during a capture."""
+    told = []
+    states = {0x7000: "works", 0x8000: "has finished", 0x9000: "is no more"}
+
+    class Workspace:
+        device, is_cuda = "the device", True
+
+        def record_stream(self, stream):
+            told.append(stream.ptr)
+
+    class Stream:
+        def __init__(self, ptr, device):
+            assert device == "the device"
+            self.ptr = ptr
+
+        def query(self):
+            assert not capturing
+            if states[self.ptr] == "is no more":
+                raise RuntimeError
+            return states[self.ptr] == "has finished"
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *args: 0x9000 if name == "kutacc_hip_get_stream" else 0
+
+    calls = [c for c in owners() if c.workspace is not None]
+    assert len(calls) == 3
+    monkeypatch.setattr(capi, "lib", Library)
+    monkeypatch.setattr(torch.cuda, "ExternalStream", Stream)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+    while calls:
+        call = calls.pop()
+        call.workspace, call.checked_device = Workspace(), None
+        for s in streams:
+            assert call.run(s) == 0
+        del call
+        on = {s or 0x9000 for s in streams}
+        assert sorted(told) == sorted(p for p in on if capturing or states[p] == "works")
+        told.clear()

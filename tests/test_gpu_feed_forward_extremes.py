@@ -138,3 +138,26 @@ def test_rms_norm_of_rows_whose_squares_pass_32_bits(size):
     oracle.close(out.view[others], y, oracle.stored(y, y.abs() * oracle.norm_slack(size), BF16), "out")
     want, off, _, _ = oracle.rms_norm_backward(x[others], None, dy[others], EPS, ds[others])
     oracle.close(dx.view[others], want, oracle.stored(want, off, BF16), "grad_x")
+
+
+def test_an_owner_may_go_while_its_call_runs():
+    """Its workspace's memory is asked for at once and written on another stream, while the call has not begun."""
+    rows, c_o, c_i = 300, 256, 512
+    w, x = [t.cuda() for t in weights_of(1, c_o, c_i)], cpu_randn(1, rows, c_o).cuda()
+    want, out = torch.empty_like(x), torch.empty_like(x)
+    call = capi.GatedTransition(x, *w, want)
+    ok(call)
+    size = call.workspace.numel()
+    del call
+    side = torch.cuda.Stream()
+    for _ in range(5):
+        out.fill_(1)
+        torch.cuda.synchronize()
+        call = capi.GatedTransition(x, *w, out)
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)  # some ten milliseconds, by the clock
+        assert call.run(side.cuda_stream) == 0
+        del call
+        others = [torch.full((size,), 255, device="cuda", dtype=torch.uint8) for _ in range(3)]
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and all(bool((o == 255).all()) for o in others)
