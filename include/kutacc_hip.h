@@ -33,6 +33,7 @@ extern "C" {
 
 #define KUTACC_DTYPE_BF16 1
 #define KUTACC_DTYPE_FP32 2
+#define KUTACC_DTYPE_E4M3 3 /* of a cache of keys and values alone; OCP e4m3 */
 
 /* Kernel family selection for kutacc_hip_gating_attention. */
 #define KUTACC_HIP_PATH_AUTO 0    /* fused MFMA kernels when the shape allows, else tiled, else generic */
@@ -590,6 +591,155 @@ typedef struct kutacc_hip_gated_transition_backward_args {
 
 kutacc_export int64_t kutacc_hip_gated_transition_backward_workspace(int64_t rows, int64_t c_o, int64_t c_i);
 kutacc_export int kutacc_hip_gated_transition_backward(const kutacc_hip_gated_transition_backward_args_t *args, void *stream);
+
+/* ---- the attention half of a transformer block (no counterpart in the reference) ---- */
+
+/* [tokens, heads, head_size] with contiguous channels: element (t, h, c) at data[t * token_stride + h * head_stride + c].  Strides of what is written keep
+ * its elements apart: the heads of a token within its stride, or the tokens of a head within the head's. */
+typedef struct kutacc_hip_heads {
+    void *data;
+    int64_t token_stride;
+    int64_t head_stride;
+} kutacc_hip_heads_t;
+
+/*
+ * Rotary positions.  The channels first .. first + rotated - 1 of a head are rotated / 2 pairs; pair j of a token at position t is turned by the angle
+ * t inv_freq[j]:
+ *   a' = magnitude (a cos - b sin),  b' = magnitude (b cos + a sin)      (inverse: by the negative angle)
+ * (a, b) are channels (first + j, first + rotated / 2 + j), or with `interleaved` (first + 2 j, first + 2 j + 1).  The angle is the exact product of the
+ * position and the fp32 frequency, reduced in 64 bits; its sine and cosine and the turn are fp32.  rotated == 0: nothing is turned.
+ */
+typedef struct kutacc_hip_rotation {
+    const float *inv_freq; /* [rotated / 2] */
+    int32_t rotated;       /* channels, even, up to 512 */
+    int32_t first;
+    int32_t interleaved;
+    int32_t inverse;
+    float magnitude;
+    int32_t reserved;
+} kutacc_hip_rotation_t;
+
+/*
+ * Frequencies for inv_freq, formed on the host in 64 bits (`inv_freq` is HOST memory here, [rotated / 2]): base^(-2 j / rotated), for contexts longer than the
+ * `original_length` that a model was trained with changed by `scaling`:
+ *   KUTACC_HIP_ROTARY_PLAIN       as they are
+ *   KUTACC_HIP_ROTARY_LINEAR      over `factor`
+ *   KUTACC_HIP_ROTARY_BASE        of the base times factor^(rotated / (rotated - 2)): the lowest frequency over `factor`, the highest as it is
+ *   KUTACC_HIP_ROTARY_BY_PAIRS    as they are for pairs that turn at least `fast` times over original_length, over `factor` for those that turn at most `slow` times,
+ *                                 and mixed linearly in the pair's number between (from the last whole pair at or before the one to the first whole one at or after the other)
+ *   KUTACC_HIP_ROTARY_BY_TURNS    the same, mixed linearly in the number of turns
+ * base > 1, factor >= 1; fast > slow > 0 and original_length > 0 where they are used.
+ */
+#define KUTACC_HIP_ROTARY_PLAIN 0
+#define KUTACC_HIP_ROTARY_LINEAR 1
+#define KUTACC_HIP_ROTARY_BASE 2
+#define KUTACC_HIP_ROTARY_BY_PAIRS 3
+#define KUTACC_HIP_ROTARY_BY_TURNS 4
+kutacc_export int kutacc_hip_rotary_frequencies(float *inv_freq, int32_t rotated, int32_t scaling, double base, double factor, double original_length, double fast,
+                                                double slow);
+
+/*
+ * Rotary positions of queries and keys (k.data NULL: of one of them alone).  Channels that are not rotated are copied; q_out may be q, and k_out k, with the same
+ * strides, and must not overlap an input otherwise.  The gradient of a rotation is the rotation of the gradient with `inverse` turned over.  Any head
+ * size, strides and addresses; bf16 or fp32 with fp32 arithmetic, rounded once.  tokens == 0 is a call that does nothing.
+ */
+typedef struct kutacc_hip_rotary_args {
+    int64_t tokens;
+    int64_t head_size;
+    int64_t q_heads;
+    int64_t k_heads;
+    int32_t dtype; /* KUTACC_DTYPE_BF16 or KUTACC_DTYPE_FP32 */
+    int32_t reserved;
+    const int32_t *positions; /* [tokens], of either sign; NULL: 0, 1, 2, .. */
+    kutacc_hip_rotation_t rotation;
+    kutacc_hip_heads_t q, q_out;
+    kutacc_hip_heads_t k, k_out;
+} kutacc_hip_rotary_args_t;
+
+kutacc_export int kutacc_hip_rotary(const kutacc_hip_rotary_args_t *args, void *stream);
+
+/*
+ * A cache of keys and values in pages: entry (page, slot, kv head, channel) at k[page * k_page_stride + slot * k_token_stride + head * k_head_stride + channel], so that
+ * pages may hold their heads inside or outside of their slots.  bf16, or e4m3 of which an entry stands for its value times the head's scale.  head_size: a
+ * multiple of 8 (e4m3: of 16) up to 256; k, v and all strides on multiples of 16 bytes (else KUTACC_HIP_EUNSUPPORTED).  pages * page_size below 2^30.
+ */
+typedef struct kutacc_hip_cache {
+    int64_t pages;
+    int64_t page_size;
+    int64_t kv_heads;
+    int64_t head_size;
+    int32_t dtype; /* KUTACC_DTYPE_BF16 or KUTACC_DTYPE_E4M3 */
+    int32_t reserved;
+    void *k;
+    int64_t k_page_stride, k_token_stride, k_head_stride;
+    void *v;
+    int64_t v_page_stride, v_token_stride, v_head_stride;
+    const float *k_scales, *v_scales; /* [kv_heads], positive, both with e4m3 and none with bf16 */
+} kutacc_hip_cache_t;
+
+/*
+ * What of a cache belongs to whom, all on the device, so that a captured call goes on with the values it finds: a prefix of prefix_length entries that all sequences share,
+ * entry p in slot p % page_size of page prefix_pages[p / page_size], and behind it each sequence's own lengths[s] entries, the new ones included, entry p
+ * of them in slot p % page_size of page page_table[s * page_table_ld + p / page_size].  Tokens query_starts[s] .. query_starts[s + 1] - 1 of a call are the last of
+ * sequence s: token i of its n has position prefix_length + lengths[s] - n + i.  Tokens in front of the first and behind the last sequence are padding: nothing of
+ * theirs is written.  A page number outside of the cache stands for entries that are not there (nothing is kept, none is seen); so does what lies past
+ * the page table's columns.  A negative length is one of zero.  query_starts never fall and lie within 0 .. tokens.
+ */
+typedef struct kutacc_hip_cache_batch {
+    int64_t sequences;
+    int64_t tokens;
+    const int32_t *query_starts; /* [sequences + 1] */
+    const int32_t *lengths;      /* [sequences] */
+    const int32_t *page_table;   /* [sequences, columns] */
+    int64_t page_table_ld;
+    int64_t columns;
+    const int32_t *prefix_pages; /* [ceil(prefix_length / page_size)], NULL with prefix_length 0 */
+    int64_t prefix_length;
+} kutacc_hip_cache_batch_t;
+
+/*
+ * Appends the keys, rotated, and values of the batch's tokens to the sequences' own entries, and rotates their queries on the way (q.data NULL: no queries; q_out may
+ * be q with the same strides).  `lengths` counts the new entries already; a token without a place (its position before the sequence's own entries, past the page table, or on
+ * a page outside of the cache) is not kept, its query rotated all the same.  bf16 inputs and q_out; keys and values are rounded once to the cache's type, to e4m3
+ * over their head's scale, what lies past +-448 as that.  No two tokens of a call may have the same place: which of them a place then holds, in whole pieces
+ * of either, is left open.  Positions are those of the batch, or `positions` [tokens] where that is not NULL (they turn, but do not place).
+ */
+typedef struct kutacc_hip_cache_append_args {
+    kutacc_hip_cache_t cache;
+    kutacc_hip_cache_batch_t batch;
+    kutacc_hip_rotation_t rotation;
+    const int32_t *positions;
+    int64_t q_heads;
+    kutacc_hip_heads_t q, q_out;
+    kutacc_hip_heads_t k, v;
+} kutacc_hip_cache_append_args_t;
+
+kutacc_export int kutacc_hip_cache_append(const kutacc_hip_cache_append_args_t *args, void *stream);
+
+/*
+ * Attention of a batch's tokens over the cache: query head h reads kv head h / (q_heads / kv_heads).  A token sees the whole prefix and of its sequence's own entries all
+ * (causal 0) or those up to its own position (causal 1):
+ *   out = sum_j softmax_j(scale q k_j) v_j,   lse = ln sum_j exp(scale q k_j)
+ * A token that sees nothing gets zeros, and -inf as lse.  Entries that a token does not see may hold anything, infinities and NaN included.  The prefix is
+ * read once for all sequences where they have few tokens each.  bf16 queries and results; products accumulate, and the softmax is held, in fp32, its weights are rounded to
+ * bf16 as an operand (tiles of up to 64 rows -- a sequence's tokens times the q_heads / kv_heads that share a head -- keep 16 bits of them).  Sums
+ * are taken in one order for given lengths and a GPU: the same bits every time.  Any strides and addresses of q and out.
+ * `workspace`: device memory, 256-byte aligned, of at least kutacc_hip_cached_attention_workspace(args) bytes, which reads the sizes alone: no pointer needs to be set.
+ */
+typedef struct kutacc_hip_cached_attention_args {
+    kutacc_hip_cache_t cache;
+    kutacc_hip_cache_batch_t batch;
+    int64_t q_heads;
+    float scale; /* > 0 */
+    int32_t causal;
+    kutacc_hip_heads_t q, out;
+    float *lse; /* [tokens, q_heads] or NULL */
+    void *workspace;
+    int64_t workspace_bytes;
+} kutacc_hip_cached_attention_args_t;
+
+kutacc_export int64_t kutacc_hip_cached_attention_workspace(const kutacc_hip_cached_attention_args_t *args);
+kutacc_export int kutacc_hip_cached_attention(const kutacc_hip_cached_attention_args_t *args, void *stream);
 
 /* ---- runtime control (no counterpart in the reference; the CPU library has no device) ---- */
 

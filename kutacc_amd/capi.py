@@ -18,7 +18,7 @@ LIB_PATH = os.path.join(_PKG, "lib", "libkutacc.so")
 
 KUTACC_OK = 0
 KUTACC_ERROR = -1
-K_INT64, K_BF16, K_FP32 = 0, 1, 2
+K_INT64, K_BF16, K_FP32, K_E4M3 = 0, 1, 2, 3
 PATH_AUTO, PATH_GENERIC, PATH_FUSED, PATH_TILED = 0, 1, 2, 3
 EINVAL, EUNSUPPORTED = -2, -3
 
@@ -86,6 +86,59 @@ class HipGemmArgs(ctypes.Structure):
         ("c", _vp), ("c_stride_m", _i64), ("c_stride_batch", _i64),
         ("bias", _vp), ("bias_axis", _i32), ("relu", _i32),
         ("a_gate", _vp), ("bias_gate", _vp), ("mask", _vp), ("mask_stride_batch", _i64),
+    ]
+
+
+class HipHeads(ctypes.Structure):
+    """kutacc_hip_heads_t"""
+    _fields_ = [("data", _vp), ("token_stride", _i64), ("head_stride", _i64)]
+
+
+class HipRotation(ctypes.Structure):
+    """kutacc_hip_rotation_t"""
+    _fields_ = [("inv_freq", _vp), ("rotated", _i32), ("first", _i32), ("interleaved", _i32), ("inverse", _i32), ("magnitude", ctypes.c_float),
+                ("reserved", _i32)]
+
+
+class HipRotaryArgs(ctypes.Structure):
+    """kutacc_hip_rotary_args_t"""
+    _fields_ = [
+        ("tokens", _i64), ("head_size", _i64), ("q_heads", _i64), ("k_heads", _i64), ("dtype", _i32), ("reserved", _i32),
+        ("positions", _vp), ("rotation", HipRotation), ("q", HipHeads), ("q_out", HipHeads), ("k", HipHeads), ("k_out", HipHeads),
+    ]
+
+
+class HipCache(ctypes.Structure):
+    """kutacc_hip_cache_t"""
+    _fields_ = [
+        ("pages", _i64), ("page_size", _i64), ("kv_heads", _i64), ("head_size", _i64), ("dtype", _i32), ("reserved", _i32),
+        ("k", _vp), ("k_page_stride", _i64), ("k_token_stride", _i64), ("k_head_stride", _i64),
+        ("v", _vp), ("v_page_stride", _i64), ("v_token_stride", _i64), ("v_head_stride", _i64),
+        ("k_scales", _vp), ("v_scales", _vp),
+    ]
+
+
+class HipCacheBatch(ctypes.Structure):
+    """kutacc_hip_cache_batch_t"""
+    _fields_ = [
+        ("sequences", _i64), ("tokens", _i64), ("query_starts", _vp), ("lengths", _vp), ("page_table", _vp), ("page_table_ld", _i64),
+        ("columns", _i64), ("prefix_pages", _vp), ("prefix_length", _i64),
+    ]
+
+
+class HipCacheAppendArgs(ctypes.Structure):
+    """kutacc_hip_cache_append_args_t"""
+    _fields_ = [
+        ("cache", HipCache), ("batch", HipCacheBatch), ("rotation", HipRotation), ("positions", _vp), ("q_heads", _i64),
+        ("q", HipHeads), ("q_out", HipHeads), ("k", HipHeads), ("v", HipHeads),
+    ]
+
+
+class HipCachedAttentionArgs(ctypes.Structure):
+    """kutacc_hip_cached_attention_args_t"""
+    _fields_ = [
+        ("cache", HipCache), ("batch", HipCacheBatch), ("q_heads", _i64), ("scale", ctypes.c_float), ("causal", _i32),
+        ("q", HipHeads), ("out", HipHeads), ("lse", _vp), ("workspace", _vp), ("workspace_bytes", _i64),
     ]
 
 
@@ -327,6 +380,13 @@ def lib() -> ctypes.CDLL:
         workspace, call = getattr(L, f"kutacc_hip_{name}_workspace"), getattr(L, f"kutacc_hip_{name}")
         workspace.argtypes, workspace.restype = [_i64, _i64, _i64], _i64
         call.argtypes, call.restype = [ctypes.POINTER(args), _vp], ctypes.c_int
+    L.kutacc_hip_rotary_frequencies.argtypes = [_vp, _i32, _i32, *[ctypes.c_double] * 5]
+    L.kutacc_hip_rotary_frequencies.restype = ctypes.c_int
+    for name, args in (("rotary", HipRotaryArgs), ("cache_append", HipCacheAppendArgs), ("cached_attention", HipCachedAttentionArgs)):
+        call = getattr(L, f"kutacc_hip_{name}")
+        call.argtypes, call.restype = [ctypes.POINTER(args), _vp], ctypes.c_int
+    L.kutacc_hip_cached_attention_workspace.argtypes = [ctypes.POINTER(HipCachedAttentionArgs)]
+    L.kutacc_hip_cached_attention_workspace.restype = _i64
     L.kutacc_hip_set_stream.argtypes = [_vp]
     L.kutacc_hip_get_stream.restype = _vp
     L.kutacc_hip_set_blocking.argtypes = [ctypes.c_int]
@@ -838,3 +898,181 @@ class GatedTransitionBackward(_DeviceCall):
     def run(self, stream_ptr=None) -> int:
         self._enter(stream_ptr)
         return lib().kutacc_hip_gated_transition_backward(ctypes.byref(self.args), stream_ptr)
+
+
+# ---- the attention half of a transformer block ----------------------------------------------------------------
+ROTARY_SCALINGS = {"plain": 0, "linear": 1, "base": 2, "by_pairs": 3, "by_turns": 4}  # KUTACC_HIP_ROTARY_*
+
+
+def rotary_frequencies(rotated, base=10000.0, scaling="plain", factor=1.0, original_length=0.0, fast=32.0, slow=1.0):
+    """kutacc_hip_rotary_frequencies: fp32 [rotated / 2] on the host."""
+    import torch
+    out = torch.empty(max(rotated // 2, 1), dtype=torch.float32)
+    rc = lib().kutacc_hip_rotary_frequencies(out.data_ptr(), rotated, ROTARY_SCALINGS[scaling], base, factor, original_length, fast, slow)
+    if rc != 0:
+        raise ValueError(f"the library returned {rc}")
+    return out
+
+
+def _heads(t, shape, dtype, what):
+    """kutacc_hip_heads_t of a [tokens, heads, head_size] tensor with contiguous channels; an empty one for None."""
+    if t is None:
+        return HipHeads(None, 0, 0)
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+        raise ValueError(f"{what}: {tuple(t.shape)} of {t.dtype}, wanted {tuple(shape)} of {dtype}")
+    if t.shape[2] > 1 and t.stride(2) != 1:
+        raise ValueError(f"{what}: its channels are not contiguous")
+    size = max(t.shape[2], 1)
+    # what there is one of has no stride of its own; torch's may be anything
+    return HipHeads(t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1] * size, t.stride(1) if t.shape[1] > 1 else size)
+
+
+def _rotation(inv_freq, interleaved, inverse, first, magnitude):
+    import torch
+    r = HipRotation()
+    if inv_freq is not None:
+        if inv_freq.dim() != 1:
+            raise ValueError(f"inv_freq: {inv_freq.dim()} axes, wanted one")
+        r.inv_freq, r.rotated = _dense(inv_freq, inv_freq.shape, torch.float32, "inv_freq"), 2 * inv_freq.shape[0]
+    r.first, r.interleaved, r.inverse, r.magnitude = first, int(interleaved), int(inverse), magnitude
+    return r
+
+
+class Rotary(_DeviceCall):
+    """One kutacc_hip_rotary call: q [tokens, heads, head_size] in bf16 or fp32, and k with heads of its own or None, into q_out and k_out (None: in place).  Channels
+    contiguous, any other strides.  inv_freq fp32 [rotated / 2]; positions int32 [tokens] or None: 0, 1, 2, ..; `inverse` for gradients."""
+
+    def __init__(self, q, inv_freq, positions=None, k=None, q_out=None, k_out=None, interleaved=False, first=0, magnitude=1.0, inverse=False):
+        import torch
+        self._on(q, inv_freq, positions, k, q_out, k_out)
+        if k is None and k_out is not None:
+            raise ValueError("k_out without k")
+        a = HipRotaryArgs()
+        a.tokens, a.q_heads, a.head_size = q.shape
+        if q.dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError(f"q: {q.dtype}, wanted bf16 or fp32")
+        a.dtype = _torch_dtype_code(q)
+        a.positions = _dense(positions, (a.tokens,), torch.int32, "positions")
+        a.rotation = _rotation(inv_freq, interleaved, inverse, first, magnitude)
+        q_out = q if q_out is None else q_out
+        a.q, a.q_out = _heads(q, q.shape, q.dtype, "q"), _heads(q_out, q.shape, q.dtype, "q_out")
+        if k is not None:
+            a.k_heads = k.shape[1]
+            shape = (a.tokens, a.k_heads, a.head_size)
+            k_out = k if k_out is None else k_out
+            a.k, a.k_out = _heads(k, shape, q.dtype, "k"), _heads(k_out, shape, q.dtype, "k_out")
+        self.keep = (q, inv_freq, positions, k, q_out, k_out)
+        self.args = a
+
+    def run(self, stream_ptr=None) -> int:
+        self._enter(stream_ptr)
+        return lib().kutacc_hip_rotary(ctypes.byref(self.args), stream_ptr)
+
+
+class Cache:
+    """kutacc_hip_cache_t over k and v [pages, page_size, kv_heads, head_size] (heads outside of the slots: a transposed view), bf16, or torch.float8_e4m3fn with fp32
+    scales [kv_heads]."""
+
+    def __init__(self, k, v, k_scales=None, v_scales=None):
+        import torch
+        c = HipCache()
+        c.pages, c.page_size, c.kv_heads, c.head_size = k.shape
+        if k.dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+            raise ValueError(f"k: {k.dtype}, wanted bf16 or e4m3")
+        if v.shape != k.shape or v.dtype != k.dtype:
+            raise ValueError(f"v: {tuple(v.shape)} of {v.dtype}, wanted {tuple(k.shape)} of {k.dtype}")
+        c.dtype = K_BF16 if k.dtype == torch.bfloat16 else K_E4M3
+        for t, what in ((k, "k"), (v, "v")):
+            if t.shape[3] > 1 and t.stride(3) != 1:
+                raise ValueError(f"{what}: its channels are not contiguous")
+            setattr(c, what, t.data_ptr())
+            dense = (t.shape[1] * t.shape[2] * t.shape[3], t.shape[2] * t.shape[3], t.shape[3])
+            for i, axis in enumerate(("page", "token", "head")):
+                setattr(c, f"{what}_{axis}_stride", t.stride(i) if t.shape[i] > 1 else dense[i])
+        c.k_scales, c.v_scales = (_dense(s, (c.kv_heads,), torch.float32, f"{w}_scales") for s, w in ((k_scales, "k"), (v_scales, "v")))
+        self.tensors = (k, v, k_scales, v_scales)
+        self.struct = c
+
+
+class CacheBatch:
+    """kutacc_hip_cache_batch_t, all int32 on the device: query_starts [sequences + 1], lengths [sequences], page_table [sequences, columns] with contiguous rows,
+    prefix_pages [at least ceil(prefix_length / page_size)].  Values may change between calls, and between replays of a captured one."""
+
+    def __init__(self, query_starts, lengths, page_table, prefix_pages=None, prefix_length=0):
+        import torch
+        b = HipCacheBatch()
+        if lengths.dim() != 1 or page_table.dim() != 2:
+            raise ValueError("lengths has one axis, page_table two")
+        b.sequences, b.columns = lengths.shape[0], page_table.shape[1]
+        b.query_starts = _dense(query_starts, (b.sequences + 1,), torch.int32, "query_starts")
+        b.lengths = _dense(lengths, (b.sequences,), torch.int32, "lengths")
+        b.page_table, b.page_table_ld = _rows(page_table, (b.sequences, b.columns), torch.int32, "page_table")
+        if prefix_length > 0:
+            if prefix_pages is None:
+                raise ValueError("a prefix without pages")
+            b.prefix_pages = _dense(prefix_pages, prefix_pages.shape, torch.int32, "prefix_pages")
+        b.prefix_length = prefix_length
+        self.tensors = (query_starts, lengths, page_table, prefix_pages)
+        self.struct = b
+
+    def of(self, cache, tokens):
+        """The structure for a call on `tokens` tokens of `cache`."""
+        b, c = self.struct, cache.struct
+        if b.prefix_length > 0 and self.tensors[3].numel() * c.page_size < b.prefix_length:
+            raise ValueError(f"{self.tensors[3].numel()} pages of {c.page_size} for a prefix of {b.prefix_length}")
+        own = HipCacheBatch()
+        ctypes.pointer(own)[0] = b
+        own.tokens = tokens
+        return own
+
+
+class CacheAppend(_DeviceCall):
+    """One kutacc_hip_cache_append call: k and v [tokens, kv_heads, head_size] in bf16 into the cache, k rotated by inv_freq fp32 [rotated / 2] (None: as it is), and q
+    [tokens, heads, head_size] rotated into q_out (None: in place) where there is one.  positions int32 [tokens], or None: the batch's."""
+
+    def __init__(self, cache, batch, k, v, inv_freq=None, q=None, q_out=None, positions=None, interleaved=False, first=0, magnitude=1.0):
+        import torch
+        self._on(*cache.tensors, *batch.tensors, k, v, inv_freq, q, q_out, positions)
+        if q is None and q_out is not None:
+            raise ValueError("q_out without q")
+        bf16 = torch.bfloat16
+        a = HipCacheAppendArgs()
+        tokens, c = k.shape[0], cache.struct
+        a.cache, a.batch = c, batch.of(cache, tokens)
+        a.rotation = _rotation(inv_freq, interleaved, False, first, magnitude)
+        a.positions = _dense(positions, (tokens,), torch.int32, "positions")
+        a.k, a.v = (_heads(t, (tokens, c.kv_heads, c.head_size), bf16, what) for t, what in ((k, "k"), (v, "v")))
+        if q is not None:
+            q_out = q if q_out is None else q_out
+            a.q_heads = q.shape[1]
+            a.q, a.q_out = (_heads(t, (tokens, a.q_heads, c.head_size), bf16, what) for t, what in ((q, "q"), (q_out, "q_out")))
+        self.keep = (cache, batch, k, v, inv_freq, q, q_out, positions)
+        self.args = a
+
+    def run(self, stream_ptr=None) -> int:
+        self._enter(stream_ptr)
+        return lib().kutacc_hip_cache_append(ctypes.byref(self.args), stream_ptr)
+
+
+class CachedAttention(_DeviceCall):
+    """One kutacc_hip_cached_attention call: q and out [tokens, heads, head_size] in bf16 over the cache, lse fp32 [tokens, heads] or None; scale None: 1 / sqrt(head_size).
+    Owns the workspace."""
+
+    def __init__(self, cache, batch, q, out, scale=None, causal=True, lse=None):
+        import torch
+        self._on(*cache.tensors, *batch.tensors, q, out, lse)
+        bf16 = torch.bfloat16
+        a = HipCachedAttentionArgs()
+        tokens, c = q.shape[0], cache.struct
+        a.cache, a.batch, a.q_heads = c, batch.of(cache, tokens), q.shape[1]
+        a.scale, a.causal = c.head_size ** -0.5 if scale is None else scale, int(causal)
+        a.q, a.out = (_heads(t, (tokens, a.q_heads, c.head_size), bf16, what) for t, what in ((q, "q"), (out, "out")))
+        a.lse = _dense(lse, (tokens, a.q_heads), torch.float32, "lse")
+        self.workspace = _workspace(lib().kutacc_hip_cached_attention_workspace(ctypes.byref(a)), q.device)
+        a.workspace, a.workspace_bytes = self.workspace.data_ptr(), self.workspace.numel()
+        self.keep = (cache, batch, q, out, lse)
+        self.args = a
+
+    def run(self, stream_ptr=None) -> int:
+        self._enter(stream_ptr)
+        return lib().kutacc_hip_cached_attention(ctypes.byref(self.args), stream_ptr)

@@ -249,4 +249,12 @@ int gated_transition(const kutacc_hip_gated_transition_args_t &args, hipStream_t
 int64_t gated_transition_backward_workspace(int64_t rows, int64_t c_o, int64_t c_i);
 int gated_transition_backward(const kutacc_hip_gated_transition_backward_args_t &args, hipStream_t stream);
 
+// rotary.hip: arguments as checked by api_cached_attention.cpp, here and below
+int rotary(const kutacc_hip_rotary_args_t &args, hipStream_t stream);
+int cache_append(const kutacc_hip_cache_append_args_t &args, hipStream_t stream);
+
+// cached_attention.hip
+int64_t cached_attention_workspace(const kutacc_hip_cached_attention_args_t &args); // from the sizes alone
+int cached_attention(const kutacc_hip_cached_attention_args_t &args, hipStream_t stream);
+
 } // namespace kutacc_launch
