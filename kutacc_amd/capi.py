@@ -268,6 +268,8 @@ DECLARED_SYMBOLS = [
     "kutacc_hip_gating_attention_static", "kutacc_hip_release_staging", "kutacc_hip_rms_norm", "kutacc_hip_rms_norm_backward_workspace",
     "kutacc_hip_rms_norm_backward", "kutacc_hip_quantize_fp8", "kutacc_hip_linear_fp8", "kutacc_hip_gated_transition_workspace",
     "kutacc_hip_gated_transition", "kutacc_hip_gated_transition_backward_workspace", "kutacc_hip_gated_transition_backward",
+    "kutacc_hip_rotary_frequencies", "kutacc_hip_rotary", "kutacc_hip_cache_append", "kutacc_hip_cached_attention_workspace",
+    "kutacc_hip_cached_attention",
 ]
 
 _lib = None

@@ -180,10 +180,10 @@ class Batch:
         return self.cache, self.batch
 
     def coarse(self, group):
-        """Of the weights: what their rounding is relative to the weight.  16 bits of them are kept in tiles of up to 64 rows."""
+        """Of the weights: what their rounding is relative to the weight.  16 bits of them are kept in tiles of up to 16 rows."""
         average = -(-self.tokens * group // min(len(self.sequences), self.tokens))
         whole_batch = self.prefix > 0 and len(self.sequences) > 1 and average <= 64
-        return 2.0 ** -16 if average <= 64 and (not whole_batch or self.tokens * group <= 64) else 2.0 ** -8
+        return 2.0 ** -16 if average <= 16 and (not whole_batch or self.tokens * group <= 16) else 2.0 ** -8
 
     def attention(self, q, scale, causal):
         """Results, lse, and bounds, rows of padding as NaN."""
@@ -255,6 +255,10 @@ SHAPES = [  # (queries, length) of each sequence, prefix, page, heads, kv_heads,
     ([(70, 90), (3, 3)], 40, 16, 6, 2, 256),
     ([(9, 5), (3, 0), (2, 1)], 0, 16, 2, 1, 128),
     ([(9, 5), (3, 0), (2, 1), (300, 100)], 33, 16, 2, 1, 64),
+    ([(1, 1 + 7 * i % 90) for i in range(300)], 40, 16, 64, 8, 16),
+    ([(1, 1 + 7 * i % 90) for i in range(300)], 0, 16, 64, 8, 16),
+    ([(12, 20 + i) for i in range(100)], 70, 16, 10, 2, 32),
+    ([(1, 7 * i % 300) for i in range(70)], 0, 16, 4, 2, 128),
 ]
 
 
