@@ -1,6 +1,9 @@
 // Attention over a cache of keys and values in pages, behind a prefix that the sequences share.
 //
-//   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q k_j - m),  m = max_j scale q k_j
+//   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q k_j - m),  m close to max_j scale q k_j
+//
+// m is the largest logit of the first keys, and follows the larger ones of later keys only when they leave it behind by more than 8 powers of two: nothing comes
+// near the ends of fp32 before, and the results are multiplied with exp(m - m') for few tiles instead of most.
 //
 // A row is one token's query head; the rows of a tile share a kv head: the tokens of one sequence times the heads of its group, or, over the shared prefix, all of the
 // batch's.  A pass over the keys holds m, the sum and a wave's results in registers, by the transposed products of the matrix instructions: K Q^T leaves a row's
@@ -21,6 +24,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "attention_util.h"
 #include "launch_internal.h"
 #include "mfma_tiles.h"
 #include "paged_cache.h"
@@ -59,6 +63,14 @@ struct AttentionParams {
     float2 *prefix_sums, *sums;                                // [kv head][tile + share][row]: m log2(e), sum
     int4 *rows;                                                // [token][head]: first piece, pieces (0: done), row of the tile
 };
+
+// The parameters once more, for what is done once a piece: those that are read through here are read when they are needed, and take no scalar registers in the loops
+__device__ __forceinline__ const AttentionParams &again()
+{
+    auto p = (const __attribute__((address_space(4))) AttentionParams *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const AttentionParams *)p;
+}
 
 __device__ const uint4 NOTHING[32] = {}; // what is read for entries that are not there: the longest one's bytes
 
@@ -101,6 +113,7 @@ struct FewRows {
     static constexpr int PITCH = 2 * D, CHUNKS = D / 8; // bytes and 16-byte pieces of an entry in the LDS
     static constexpr int TILE = KT * PITCH;
     static constexpr int LOADS = TILE / (FP8 ? 2048 : 1024);  // of values
+    static constexpr int AHEAD = 1;
     static constexpr int JOIN = WAVES * ROWS * ((D + 4) * 4 + 8);
     static constexpr int LDS = WAVES * TILE > JOIN ? WAVES * TILE : JOIN;
     // the two pieces that a transposing read takes of each of 8 entries stand in different banks
@@ -434,6 +447,8 @@ struct Results {
     }
 };
 
+constexpr float BEHIND = 8.f; // powers of two by which m may stay behind the largest logit
+
 // COUNT groups of N operands, each read from the LDS while the products of the one before it are formed.  Left to itself the compiler reads one operand, waits, and goes on
 // with its product.
 template <int N, int COUNT, typename R, typename F>
@@ -477,6 +492,7 @@ __device__ __forceinline__ void attend_few(const AttentionParams &p, const Piece
 {
     constexpr int D = S::D, KT = S::KT, BLOCKS = KT / 16;
     constexpr bool FP8 = S::FP8;
+    constexpr int AHEAD = PAGED_BLOCKS ? S::AHEAD : 1;
     constexpr int PIECES = D / (FP8 ? 64 : 32); // 16-byte pieces of a key in a lane
     constexpr uint64_t ALL = KT == 64 ? ~(uint64_t)0 : ((uint64_t)1 << (KT & 63)) - 1;
     const int lane = (int)threadIdx.x & 63, row = lane & 15, quarter = lane >> 4, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -522,24 +538,25 @@ __device__ __forceinline__ void attend_few(const AttentionParams &p, const Piece
     // tiles on their way: keys as the matrix instructions take them, lane -> entry lane & 15 of 16, values by whole entries
     const char *k_head = p.k + head * p.k_head, *v_head = p.v + head * p.v_head;
     constexpr int ACROSS = FP8 ? D / 16 : S::CHUNKS, PER_LOAD = 64 / ACROSS; // pieces of an entry, entries of a load
-    uint4 k[BLOCKS][PIECES], v[S::LOADS];
-    uint64_t there = 0;
-    const auto ask = [&](int step) {
+    uint4 k[AHEAD][BLOCKS][PIECES], v[AHEAD][S::LOADS];
+    uint64_t there[AHEAD] = {};
+    const auto ask = [&](auto slot, int step) {
+        constexpr int B = decltype(slot)::value;
         int l = lane;
         asm volatile("" : "+v"(l)); // what follows from it is formed anew for each tile: kept, it would take the registers that the tiles need
         const int row = l & 15, k_byte = 16 * (l >> 4), in_load = l / ACROSS, v_byte = 16 * (l % ACROSS), bytes = (FP8 ? 1 : 2) * p.size; // piece i of a key is at k_byte + 64 i
         if constexpr (PAGED_BLOCKS) {
             if (step % blocks.TILES == 0) {
-                blocks.find(p, u, begin, end, step);
+                blocks.find(again(), u, begin, end, step);
             }
-            there = blocks.there(step);
+            there[B] = blocks.there(step);
             const uint32_t k_lane = (uint32_t)(row * (int)p.k_token + k_byte), v_lane = v_byte < bytes ? (uint32_t)(in_load * (int)p.v_token + v_byte) : PAST_BLOCKS;
 #pragma unroll
             for (int b = 0; b < BLOCKS; ++b) {
                 const Buffer from = buffer_of(k_head + blocks.key(step, b), blocks.entries(step, b) * p.k_token);
 #pragma unroll
                 for (int i = 0; i < PIECES; ++i) {
-                    k[b][i] = load16(from, k_byte + 64 * i < bytes ? k_lane : PAST_BLOCKS, 64 * i);
+                    k[B][b][i] = load16(from, k_byte + 64 * i < bytes ? k_lane : PAST_BLOCKS, 64 * i);
                 }
             }
 #pragma unroll
@@ -547,12 +564,12 @@ __device__ __forceinline__ void attend_few(const AttentionParams &p, const Piece
                 const Buffer from = buffer_of(v_head + blocks.value(step, b), blocks.entries(step, b) * p.v_token);
 #pragma unroll
                 for (int i = 0; i < 16 / PER_LOAD; ++i) {
-                    v[b * (16 / PER_LOAD) + i] = load16(from, v_lane, i * PER_LOAD * (uint32_t)p.v_token);
+                    v[B][b * (16 / PER_LOAD) + i] = load16(from, v_lane, i * PER_LOAD * (uint32_t)p.v_token);
                 }
             }
         } else {
             entries.place(p);
-            there = entries.next;
+            there[B] = entries.next;
             entries.ask<KT>(p, u, begin + (step + 1) * S::STEP, end, lane);
 #pragma unroll
             for (int b = 0; b < BLOCKS; ++b) {
@@ -560,7 +577,7 @@ __device__ __forceinline__ void attend_few(const AttentionParams &p, const Piece
                 const bool ok = ((entries.next >> (16 * b + row)) & 1) != 0;
 #pragma unroll
                 for (int i = 0; i < PIECES; ++i) {
-                    k[b][i] = load16(ok && k_byte + 64 * i < bytes ? k_head + at + (k_byte + 64 * i) : (const char *)NOTHING);
+                    k[B][b][i] = load16(ok && k_byte + 64 * i < bytes ? k_head + at + (k_byte + 64 * i) : (const char *)NOTHING);
                 }
             }
 #pragma unroll
@@ -568,13 +585,14 @@ __device__ __forceinline__ void attend_few(const AttentionParams &p, const Piece
                 const int of = i * PER_LOAD + in_load;
                 const int64_t at = from_lane(entries.v, of);
                 const bool ok = ((entries.next >> of) & 1) != 0 && v_byte < bytes;
-                v[i] = load16(ok ? v_head + at + v_byte : (const char *)NOTHING);
+                v[B][i] = load16(ok ? v_head + at + v_byte : (const char *)NOTHING);
             }
         }
     };
-    const auto tile = [&](int step) {
+    const auto tile = [&](auto slot, int step) {
+        constexpr int B = decltype(slot)::value;
         const int tile0 = begin + step * S::STEP;
-        const uint64_t seen = there;
+        const uint64_t seen = there[B];
         const bool limited = first_limit < min(tile0 + KT, end); // not all rows see all of its entries
         int l = lane;
         asm volatile("" : "+v"(l)); // as above
@@ -584,10 +602,10 @@ __device__ __forceinline__ void attend_few(const AttentionParams &p, const Piece
             const int of = i * PER_LOAD + in_load;
             char *to = mine + of * S::PITCH;
             if constexpr (FP8) {
-                *(uint4 *)(to + 16 * ((2 * piece) ^ S::value_swizzle(of))) = as_uint4(from_bytes(v[i].x, v[i].y));
-                *(uint4 *)(to + 16 * ((2 * piece + 1) ^ S::value_swizzle(of))) = as_uint4(from_bytes(v[i].z, v[i].w));
+                *(uint4 *)(to + 16 * ((2 * piece) ^ S::value_swizzle(of))) = as_uint4(from_bytes(v[B][i].x, v[B][i].y));
+                *(uint4 *)(to + 16 * ((2 * piece + 1) ^ S::value_swizzle(of))) = as_uint4(from_bytes(v[B][i].z, v[B][i].w));
             } else {
-                *(uint4 *)(to + 16 * (piece ^ S::value_swizzle(of))) = v[i];
+                *(uint4 *)(to + 16 * (piece ^ S::value_swizzle(of))) = v[B][i];
             }
         }
         f32x4 s[BLOCKS];
@@ -598,15 +616,15 @@ __device__ __forceinline__ void attend_few(const AttentionParams &p, const Piece
             for (int i = 0; i < D / 32; ++i) {
                 bf16x8 key;
                 if constexpr (FP8) {
-                    key = (i & 1) == 0 ? from_bytes(k[b][i / 2].x, k[b][i / 2].y) : from_bytes(k[b][i / 2].z, k[b][i / 2].w);
+                    key = (i & 1) == 0 ? from_bytes(k[B][b][i / 2].x, k[B][b][i / 2].y) : from_bytes(k[B][b][i / 2].z, k[B][b][i / 2].w);
                 } else {
-                    key = as_bf16x8(k[b][i]);
+                    key = as_bf16x8(k[B][b][i]);
                 }
                 s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(key, q[i], s[b], 0, 0, 0);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
-        ask(step + 1); // past the end: nothing.  Without a condition, so that how many loads are on their way is known
+        ask(slot, step + AHEAD); // past the end: nothing.  Without a condition, so that how many loads are on their way is known
         if (seen == 0) {
             return;
         }
@@ -628,23 +646,22 @@ __device__ __forceinline__ void attend_few(const AttentionParams &p, const Piece
                 most = fmaxf(most, s[b][i]);
             }
         }
-        most = fmaxf(m, quarter_swap_max(half_swap_max(most)));
-        const float base = (most == -INFINITY ? 0.f : most) * factor; // nothing seen yet: weights of zero
-        const float keep = __builtin_amdgcn_exp2f(fmaf(m, factor, -base));
-        m = most;
-        sum *= keep; // of this lane's quarter of the keys
+        most = quarter_swap_max(half_swap_max(most));
+        if (__any((most - m) * factor > BEHIND)) { // also where nothing has been seen yet
+            const float next = fmaxf(m, most), keep = __builtin_amdgcn_exp2f((m - (next == -INFINITY ? 0.f : next)) * factor);
+            m = next, sum *= keep;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+                o[d] *= keep;
+            }
+        }
+        const float base = (m == -INFINITY ? 0.f : m) * factor; // nothing seen yet: weights of zero
 #pragma unroll
         for (int b = 0; b < BLOCKS; ++b) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], factor, -base));
-                sum += s[b][i];
-            }
-        }
-        if (__any(keep != 1.f)) {
-#pragma unroll
-            for (int d = 0; d < D / 16; ++d) {
-                o[d] *= keep;
+                sum += s[b][i]; // of this lane's quarter of the keys
             }
         }
         if (limited) {
@@ -702,9 +719,23 @@ __device__ __forceinline__ void attend_few(const AttentionParams &p, const Piece
     };
 
     if (steps > 0) {
-        ask(0);
-        for (int step = 0; step < steps; ++step) {
-            tile(step);
+        constexpr std::integral_constant<int, 0> first;
+        constexpr std::integral_constant<int, AHEAD - 1> second;
+        ask(first, 0);
+        if constexpr (AHEAD > 1) {
+            ask(second, 1);
+        }
+        for (int step = 0;;) {
+            tile(first, step);
+            if (++step == steps) {
+                break;
+            }
+            if constexpr (AHEAD > 1) {
+                tile(second, step);
+                if (++step == steps) {
+                    break;
+                }
+            }
         }
     }
 
@@ -724,7 +755,7 @@ __device__ __forceinline__ void attend_few(const AttentionParams &p, const Piece
         }
     }
     __syncthreads();
-    const Results<S> results(p, u, head, shared_prefix);
+    const Results<S> results(again(), u, head, shared_prefix);
     for (int i = (int)threadIdx.x; i < u.rows * (D / 4); i += S::THREADS) {
         const int r = i / (D / 4), at = 4 * (i % (D / 4));
         float most = -INFINITY, total = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
@@ -783,7 +814,13 @@ __device__ __forceinline__ void attend_many(const AttentionParams &p, const Piec
     const bool wave_idle = wave_row >= u.rows;
 
     f32x16 o[D / 32];
-    float m = -INFINITY, sum = 0.f;
+    // sums of the weights: of the rounded ones that the values are multiplied with, by the matrix instructions, which have less to do than the vector ones; but of the
+    // unrounded ones where their logarithm is wanted
+    f32x4 sums = {0.f, 0.f, 0.f, 0.f};
+    float fine_sum = 0.f; // of this lane's half of the keys
+    const bool fine = p.lse != nullptr;
+    const bf16x8 selector = rowsum_selector(lane);
+    float m = -INFINITY;
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) {
         o[d] = zero16();
@@ -805,7 +842,7 @@ __device__ __forceinline__ void attend_many(const AttentionParams &p, const Piec
         const int in_load = lane / ACROSS, piece = lane % ACROSS, bytes = (FP8 ? 1 : 2) * p.size;
         if constexpr (PAGED_BLOCKS) {
             if (step % blocks.TILES == 0) {
-                blocks.find(p, u, u.begin, end, step);
+                blocks.find(again(), u, u.begin, end, step);
             }
             there_next = blocks.there(step);
             const int block = wave * OF_WAVE / 16, count = blocks.entries(step, block);
@@ -889,8 +926,8 @@ __device__ __forceinline__ void attend_many(const AttentionParams &p, const Piec
         asm volatile("" : "+v"(key_at));
         constexpr int GROUP = LIMITED ? 2 : 4; // fewer registers, where there are others to keep
         ahead<GROUP, KT / 32 * D / 16 / GROUP>(
-            [&](int i) { return as_bf16x8(*(const uint4 *)(keys + 32 * (i / (D / 16)) * S::PITCH + (key_at ^ (32 * (i % (D / 16)))))); }, // piece 2 i + half
-            [&](int i, bf16x8 k) { s[i / (D / 16)] = mfma(k, q[i % (D / 16)], s[i / (D / 16)]); });
+            [&](int i) { return as_bf16x8(*(const uint4 *)(keys + 32 * (i % (KT / 32)) * S::PITCH + (key_at ^ (32 * (i / (KT / 32)))))); }, // piece 2 i + half
+            [&](int i, bf16x8 k) { s[i % (KT / 32)] = mfma(k, q[i / (KT / 32)], s[i % (KT / 32)]); });
         if (LIMITED || there != ALL) {
 #pragma unroll
             for (int kb = 0; kb < KT / 32; ++kb) {
@@ -913,31 +950,37 @@ __device__ __forceinline__ void attend_many(const AttentionParams &p, const Piec
                 most = fmaxf(most, s[kb][i]);
             }
         }
-        most = fmaxf(m, half_swap_max(most));
-        const float base = (most == -INFINITY ? 0.f : most) * factor; // nothing seen yet: weights of zero
-        const float keep = __builtin_amdgcn_exp2f(fmaf(m, factor, -base));
-        m = most;
-        float add = 0.f;
-#pragma unroll
-        for (int kb = 0; kb < KT / 32; ++kb) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], factor, -base));
-                add += s[kb][i];
-            }
-        }
-        sum = fmaf(sum, keep, add); // of this lane's half of the keys
-        bf16x8 w[KT / 16];
-#pragma unroll
-        for (int i = 0; i < KT / 16; ++i) {
-            w[i] = pack8(s[i / 2], 8 * (i & 1)); // the weights' one rounding, as an operand: 2^-8 of each at most
-        }
-        if (__any(keep != 1.f)) {
+        most = half_swap_max(most);
+        if (__any((most - m) * factor > BEHIND)) { // also where nothing has been seen yet
+            const float next = fmaxf(m, most), keep = __builtin_amdgcn_exp2f((m - (next == -INFINITY ? 0.f : next)) * factor);
+            m = next, fine_sum *= keep;
+            sums[0] *= __shfl(keep, lane & 15, 64), sums[1] *= __shfl(keep, 16 + (lane & 15), 64);
 #pragma unroll
             for (int d = 0; d < D / 32; ++d) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     o[d][i] *= keep;
+                }
+            }
+        }
+        const float base = (m == -INFINITY ? 0.f : m) * factor; // nothing seen yet: weights of zero
+        bf16x8 w[KT / 16];
+#pragma unroll
+        for (int i = 0; i < KT / 16; ++i) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int at = 8 * (i & 1) + e;
+                s[i / 2][at] = __builtin_amdgcn_exp2f(fmaf(s[i / 2][at], factor, -base));
+                w[i][e] = (bf16_t)s[i / 2][at]; // the one rounding, as an operand: 2^-8 of each at most
+            }
+            sums = __builtin_amdgcn_mfma_f32_16x16x32_bf16(selector, w[i], sums, 0, 0, 0);
+        }
+        if (fine) {
+#pragma unroll
+            for (int kb = 0; kb < KT / 32; ++kb) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    fine_sum += s[kb][i];
                 }
             }
         }
@@ -1007,8 +1050,8 @@ __device__ __forceinline__ void attend_many(const AttentionParams &p, const Piec
     pass(0, whole_steps, std::false_type{});
     pass(whole_steps, steps, std::true_type{});
 
-    const Results<S> results(p, u, head, shared_prefix);
-    sum = half_swap_sum(sum);
+    const Results<S> results(again(), u, head, shared_prefix);
+    const float sum = fine ? half_swap_sum(fine_sum) : rowsum_fetch(sums, lane);
     if (has_row) {
         if (half == 0) {
             results.sums(row, m == -INFINITY ? m : m * factor, sum);
@@ -1024,7 +1067,7 @@ __device__ __forceinline__ void attend_all(const AttentionParams &p, int block, 
     const int share = block / p.kv_heads, head = block - share * p.kv_heads;
     int at = -1, next = 0;
     Piece u;
-    while (shared_prefix ? find_prefix_piece<S>(p, head, share, at, next, u) : find_piece<S>(p, head, share, at, next, u)) {
+    while (shared_prefix ? find_prefix_piece<S>(again(), head, share, at, next, u) : find_piece<S>(again(), head, share, at, next, u)) {
         if constexpr (S::FEW) {
             attend_few<S, PAGED_BLOCKS>(p, u, head, shared_prefix, lds);
         } else {
@@ -1212,6 +1255,9 @@ struct Plan {
 // keys up to which a workgroup has a tile of few rows however few tiles there are
 constexpr int64_t FEW_KEYS = 2048;
 
+// steps of a share of the prefix
+constexpr int64_t LEAST_PREFIX = 4;
+
 Plan plan_of(const kutacc_hip_cached_attention_args_t &a)
 {
     const kutacc_hip_cache_batch_t &b = a.batch;
@@ -1223,7 +1269,11 @@ Plan plan_of(const kutacc_hip_cached_attention_args_t &a)
     by_size(a.cache.head_size, [&](auto d) {
         constexpr int D = decltype(d)::value;
         const int64_t groups = (D <= 128 ? 2 : 1) * (int64_t)kutacc_cu_count(); // workgroups that are on the chip at a time
-        const int64_t prefix_groups = p.shared ? std::max<int64_t>(groups / 2, 1) : 0;
+        // The prefix's workgroups and the sequences' share the CUs, the ones bound by the matrix cores, the others by memory: they are best done at the same time.  Few of the prefix
+        // leave room for the sequences' and have few pieces to join (64 sequences behind 8192 entries: 256 of them 63 us, 128 54, 64 67); where those would be long, every
+        // CU has one (256 behind 16384: 191, 207 and 369).
+        const int64_t steps = p.prefix_few ? 0 : (stacked + 127) / 128 * ((b.prefix_length + 63) / 64) * kv_heads;
+        const int64_t prefix_groups = !p.shared ? 0 : steps <= 32 * (groups / 4) ? groups / 4 : groups / 2;
         p.d = D;
         // steps of a tile's keys, and so few of them that those of all tiles are counted in 30 bits
         const auto steps_of = [](int64_t tiles, int64_t keys, int step, int &log2) {
@@ -1250,7 +1300,7 @@ Plan plan_of(const kutacc_hip_cached_attention_args_t &a)
             p.prefix_tile = S::ROWS;
             p.prefix_tiles = (stacked + S::ROWS - 1) / S::ROWS, p.prefix_steps = steps_of(p.prefix_tiles, b.prefix_length, S::STEP, p.prefix_step_log2);
             const int64_t all = p.prefix_tiles * p.prefix_steps, shares = std::max<int64_t>(1, prefix_groups / kv_heads);
-            p.prefix_per = std::max<int64_t>((all + shares - 1) / shares, 2);
+            p.prefix_per = std::max<int64_t>((all + shares - 1) / shares, LEAST_PREFIX);
             p.prefix_shares = (all + p.prefix_per - 1) / p.prefix_per;
             p.blocks += p.prefix_shares * kv_heads;
         };
