@@ -24,7 +24,6 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "attention_util.h"
 #include "launch_internal.h"
 #include "mfma_tiles.h"
 #include "paged_cache.h"
@@ -113,7 +112,6 @@ struct FewRows {
     static constexpr int PITCH = 2 * D, CHUNKS = D / 8; // bytes and 16-byte pieces of an entry in the LDS
     static constexpr int TILE = KT * PITCH;
     static constexpr int LOADS = TILE / (FP8 ? 2048 : 1024);  // of values
-    static constexpr int AHEAD = 1;
     static constexpr int JOIN = WAVES * ROWS * ((D + 4) * 4 + 8);
     static constexpr int LDS = WAVES * TILE > JOIN ? WAVES * TILE : JOIN;
     // the two pieces that a transposing read takes of each of 8 entries stand in different banks
@@ -492,7 +490,6 @@ __device__ __forceinline__ void attend_few(const AttentionParams &p, const Piece
 {
     constexpr int D = S::D, KT = S::KT, BLOCKS = KT / 16;
     constexpr bool FP8 = S::FP8;
-    constexpr int AHEAD = PAGED_BLOCKS ? S::AHEAD : 1;
     constexpr int PIECES = D / (FP8 ? 64 : 32); // 16-byte pieces of a key in a lane
     constexpr uint64_t ALL = KT == 64 ? ~(uint64_t)0 : ((uint64_t)1 << (KT & 63)) - 1;
     const int lane = (int)threadIdx.x & 63, row = lane & 15, quarter = lane >> 4, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -535,13 +532,12 @@ __device__ __forceinline__ void attend_few(const AttentionParams &p, const Piece
         o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    // tiles on their way: keys as the matrix instructions take them, lane -> entry lane & 15 of 16, values by whole entries
+    // the tile on its way: keys as the matrix instructions take them, lane -> entry lane & 15 of 16, values by whole entries
     const char *k_head = p.k + head * p.k_head, *v_head = p.v + head * p.v_head;
     constexpr int ACROSS = FP8 ? D / 16 : S::CHUNKS, PER_LOAD = 64 / ACROSS; // pieces of an entry, entries of a load
-    uint4 k[AHEAD][BLOCKS][PIECES], v[AHEAD][S::LOADS];
-    uint64_t there[AHEAD] = {};
-    const auto ask = [&](auto slot, int step) {
-        constexpr int B = decltype(slot)::value;
+    uint4 k[BLOCKS][PIECES], v[S::LOADS];
+    uint64_t there = 0;
+    const auto ask = [&](int step) {
         int l = lane;
         asm volatile("" : "+v"(l)); // what follows from it is formed anew for each tile: kept, it would take the registers that the tiles need
         const int row = l & 15, k_byte = 16 * (l >> 4), in_load = l / ACROSS, v_byte = 16 * (l % ACROSS), bytes = (FP8 ? 1 : 2) * p.size; // piece i of a key is at k_byte + 64 i
@@ -549,14 +545,14 @@ __device__ __forceinline__ void attend_few(const AttentionParams &p, const Piece
             if (step % blocks.TILES == 0) {
                 blocks.find(again(), u, begin, end, step);
             }
-            there[B] = blocks.there(step);
+            there = blocks.there(step);
             const uint32_t k_lane = (uint32_t)(row * (int)p.k_token + k_byte), v_lane = v_byte < bytes ? (uint32_t)(in_load * (int)p.v_token + v_byte) : PAST_BLOCKS;
 #pragma unroll
             for (int b = 0; b < BLOCKS; ++b) {
                 const Buffer from = buffer_of(k_head + blocks.key(step, b), blocks.entries(step, b) * p.k_token);
 #pragma unroll
                 for (int i = 0; i < PIECES; ++i) {
-                    k[B][b][i] = load16(from, k_byte + 64 * i < bytes ? k_lane : PAST_BLOCKS, 64 * i);
+                    k[b][i] = load16(from, k_byte + 64 * i < bytes ? k_lane : PAST_BLOCKS, 64 * i);
                 }
             }
 #pragma unroll
@@ -564,12 +560,12 @@ __device__ __forceinline__ void attend_few(const AttentionParams &p, const Piece
                 const Buffer from = buffer_of(v_head + blocks.value(step, b), blocks.entries(step, b) * p.v_token);
 #pragma unroll
                 for (int i = 0; i < 16 / PER_LOAD; ++i) {
-                    v[B][b * (16 / PER_LOAD) + i] = load16(from, v_lane, i * PER_LOAD * (uint32_t)p.v_token);
+                    v[b * (16 / PER_LOAD) + i] = load16(from, v_lane, i * PER_LOAD * (uint32_t)p.v_token);
                 }
             }
         } else {
             entries.place(p);
-            there[B] = entries.next;
+            there = entries.next;
             entries.ask<KT>(p, u, begin + (step + 1) * S::STEP, end, lane);
 #pragma unroll
             for (int b = 0; b < BLOCKS; ++b) {
@@ -577,7 +573,7 @@ __device__ __forceinline__ void attend_few(const AttentionParams &p, const Piece
                 const bool ok = ((entries.next >> (16 * b + row)) & 1) != 0;
 #pragma unroll
                 for (int i = 0; i < PIECES; ++i) {
-                    k[B][b][i] = load16(ok && k_byte + 64 * i < bytes ? k_head + at + (k_byte + 64 * i) : (const char *)NOTHING);
+                    k[b][i] = load16(ok && k_byte + 64 * i < bytes ? k_head + at + (k_byte + 64 * i) : (const char *)NOTHING);
                 }
             }
 #pragma unroll
@@ -585,14 +581,13 @@ __device__ __forceinline__ void attend_few(const AttentionParams &p, const Piece
                 const int of = i * PER_LOAD + in_load;
                 const int64_t at = from_lane(entries.v, of);
                 const bool ok = ((entries.next >> of) & 1) != 0 && v_byte < bytes;
-                v[B][i] = load16(ok ? v_head + at + v_byte : (const char *)NOTHING);
+                v[i] = load16(ok ? v_head + at + v_byte : (const char *)NOTHING);
             }
         }
     };
-    const auto tile = [&](auto slot, int step) {
-        constexpr int B = decltype(slot)::value;
+    const auto tile = [&](int step) {
         const int tile0 = begin + step * S::STEP;
-        const uint64_t seen = there[B];
+        const uint64_t seen = there;
         const bool limited = first_limit < min(tile0 + KT, end); // not all rows see all of its entries
         int l = lane;
         asm volatile("" : "+v"(l)); // as above
@@ -602,10 +597,10 @@ __device__ __forceinline__ void attend_few(const AttentionParams &p, const Piece
             const int of = i * PER_LOAD + in_load;
             char *to = mine + of * S::PITCH;
             if constexpr (FP8) {
-                *(uint4 *)(to + 16 * ((2 * piece) ^ S::value_swizzle(of))) = as_uint4(from_bytes(v[B][i].x, v[B][i].y));
-                *(uint4 *)(to + 16 * ((2 * piece + 1) ^ S::value_swizzle(of))) = as_uint4(from_bytes(v[B][i].z, v[B][i].w));
+                *(uint4 *)(to + 16 * ((2 * piece) ^ S::value_swizzle(of))) = as_uint4(from_bytes(v[i].x, v[i].y));
+                *(uint4 *)(to + 16 * ((2 * piece + 1) ^ S::value_swizzle(of))) = as_uint4(from_bytes(v[i].z, v[i].w));
             } else {
-                *(uint4 *)(to + 16 * (piece ^ S::value_swizzle(of))) = v[B][i];
+                *(uint4 *)(to + 16 * (piece ^ S::value_swizzle(of))) = v[i];
             }
         }
         f32x4 s[BLOCKS];
@@ -616,15 +611,15 @@ __device__ __forceinline__ void attend_few(const AttentionParams &p, const Piece
             for (int i = 0; i < D / 32; ++i) {
                 bf16x8 key;
                 if constexpr (FP8) {
-                    key = (i & 1) == 0 ? from_bytes(k[B][b][i / 2].x, k[B][b][i / 2].y) : from_bytes(k[B][b][i / 2].z, k[B][b][i / 2].w);
+                    key = (i & 1) == 0 ? from_bytes(k[b][i / 2].x, k[b][i / 2].y) : from_bytes(k[b][i / 2].z, k[b][i / 2].w);
                 } else {
-                    key = as_bf16x8(k[B][b][i]);
+                    key = as_bf16x8(k[b][i]);
                 }
                 s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(key, q[i], s[b], 0, 0, 0);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
-        ask(slot, step + AHEAD); // past the end: nothing.  Without a condition, so that how many loads are on their way is known
+        ask(step + 1); // past the end: nothing.  Without a condition, so that how many loads are on their way is known
         if (seen == 0) {
             return;
         }
@@ -647,8 +642,9 @@ __device__ __forceinline__ void attend_few(const AttentionParams &p, const Piece
             }
         }
         most = quarter_swap_max(half_swap_max(most));
-        if (__any((most - m) * factor > BEHIND)) { // also where nothing has been seen yet
-            const float next = fmaxf(m, most), keep = __builtin_amdgcn_exp2f((m - (next == -INFINITY ? 0.f : next)) * factor);
+        const bool follow = (most - m) * factor > BEHIND; // also where nothing has been seen yet; each row for itself, so that none's bits depend on its neighbours
+        if (__any(follow)) {
+            const float next = follow ? most : m, keep = __builtin_amdgcn_exp2f((m - (next == -INFINITY ? 0.f : next)) * factor);
             m = next, sum *= keep;
 #pragma unroll
             for (int d = 0; d < D / 16; ++d) {
@@ -719,23 +715,9 @@ __device__ __forceinline__ void attend_few(const AttentionParams &p, const Piece
     };
 
     if (steps > 0) {
-        constexpr std::integral_constant<int, 0> first;
-        constexpr std::integral_constant<int, AHEAD - 1> second;
-        ask(first, 0);
-        if constexpr (AHEAD > 1) {
-            ask(second, 1);
-        }
-        for (int step = 0;;) {
-            tile(first, step);
-            if (++step == steps) {
-                break;
-            }
-            if constexpr (AHEAD > 1) {
-                tile(second, step);
-                if (++step == steps) {
-                    break;
-                }
-            }
+        ask(0);
+        for (int step = 0; step < steps; ++step) {
+            tile(step);
         }
     }
 
@@ -814,13 +796,7 @@ __device__ __forceinline__ void attend_many(const AttentionParams &p, const Piec
     const bool wave_idle = wave_row >= u.rows;
 
     f32x16 o[D / 32];
-    // sums of the weights: of the rounded ones that the values are multiplied with, by the matrix instructions, which have less to do than the vector ones; but of the
-    // unrounded ones where their logarithm is wanted
-    f32x4 sums = {0.f, 0.f, 0.f, 0.f};
-    float fine_sum = 0.f; // of this lane's half of the keys
-    const bool fine = p.lse != nullptr;
-    const bf16x8 selector = rowsum_selector(lane);
-    float m = -INFINITY;
+    float m = -INFINITY, sum = 0.f; // of this lane's half of the keys
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) {
         o[d] = zero16();
@@ -951,10 +927,10 @@ __device__ __forceinline__ void attend_many(const AttentionParams &p, const Piec
             }
         }
         most = half_swap_max(most);
-        if (__any((most - m) * factor > BEHIND)) { // also where nothing has been seen yet
-            const float next = fmaxf(m, most), keep = __builtin_amdgcn_exp2f((m - (next == -INFINITY ? 0.f : next)) * factor);
-            m = next, fine_sum *= keep;
-            sums[0] *= __shfl(keep, lane & 15, 64), sums[1] *= __shfl(keep, 16 + (lane & 15), 64);
+        const bool follow = (most - m) * factor > BEHIND; // also where nothing has been seen yet; each row for itself, so that none's bits depend on its neighbours
+        if (__any(follow)) {
+            const float next = follow ? most : m, keep = __builtin_amdgcn_exp2f((m - (next == -INFINITY ? 0.f : next)) * factor);
+            m = next, sum *= keep;
 #pragma unroll
             for (int d = 0; d < D / 32; ++d) {
 #pragma unroll
@@ -971,17 +947,8 @@ __device__ __forceinline__ void attend_many(const AttentionParams &p, const Piec
             for (int e = 0; e < 8; ++e) {
                 const int at = 8 * (i & 1) + e;
                 s[i / 2][at] = __builtin_amdgcn_exp2f(fmaf(s[i / 2][at], factor, -base));
+                sum += s[i / 2][at];
                 w[i][e] = (bf16_t)s[i / 2][at]; // the one rounding, as an operand: 2^-8 of each at most
-            }
-            sums = __builtin_amdgcn_mfma_f32_16x16x32_bf16(selector, w[i], sums, 0, 0, 0);
-        }
-        if (fine) {
-#pragma unroll
-            for (int kb = 0; kb < KT / 32; ++kb) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    fine_sum += s[kb][i];
-                }
             }
         }
         // values of 16 keys and 32 channels, transposed: lane -> channel lane & 31, keys 4 half .. + 3 and 8 further on, as the logits have them
@@ -1051,7 +1018,7 @@ __device__ __forceinline__ void attend_many(const AttentionParams &p, const Piec
     pass(whole_steps, steps, std::true_type{});
 
     const Results<S> results(again(), u, head, shared_prefix);
-    const float sum = fine ? half_swap_sum(fine_sum) : rowsum_fetch(sums, lane);
+    sum = half_swap_sum(sum);
     if (has_row) {
         if (half == 0) {
             results.sums(row, m == -INFINITY ? m : m * factor, sum);

@@ -21,9 +21,8 @@ def close(got, want, bound, what):
     assert got.shape == want.shape, (what, got.shape, want.shape)
     assert torch.equal(torch.isnan(got), torch.isnan(want)), what
     same = (got == want) | torch.isnan(want)
-    off = torch.where(same, torch.zeros_like(want), (got - want).abs())
-    worst = (off / (bound + 1e-300)).max() if off.numel() else 0.0
-    assert worst <= 1.0, f"{what}: {float(worst):.3g} times the bound at {int((off / (bound + 1e-300)).argmax())}"
+    off = torch.where(same, torch.zeros_like(want), (got - want).abs() / (bound + 1e-300))
+    assert off.numel() == 0 or off.max() <= 1.0, f"{what}: {float(off.max()):.3g} times the bound at {int(off.argmax())}"
 
 
 # ---- rotary positions ----
@@ -70,7 +69,7 @@ def attention(q, k, v, seen, scale):
     most = logits.max(1, keepdim=True).values if k.shape[0] else torch.full((q.shape[0], 1), -math.inf, dtype=torch.float64)
     p = torch.exp(logits - torch.where(most == -math.inf, torch.zeros_like(most), most))
     total = p.sum(1, keepdim=True)
-    p = torch.where(total > 0, p / total, torch.zeros_like(p))
+    p = torch.where(total == 0, torch.zeros_like(p), p / total)  # what is no number stays none
     vz = torch.where(torch.isfinite(v), v, torch.zeros_like(v))
     out = p @ vz
     mass = p @ vz.abs()

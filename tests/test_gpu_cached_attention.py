@@ -228,11 +228,10 @@ class Batch:
         call.workspace.fill_(0xff)
         ok(call)
         assert torch.equal(first.view(torch.int16), out.buffer.view(torch.int16)), f"{what}: other bits the second time"
-        # without the logarithm the sums may be of the rounded weights: off by as much once more
+        bits = out.view.contiguous().clone()
         out.buffer.fill_(FILL)
         ok(capi.CachedAttention(cache, batch, qi.view, out.view, scale=scale, causal=causal))
-        oracle.close(out.view[mine], want[mine], bound[mine] + want[mine].abs() * self.coarse(heads // self.kv_heads) * (1 + 2.0 ** -7), f"out without lse {what}")
-        out.untouched(what)
+        assert torch.equal(bits.view(torch.int16), out.view.contiguous().view(torch.int16)), f"{what}: other bits without lse"
         return out.view
 
 
@@ -277,3 +276,394 @@ def test_attention(sequences, prefix, page, heads, kv_heads, size, causal, dtype
     layout = ("slots", "heads", "padded")[(page + len(sequences)) % 3]
     b = Batch(sequences, prefix, page, kv_heads, size, dtype, layout=layout, in_front=odd * 2, behind=3 - odd)
     b.check(heads, causal, pad=3 * odd, offset=odd, outer=page % 2 == 0, what=f"{sequences} {prefix} {page} {heads} {kv_heads} {size}")
+
+
+def test_attention_lengths_around_every_border():
+    """One sequence after the other, of lengths around the tiles', the blocks' and the pages' ends, with a few tokens each."""
+    lengths = [1, 2, 15, 16, 17, 31, 32, 33, 47, 48, 49, 63, 64, 65, 127, 128, 129, 191, 192, 193, 255, 256, 257, 511, 512, 513, 1023, 1025]
+    for page in (16, 48, 20):
+        for size, heads, kv_heads, tokens in ((128, 4, 2, 1), (64, 3, 1, 5), (128, 40, 1, 3)):
+            b = Batch([(min(tokens, n), n) for n in lengths], 0, page, kv_heads, size, seed=page, spare_columns=0)
+            b.check(heads, what=f"{page} {size} {tokens}")
+
+
+@pytest.mark.parametrize("queries", [1, 3, 40])
+def test_prefix_lengths_around_every_border(queries):
+    for prefix in (1, 15, 16, 17, 63, 64, 65, 127, 128, 129, 1000, 1024, 1025):
+        b = Batch([(queries, 50), (queries, 41), (queries, 300)], prefix, 16, 2, 64, seed=prefix)
+        b.check(4, what=f"{queries} {prefix}")
+
+
+@pytest.mark.parametrize("queries,prefix", [(1, 0), (1, 70), (30, 0), (30, 70), (200, 70)])
+def test_pages_that_are_not_there(queries, prefix):
+    """Their entries are not seen, whatever number stands for them."""
+    b = Batch([(queries, 200), (queries, 333), (min(queries, 16), 16), (queries, 210)], prefix, 16, 2, 64, seed=3)
+    b.table[0, 2], b.table[0, 5], b.table[1, 0], b.table[1, -2], b.table[2, 0] = -1, b.pages, -(1 << 31), (1 << 31) - 1, -5
+    if prefix:
+        b.prefix_pages[1] = b.pages + 7
+    b.check(4, what="missing pages")
+
+
+def test_a_length_past_the_page_table():
+    """Entries past its columns are not there; positions are those of the length all the same."""
+    b = Batch([(4, 100), (1, 64), (4, -3)], 30, 16, 2, 64, spare_columns=0)
+    b.lengths[0], b.lengths[1] = 130, 1000
+    b.sequences = [(4, 130), (1, 1000), (4, -3)]
+    b.check(4, what="past the table")
+
+
+@pytest.mark.parametrize("size", [64, 128, 256])
+@pytest.mark.parametrize("heads,queries", [(2, 7), (2, 60), (16, 33)])
+@pytest.mark.parametrize("page", [16, 6])
+def test_what_is_not_seen_may_be_anything(heads, queries, size, page):
+    """Infinities and NaN among the entries that a token must not see yet change nothing of its results; those of the tokens that see them are theirs."""
+    b = Batch([(queries, queries + 10), (5, 90)], 0, page, 1, size, seed=5)
+    q = randn(9, b.tokens, heads, size)
+    cache, batch = b.on_gpu()
+    clean, out = torch.empty(b.tokens, heads, size, dtype=BF16, device="cuda"), torch.empty(b.tokens, heads, size, dtype=BF16, device="cuda")
+    ok(capi.CachedAttention(cache, batch, q.cuda(), clean))
+    wild = {(0, queries + 4): (math.nan, math.inf), (0, queries + 8): (1.0, -math.inf), (1, 88): (math.inf, math.nan)}  # (sequence, entry): of its key, of its value
+    for (s, at), (k, v) in wild.items():
+        page_at = int(b.table[s, at // page])
+        b.gpu[0][page_at, at % page, 0, 3], b.gpu[1][page_at, at % page, 0, 1] = k, v
+    ok(capi.CachedAttention(cache, batch, q.cuda(), out))
+    first = queries + 10 - queries  # entries in front of the first token's
+    free = list(range(0, queries + 4 - first)) + list(range(queries, queries + 3))  # tokens that see none of them
+    assert torch.equal(out[free].view(torch.int16), clean[free].view(torch.int16))
+    seen = [queries + 4 - first, queries - 1, queries + 3, queries + 4]
+    assert bool(torch.isnan(out[seen]).any(2).all()), "a NaN that is seen"
+    # values alone: an infinity stays one, in its channel alone
+    b2 = Batch([(queries, queries + 10)], 0, page, 1, size, seed=5)
+    cache, batch = b2.on_gpu()
+    at = queries + 6
+    b2.gpu[1][int(b2.table[0, at // page]), at % page, 0, 2] = -math.inf
+    q = randn(9, b2.tokens, heads, size)
+    ok(capi.CachedAttention(cache, batch, q.cuda(), out[:queries]))
+    sees = torch.arange(queries) + 10 >= at
+    assert bool((out[:queries][sees][..., 2] == -math.inf).all()) and bool(torch.isfinite(out[:queries][~sees]).all())
+    rest = out[:queries].clone()
+    rest[..., 2] = 0
+    assert bool(torch.isfinite(rest).all())
+
+
+def test_large_logits_and_scales():
+    """Logits that grow along the keys, so that the maximum has to be followed, and such that one key has all of the weight."""
+    for size, heads, queries in ((64, 4, 1), (128, 4, 40)):
+        b = Batch([(queries, 700)], 0, 16, 1, size, values=lambda x: x * 4)
+        for scale in (1e-30, 0.01, 1.0, 30.0):
+            b.check(heads, scale=scale, what=f"scale {scale}")
+        grow = Batch([(queries, 700)], 0, 16, 1, size)
+        q = randn(1, grow.tokens, heads, size).abs()
+        for i in range(700):  # keys along q
+            grow.k[int(grow.table[0, i // 16]), i % 16, 0] = torch.full((size,), 0.02 * i).to(BF16)
+        grow.check(heads, scale=0.05, q=q, what="growing")
+
+
+def test_a_row_with_no_weight_at_all():
+    """Keys of -inf logits alone: zeros, and -inf."""
+    b = Batch([(1, 20), (1, 3)], 0, 16, 1, 64)
+    b.k[int(b.table[1, 0]), :3, 0] = -math.inf
+    cache, batch = b.on_gpu()
+    q, out, lse = torch.ones(2, 4, 64, dtype=BF16, device="cuda"), torch.full((2, 4, 64), FILL, dtype=BF16, device="cuda"), torch.zeros(2, 4, device="cuda")
+    ok(capi.CachedAttention(cache, batch, q, out, lse=lse))
+    assert bool((out[1] == 0).all()) and bool((lse[1] == -math.inf).all()) and bool(torch.isfinite(lse[0]).all())
+
+
+def test_a_cache_of_more_than_2_to_the_32_bytes():
+    """Keys and values at both ends of one, each page's number times its bytes past 32 bits, in slots and in heads outside of them."""
+    page, kv_heads, size = 16, 8, 128
+    pages = (5 << 30) // (2 * page * kv_heads * size)
+    for outer in (False, True):
+        whole = torch.empty(pages, *((kv_heads, page) if outer else (page, kv_heads)), size, dtype=BF16, device="cuda")
+        view = whole.transpose(1, 2) if outer else whole
+        b = Batch([(1, 300), (2, 90)], 40, page, kv_heads, size, seed=11)
+        far = torch.randperm(b.pages, generator=torch.Generator().manual_seed(1)) * ((pages - 1) // b.pages)
+        far[-1] = pages - 1
+        for t in (b.k, b.v):
+            t[t.isnan()] = 0
+        view[far.cuda()] = b.k.cuda()
+        cache = capi.Cache(view, view)
+        batch = capi.CacheBatch(b.query_starts.cuda(), b.lengths.cuda(), far[b.table.clamp(0).long()].to(INT32).cuda(), far[b.prefix_pages.long()].to(INT32).cuda(), 40)
+        b.v = b.k
+        q = randn(2, b.tokens, 16, size)
+        out = torch.empty(b.tokens, 16, size, dtype=BF16, device="cuda")
+        ok(capi.CachedAttention(cache, batch, q.cuda(), out))
+        want, _, bound, _ = b.attention(q, size ** -0.5, True)
+        oracle.close(out, want, bound, "far pages")
+        k, v = randn(3, b.tokens, kv_heads, size), randn(4, b.tokens, kv_heads, size)
+        ok(capi.CacheAppend(cache, batch, k.cuda(), k.cuda()))
+        at = int(far[int(b.table[0, 299 // page])])
+        assert torch.equal(view[at, 299 % page].cpu(), k[0])
+        del whole, view, cache
+        torch.cuda.empty_cache()
+
+
+# ---- appending ----
+
+APPENDS = [  # (queries, length), prefix, page, q heads, kv_heads, size, rotated, first, interleaved
+    ([(1, 1)], 0, 16, 4, 1, 64, 64, 0, False), ([(1, 17), (1, 1), (1, 300)], 2048, 16, 32, 8, 128, 128, 0, False), ([(5, 40), (0, 9), (33, 33)], 7, 3, 2, 2, 64, 32, 16, True),
+    ([(300, 500), (2, 2)], 0, 64, 6, 3, 96, 48, 0, False), ([(7, 7)], 100, 1, 0, 4, 256, 256, 0, True), ([(9, 20)], 0, 16, 3, 2, 48, 20, 4, False), ([(3, 50)], 0, 16, 4, 2, 32, 0, 0, False),
+    ([(2, 30)] * 300, 64, 16, 5, 1, 64, 64, 0, False), ([(1, 1 + 13 * i % 200) for i in range(70)], 5, 16, 8, 2, 128, 64, 64, True),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3], ids=["bf16", "e4m3"])
+@pytest.mark.parametrize("sequences,prefix,page,heads,kv_heads,size,turned,first,interleaved", APPENDS)
+def test_append(sequences, prefix, page, heads, kv_heads, size, turned, first, interleaved, dtype):
+    odd = len(sequences) % 2
+    b = Batch(sequences, prefix, page, kv_heads, size, dtype, layout=("slots", "heads", "padded")[page % 3], in_front=odd, behind=2)
+    tokens = b.tokens
+    q, k, v = randn(1, tokens, max(heads, 1), size, scale=3.0), randn(2, tokens, kv_heads, size, scale=3.0), randn(3, tokens, kv_heads, size, scale=3.0)
+    inv_freq = capi.rotary_frequencies(turned).cuda() if turned else None
+    cache, batch = b.on_gpu()
+    before = [x.clone() for x in b.gpu]
+    qi, qo = Placed(tokens, max(heads, 1), size, pad=odd, values=q), Placed(tokens, max(heads, 1), size, pad=8, outer=bool(odd))
+    ki, vi = Placed(tokens, kv_heads, size, pad=3 * odd, offset=odd, values=k), Placed(tokens, kv_heads, size, outer=True, values=v)
+    more = dict(q=qi.view, q_out=qo.view) if heads else {}
+    ok(capi.CacheAppend(cache, batch, ki.view, vi.view, inv_freq, interleaved=interleaved, first=first, magnitude=1.5, **more))
+    inv_freq = torch.zeros(0) if inv_freq is None else inv_freq.cpu()
+    positions = torch.zeros(tokens, dtype=torch.long)
+    for i, (n, length) in enumerate(sequences):
+        positions[b.starts[i]:b.starts[i] + n] = prefix + length - n + torch.arange(n)
+    mine = slice(b.starts[0], b.starts[-1])
+    if heads:
+        want, off = oracle.rotated(q, positions, inv_freq, interleaved, first, False, 1.5)
+        oracle.close(qo.view[mine], want[mine], oracle.stored(want, off, BF16)[mine], "q")
+        assert bool((qo.view[:mine.start] == FILL).all()) and bool((qo.view[mine.stop:] == FILL).all()), "queries of padding"
+        qo.untouched("q")
+    k_want, k_off = oracle.rotated(k, positions, inv_freq, interleaved, first, False, 1.5)
+    for got, old, want, off, scales, what in ((b.gpu[0], before[0], k_want, k_off, b.scales[0], "k"), (b.gpu[1], before[1], oracle.d(v), torch.zeros_like(oracle.d(v)), b.scales[1], "v")):
+        got = got.cpu()
+        kept = torch.ones(got.shape[:2], dtype=torch.bool)
+        if scales is not None:  # divided in 32 bits
+            want, off = want / scales.double()[:, None], off / scales.double()[:, None] + (want / scales.double()[:, None]).abs() * 2.0 ** -24
+            want = want.clamp(-448, 448)
+        for i, (n, length) in enumerate(sequences):
+            for j in range(n):
+                t, at = b.starts[i] + j, length - n + j
+                place = int(b.table[i, at // page]), at % page
+                kept[place] = False
+                oracle.close(got[place], want[t], oracle.stored(want[t], off[t], dtype), f"{what} {i} {j}")
+        old, got = ((x.view(torch.uint8) if dtype == E4M3 else x.view(torch.int16)) for x in (old.cpu(), got))
+        assert torch.equal(old[kept], got[kept]), f"{what}: written outside of its places"
+
+
+def test_append_of_tokens_without_a_place():
+    """In front of the sequence's entries, past its page table, on pages outside of the cache: nothing is kept of them, their queries are rotated."""
+    b = Batch([(5, 3), (2, 40), (3, 60)], 10, 16, 2, 64, spare_columns=0)
+    b.lengths[1] = 65  # the last column ends at 64: one of the two is past it
+    b.table[2, 3] = -1  # entries 48 .. 63
+    cache, batch = b.on_gpu()
+    before = b.gpu[0].clone()
+    q, k = randn(1, 10, 4, 64), randn(2, 10, 2, 64)
+    inv_freq, q_out = capi.rotary_frequencies(64), torch.empty(10, 4, 64, dtype=BF16, device="cuda")
+    ok(capi.CacheAppend(cache, batch, k.cuda(), k.cuda(), inv_freq.cuda(), q=q.cuda(), q_out=q_out))
+    positions = torch.tensor([10 + 3 - 5 + i for i in range(5)] + [10 + 63, 10 + 64] + [10 + 57 + i for i in range(3)])
+    want, off = oracle.rotated(q, positions, inv_freq)
+    oracle.close(q_out, want, oracle.stored(want, off, BF16), "q")
+    changed = (before.view(torch.int16) != b.gpu[0].view(torch.int16)).any(3).any(2).nonzero().tolist()
+    places = [[int(b.table[0, 0]), i] for i in range(3)] + ([[int(b.table[1, 63 // 16]), 63 % 16]] if int(b.table[1, 63 // 16]) >= 0 else [])
+    assert sorted(changed) == sorted(places)
+
+
+def test_append_saturates_and_keeps_what_is_no_number():
+    b = Batch([(3, 3)], 0, 16, 1, 32, E4M3)
+    cache, batch = b.on_gpu()
+    k = torch.zeros(3, 1, 32, dtype=BF16)
+    k[0, 0, :4], k[1, 0, 0], k[2, 0, 0] = torch.tensor([1e30, -1e30, math.inf, -math.inf]), math.nan, 1.0
+    ok(capi.CacheAppend(cache, batch, k.cuda(), k.cuda()))
+    got = b.gpu[1][int(b.table[0, 0]), :3, 0].cpu().float()
+    assert got[0, :4].tolist() == [448, -448, 448, -448] and math.isnan(got[1, 0])
+    assert float(got[2, 0]) == float((torch.tensor(1.0) / b.scales[1][0]).to(E4M3).float())
+
+
+def test_append_with_positions_of_its_own():
+    b = Batch([(4, 10), (2, 2)], 0, 16, 2, 64)
+    cache, batch = b.on_gpu()
+    positions = torch.tensor([7, 3, -9, 100000, 1, 0], dtype=INT32)
+    q, inv_freq = randn(1, 6, 2, 64), capi.rotary_frequencies(64)
+    there = q.cuda()
+    ok(capi.CacheAppend(cache, batch, q.cuda(), q.cuda(), inv_freq.cuda(), q=there, positions=positions.cuda()))  # q in place
+    want, off = oracle.rotated(q, positions, inv_freq)
+    oracle.close(there, want, oracle.stored(want, off, BF16), "q in place")
+    oracle.close(b.gpu[0][int(b.table[0, 0]), 6], want[0], oracle.stored(want, off, BF16)[0], "k")
+
+
+# ---- together ----
+
+def test_decoding_steps_as_a_user_makes_them():
+    """A prompt behind a shared prefix, then token after token: append, attend; lengths go on on the device.  Against attention over all that was ever appended, in 64 bits from
+    the unrounded inputs: keys and queries are rounded once (2^-8 of each product's two factors), values and results once."""
+    page, heads, kv_heads, size, prefix = 16, 8, 2, 64, 37
+    counts = [(20, 5), (1, 1), (70, 3)]
+    inv_freq = capi.rotary_frequencies(size)
+    b = Batch([(n, n) for n, _ in counts], prefix, page, kv_heads, size, seed=21, spare_columns=3)
+    spare = b.pages - 2  # two pages that nobody has yet, in each row's spare columns
+    for i in range(3):
+        b.table[i, -3:] = -1
+    grown = torch.full((b.pages + 12, page, kv_heads, size), math.nan, dtype=BF16)
+    caches = []
+    for t in (b.k, b.v):
+        g = grown.clone()
+        g[:b.pages] = t
+        caches.append(g.cuda())
+    for i in range(3):
+        used = -(-counts[i][0] // page)
+        for c in range(used, b.table.shape[1]):
+            b.table[i, c] = b.pages + 4 * i + c - used if c - used < 4 else -1
+    del spare
+    lengths = torch.zeros(3, dtype=INT32, device="cuda")
+    table, prefix_pages = b.table.cuda(), b.prefix_pages.cuda()
+    cache = capi.Cache(*caches)
+    history = [([], []) for _ in counts]
+    k_prefix, v_prefix = (oracle.placed(t, None, b.prefix_pages.tolist(), page, prefix)[0] for t in (b.k, b.v))
+    seed = 100
+    for step in range(4):
+        new = [n if step == 0 else 1 for n, _ in counts]
+        starts = torch.tensor([0, new[0], new[0] + new[1], sum(new)], dtype=INT32)
+        lengths += torch.tensor(new, dtype=INT32, device="cuda")
+        batch = capi.CacheBatch(starts.cuda(), lengths, table, prefix_pages, prefix)
+        tokens = sum(new)
+        seed += 1
+        qkv = randn(seed, tokens, heads + 2 * kv_heads, size)
+        on_gpu = qkv.cuda()
+        q, k, v = on_gpu[:, :heads], on_gpu[:, heads:heads + kv_heads], on_gpu[:, heads + kv_heads:]
+        out = torch.empty(tokens, heads, size, dtype=BF16, device="cuda")
+        ok(capi.CacheAppend(cache, batch, k, v, inv_freq.cuda(), q=q))
+        ok(capi.CachedAttention(cache, batch, q, out))
+        at = 0
+        for i, n in enumerate(new):
+            have = len(history[i][0])
+            positions = prefix + have + torch.arange(n)
+            part = qkv[at:at + n]
+            qr, kr = (oracle.rotated(x, positions, inv_freq)[0] for x in (part[:, :heads], part[:, heads:heads + kv_heads]))
+            history[i][0].extend(kr)
+            history[i][1].extend(part[:, heads + kv_heads:].double())
+            keys, values = torch.cat([k_prefix, torch.stack(history[i][0])]), torch.cat([v_prefix, torch.stack(history[i][1])])
+            seen = torch.arange(len(keys))[None] <= positions[:, None]
+            for h in range(heads):
+                want, _, off, _, mass = oracle.attention(qr[:, h], keys[:, h // 4], values[:, h // 4], seen, size ** -0.5)
+                worst = size ** -0.5 * (qr[:, h].abs() @ keys[:, h // 4].abs().T).max(1, keepdim=True).values * (2 * 2.0 ** -8 + 2.0 ** -16)
+                bound = off + mass * (2 * torch.expm1(worst) + 2.0 ** -8 + 2.0 ** -8) + (want.abs() + mass * 0.1) * 2.0 ** -8
+                oracle.close(out[at:at + n, h], want, bound, f"step {step} sequence {i} head {h}")
+            at += n
+
+
+def test_a_block_of_norm_projections_attention_and_transition_runs():
+    """The attention half next to the feed-forward half: RMS norm in 8 bits, 8-bit projection, append, attention, 8-bit projection, RMS norm, gated transition; against the same
+    steps in 64 bits from what each call was given."""
+    import feed_forward_oracle as ff
+    tokens, width, heads, kv_heads, size = 6, 512, 8, 2, 64
+    b = Batch([(1, 100), (1, 7), (4, 33)], 48, 16, kv_heads, size, seed=31)
+    cache, batch = b.on_gpu()
+    x, gamma = randn(1, tokens, width).cuda(), (1 + 0.1 * randn(2, width, dtype=FP32)).cuda()
+    e8 = lambda *s: torch.empty(*s, dtype=E4M3, device="cuda")
+    f32 = lambda *s: torch.empty(*s, device="cuda")
+    b16 = lambda *s: torch.empty(*s, dtype=BF16, device="cuda")
+    n_qkv = (heads + 2 * kv_heads) * size
+    w_qkv, w_o = (randn(3 + i, *s, scale=s[1] ** -0.5).cuda() for i, s in enumerate(((n_qkv, width), (width, heads * size))))
+    q8, s8, w8, ws8 = e8(tokens, width), f32(tokens, 4), e8(n_qkv, width), f32(n_qkv // 128, 4)
+    qkv = b16(tokens, heads + 2 * kv_heads, size)
+    q, k, v = qkv[:, :heads], qkv[:, heads:heads + kv_heads], qkv[:, heads + kv_heads:]
+    out, o8, os8, wo8, wos8, y, s, n = b16(tokens, heads, size), e8(tokens, heads * size), f32(tokens, 4), e8(width, heads * size), f32(4, 4), b16(tokens, width), b16(tokens, width), b16(tokens, width)
+    wg, wu, wd, z = randn(7, 1024, width, scale=width ** -0.5).cuda(), randn(8, 1024, width, scale=width ** -0.5).cuda(), randn(9, width, 1024, scale=1024 ** -0.5).cuda(), b16(tokens, width)
+    inv_freq = capi.rotary_frequencies(size).cuda()
+    for w, to, scales in ((w_qkv, w8, ws8), (w_o, wo8, wos8)):
+        ok(capi.QuantizeFp8(w, to, scales, block_rows=128))
+    ok(capi.RmsNorm(x, gamma, out8=q8, scales=s8))
+    ok(capi.LinearFp8(q8, s8, w8, ws8, qkv.view(tokens, n_qkv)))
+    given = qkv.clone()
+    ok(capi.CacheAppend(cache, batch, k, v, inv_freq, q=q))
+    b.k, b.v = (t.cpu() for t in b.gpu)
+    ok(capi.CachedAttention(cache, batch, q, out))
+    ok(capi.QuantizeFp8(out.view(tokens, -1), o8, os8))
+    ok(capi.LinearFp8(o8, os8, wo8, wos8, y))
+    ok(capi.RmsNorm(y, gamma, residual=x, sum=s, out=n))
+    ok(capi.GatedTransition(n, wg, wu, wd, z))
+    positions = torch.tensor([48 + 99, 48 + 6] + [48 + 29 + i for i in range(4)])
+    want, off = oracle.rotated(given[:, :heads], positions, inv_freq)
+    oracle.close(q, want, oracle.stored(want, off, BF16), "rotated q")
+    want, _, bound, _ = b.attention(q.cpu(), size ** -0.5, True)
+    oracle.close(out, want, bound, "attention")
+    assert bool(torch.isfinite(z).all()) and float(z.float().abs().mean()) > 0
+    total, norm = ff.rms_norm(y, gamma, 1e-6, x)
+    oracle.close(s, total, total.abs() * 2.0 ** -8 * 1.01 + 1e-30, "residual")
+    oracle.close(n, norm, norm.abs() * (2.0 ** -8 + ff.norm_slack(width)) * 1.01 + 1e-30, "norm")
+
+
+def test_captured_and_replayed_with_other_lengths_and_eager_calls_between():
+    """A captured step goes on with the lengths, tables and queries that it finds; other streams and calls in between."""
+    b = Batch([(1, 900), (1, 3), (1, 200), (1, 64)], 300, 16, 2, 128, seed=41, values=lambda x: x)
+    for t in (b.k, b.v):
+        t[t.isnan()] = 0.5
+    cache, batch = b.on_gpu()
+    heads, inv_freq = 8, capi.rotary_frequencies(128).cuda()
+    q, k, out, q_out = (torch.empty(4, h, 128, dtype=BF16, device="cuda") for h in (heads, 2, heads, heads))
+    rotary = capi.Rotary(q, inv_freq, q_out=q_out)
+    append, attend = capi.CacheAppend(cache, batch, k, k, inv_freq, q=q, q_out=q_out), capi.CachedAttention(cache, batch, q_out, out)
+    eager_out = torch.empty_like(out)
+    eager = capi.CachedAttention(cache, batch, q_out, eager_out)
+    lengths = batch.tensors[1]
+    q.copy_(randn(1, 4, heads, 128).cuda())
+    k.copy_(randn(2, 4, 2, 128).cuda())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for call in (rotary, append, attend):
+            assert call.run(side.cuda_stream) == 0
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        for call in (rotary, append, attend):
+            assert call.run(side.cuda_stream) == 0
+    for i, now in enumerate(([900, 3, 200, 64], [1, 1, 1, 1], [500, 2, 190, 17], [900, 0, 5, 60])):
+        lengths.copy_(torch.tensor(now, dtype=INT32, device="cuda"))
+        q.copy_(randn(10 + i, 4, heads, 128).cuda())
+        out.fill_(FILL)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert eager.run() == 0
+        torch.cuda.synchronize()
+        assert torch.equal(out.view(torch.int16), eager_out.view(torch.int16)), now
+        b.k, b.v = (t.cpu() for t in b.gpu)
+        b.sequences = [(1, n) for n in now]
+        want, _, bound, _ = b.attention(q_out.cpu(), 128 ** -0.5, True)
+        oracle.close(out, want, bound, f"{now}")
+
+
+def test_two_streams_at_once():
+    """Calls with workspaces of their own."""
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    work = []
+    for i in range(2):
+        b = Batch([(1, 700 + i), (3, 50), (1, 1000)], 200 * i, 16, 2, 64, seed=50 + i)
+        q = randn(60 + i, b.tokens, 8, 64)
+        cache, batch = b.on_gpu()
+        out = torch.empty(b.tokens, 8, 64, dtype=BF16, device="cuda")
+        work.append((b, q, out, capi.CachedAttention(cache, batch, q.cuda(), out)))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for side, (_, _, _, call) in zip(sides, work):
+            assert call.run(side.cuda_stream) == 0
+    torch.cuda.synchronize()
+    for b, q, out, _ in work:
+        want, _, bound, _ = b.attention(q, 64 ** -0.5, True)
+        oracle.close(out, want, bound, "on a stream of its own")
+
+
+def test_query_starts_that_fall_stay_in_bounds():
+    """Not a call that means anything: nothing outside of the results is written."""
+    b = Batch([(3, 30), (4, 40), (2, 20)], 0, 16, 2, 64)
+    for starts in ([5, 1, 9, 2], [0, 9, 0, 9], [-100, 1 << 30, -5, 7], [9, 9, 9, 9], [0, 1 << 30, 1 << 30, 1 << 30]):
+        b.query_starts = torch.tensor(starts, dtype=INT32)
+        cache, batch = b.on_gpu()
+        out = Placed(9, 4, 64, pad=8)
+        call = capi.CachedAttention(cache, batch, randn(1, 9, 4, 64).cuda(), out.view)
+        room = torch.full((call.workspace.numel() + 4096,), 0x55, dtype=torch.uint8, device="cuda")
+        at = -room.data_ptr() % 256
+        call.args.workspace = room.data_ptr() + at
+        ok(call)
+        out.untouched(str(starts))
+        assert bool((room[at + call.workspace.numel():] == 0x55).all())
+        ok(capi.CacheAppend(cache, batch, randn(2, 9, 2, 64).cuda(), randn(3, 9, 2, 64).cuda()))
