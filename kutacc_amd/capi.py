@@ -737,7 +737,7 @@ class _DeviceCall:
         self.streams.add(stream_ptr)
 
     def __del__(self):
-        if self.workspace is None or not self.workspace.is_cuda or sys.is_finalizing():
+        if self.workspace is None or not self.workspace.is_cuda or sys is None or sys.is_finalizing():
             return
         import torch
         capturing = torch.cuda.is_current_stream_capturing()  # then streams are not to be asked

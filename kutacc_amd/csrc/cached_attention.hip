@@ -11,9 +11,9 @@
 // wants it, V^T P^T, when V is read from the LDS transposed in the same order of keys.  K and V go straight into the LDS, double buffered, 16 bytes a lane from any
 // page; rows that are not there come from a line of zeros.
 //
-// Few rows, up to 16 a tile: memory bounds them.  The waves of a workgroup all have the same rows and in turn a tile of keys, and join at the end.  A wave has two tiles on
-// their way in registers, the largest room there is for them; K is there as the matrix instructions take it, V goes through LDS of the wave's own.  More rows: the matrix cores and the softmax bound them.  Each wave has 32 of 128, and the four share K
-// and V in the LDS.
+// Few rows, up to 16 a tile: memory bounds them.  The waves of a workgroup all have the same rows and in turn a tile of keys, and join at the end.  A wave has a tile at hand
+// and one on its way in registers; K is there as the matrix instructions take it, V goes through LDS of the wave's own.  More rows: the matrix cores and the softmax bound
+// them.  Each wave has 32 of 128, and the four share K and V in the LDS.
 //
 // The work of a kv head, in steps of keys, is split into equal shares, one for each workgroup, as many as the chip holds at a time; a workgroup whose
 // share goes over the end of a tile goes on with the next one.  The lengths are on the device: every wave sums them up and finds its share by itself.  The pieces of a row
@@ -161,7 +161,7 @@ __device__ __forceinline__ Work work_of(const AttentionParams &p, int s)
     return w;
 }
 
-// The piece of share `share` of kv head `head` that starts at `at` of the head's work (below zero: the share's first; no shares: tile `share`), and where the next one does.
+// The piece of share `share` of kv head `head` that starts at `at` of the head's work (below zero: the share's first; no shares: tile `share`), and where the next one does, below zero: nowhere.
 // False: there is none.  Sequences in order, of one its tiles from the last one on, which sees the most entries.
 template <typename S>
 __device__ __forceinline__ bool find_piece(const AttentionParams &p, int head, int share, int &at, int &next, Piece &u)
@@ -169,17 +169,26 @@ __device__ __forceinline__ bool find_piece(const AttentionParams &p, int head, i
     const bool split = p.shares > 0;
     const int lane = (int)threadIdx.x & 63;
     Work w = work_of<S>(p, lane);
-    int work = scan(split ? w.tiles * w.steps : w.tiles); // up to this sequence
-    int per = 1, end = INT32_MAX;                          // steps of a share; where this one's end
+    int per = 1, end = INT32_MAX; // steps of a share; where this one's end
+    bool whole = false;           // whether a share stays in a tile: those of a tile are multiples of `per` then
+    const auto steps_in = [&](const Work &w) { return whole ? (int)(((uint32_t)w.steps + per - 1) / (uint32_t)per) * per : w.steps; };
     if (split) {
-        int all = uniform(work, 63);
-        for (int s0 = 64; s0 < p.sequences; s0 += 64) {
-            const Work more = work_of<S>(p, s0 + lane);
-            all += uniform(scan(more.tiles * more.steps), 63);
+        int all = 0, all_tiles = 0;
+        Work more = w;
+        for (int s0 = 64;; s0 += 64) {
+            all += uniform(scan(more.tiles * more.steps), 63), all_tiles += uniform(scan(more.tiles), 63);
+            if (s0 >= p.sequences) {
+                break;
+            }
+            more = work_of<S>(p, s0 + lane);
         }
-        per = max((int)p.by_share.quotient((uint32_t)(all + p.shares - 1)), p.least);
-        at = at < 0 ? (int)min((int64_t)share * per, (int64_t)all) : at;
-        end = (int)min((int64_t)(share + 1) * per, (int64_t)all);
+        // A second piece costs its workgroup as much as some steps: with few tiles each piece has a workgroup of its own, all / per + tiles of them at most (8 sequences of 1 to
+        // 1500 entries, 64 tiles: 14.6 us, with even shares 19.9; with more than a quarter as many tiles as shares these are the better ones, 123 us instead of 157 for 128 of 10000)
+        whole = 4 * all_tiles <= p.shares;
+        per = max((int)(whole ? (uint32_t)(all + p.shares - all_tiles - 1) / (uint32_t)(p.shares - all_tiles) : p.by_share.quotient((uint32_t)(all + p.shares - 1))), p.least);
+        const int64_t most = whole ? INT32_MAX : all;
+        at = at < 0 ? (int)min((int64_t)share * per, most) : at;
+        end = (int)min((int64_t)(share + 1) * per, most);
         if (at >= end) {
             return false;
         }
@@ -188,18 +197,18 @@ __device__ __forceinline__ bool find_piece(const AttentionParams &p, int head, i
     }
     int work_before = 0, tiles_before = 0;
     for (int s0 = 0;;) {
-        const int tiles = split ? scan(w.tiles) : work;
+        const int padded = steps_in(w), work = scan(split ? w.tiles * padded : w.tiles), tiles = split ? scan(w.tiles) : work; // up to this sequence
         const uint64_t behind = __ballot(at - work_before < work);
         if (behind != 0) {
             const int l = __builtin_ctzll(behind);
             const int first = uniform(w.first, l), tokens = uniform(w.tokens, l), own = uniform(w.own, l), keys = uniform(w.keys, l), steps = uniform(w.steps, l);
-            const int its_tiles = uniform(w.tiles, l), from = work_before + uniform(work, l) - (split ? its_tiles * steps : its_tiles); // the sequence's first
-            const int tile = !split ? at - from : its_tiles == 1 ? 0 : (int)((uint32_t)(at - from) / (uint32_t)steps);
+            const int its_tiles = uniform(w.tiles, l), room = uniform(padded, l), from = work_before + uniform(work, l) - (split ? its_tiles * room : its_tiles); // the sequence's first
+            const int tile = !split ? at - from : its_tiles == 1 ? 0 : (int)((uint32_t)(at - from) / (uint32_t)room);
             const int number = tiles_before + uniform(tiles, l) - its_tiles + tile; // of the tile
-            if (number >= p.most_tiles) {
+            if ((uint32_t)tile >= (uint32_t)its_tiles || (uint32_t)number >= (uint32_t)p.most_tiles) {
                 return false; // more tokens than there are: query_starts that fall
             }
-            const int tile_at = split ? from + tile * steps : at, step = at - tile_at, count = min(steps - step, split ? end - at : steps);
+            const int tile_at = split ? from + tile * room : at, step = at - tile_at, count = min(steps - step, split ? end - at : steps);
             u.table = p.page_table + (int64_t)(s0 + l) * p.page_table_ld;
             u.prefix = p.joined ? p.prefix_length : 0, u.keys = keys;
             u.token0 = first, u.row0 = (its_tiles - 1 - tile) * S::ROWS, u.rows = min(S::ROWS, tokens * (int)p.group.d - u.row0);
@@ -212,7 +221,7 @@ __device__ __forceinline__ bool find_piece(const AttentionParams &p, int head, i
                 u.shares = (int)((uint32_t)(tile_at + steps - 1) / (uint32_t)per) - share0 + 1;
             }
             u.first = head * (p.most_tiles + p.shares) + number + (split ? share0 : 0), u.share = share - share0, u.at = u.first + u.share;
-            next = at + count;
+            next = split && !whole && at + count < end ? at + count : -1;
             return true;
         }
         work_before += uniform(work, 63), tiles_before += uniform(tiles, 63);
@@ -221,7 +230,6 @@ __device__ __forceinline__ bool find_piece(const AttentionParams &p, int head, i
             return false;
         }
         w = work_of<S>(p, s0 + lane);
-        work = scan(split ? w.tiles * w.steps : w.tiles);
     }
 }
 
@@ -241,7 +249,7 @@ __device__ __forceinline__ bool find_prefix_piece(const AttentionParams &p, int 
     u.token0 = 0, u.row0 = tile * S::ROWS, u.rows = min(S::ROWS, p.tokens * (int)p.group.d - u.row0), u.limit0 = INT32_MAX;
     u.begin = step << p.prefix_step_log2, u.end = (int)min((int64_t)(step + count) << p.prefix_step_log2, (int64_t)u.keys);
     u.at = head * (p.prefix_tiles + p.prefix_shares) + tile + share, u.first = 0, u.share = 0, u.shares = 1;
-    next = at + count;
+    next = at + count < end ? at + count : -1;
     return true;
 }
 
@@ -1032,19 +1040,20 @@ template <typename S, bool PAGED_BLOCKS>
 __device__ __forceinline__ void attend_all(const AttentionParams &p, int block, bool shared_prefix, char *lds)
 {
     const int share = block / p.kv_heads, head = block - share * p.kv_heads;
-    int at = -1, next = 0;
-    Piece u;
-    while (shared_prefix ? find_prefix_piece<S>(again(), head, share, at, next, u) : find_piece<S>(again(), head, share, at, next, u)) {
+    int at = -1;
+    do {
+        int next = -1;
+        Piece u;
+        if (!(shared_prefix ? find_prefix_piece<S>(again(), head, share, at, next, u) : find_piece<S>(again(), head, share, at, next, u))) {
+            break;
+        }
         if constexpr (S::FEW) {
             attend_few<S, PAGED_BLOCKS>(p, u, head, shared_prefix, lds);
         } else {
             attend_many<S, PAGED_BLOCKS>(p, u, head, shared_prefix, lds);
         }
-        if (!shared_prefix && p.shares == 0) {
-            break;
-        }
         at = next;
-    }
+    } while (at >= 0);
 }
 
 // OWN: of the sequences' tiles, PREFIX: of the prefix's
@@ -1219,8 +1228,20 @@ struct Plan {
     int64_t prefix_partial, partial, prefix_sums, sums, rows, bytes; // offsets in the workspace, and its size
 };
 
-// keys up to which a workgroup has a tile of few rows however few tiles there are
-constexpr int64_t FEW_KEYS = 2048;
+// Whether the keys of the sequences' tiles are split among workgroups.  Tiles of many rows: where there are fewer of them than the chip holds, as splitting them writes what a
+// 64th of a tile's products takes.  Tiles of few rows: where there are fewer than four times as many, as long sequences among short ones leave the chip to a few workgroups
+// (64 sequences of 1 to 10000 entries, 8 kv heads: 242 us split, 298 not; all of 3000: 143 and 139), but not for few keys, whose pieces cost more to join than
+// they gain: of one CU's workgroups the keys come with 45 bytes a ns, a second kernel takes 3 us.  With an eighth of the chip's tiles 1024 keys (8 sequences: 700 entries 14.5 us
+// split, 14.1 not, 1 to 1500 14.6 and 18.5), with more 2048 (24 sequences of 1500: 40 and 34 us; of 1 to 3000: 41 and 48).  Behind a shared prefix pieces are joined anyway
+// (32 sequences behind 8192 entries: 34 and 40 us).
+template <typename S>
+bool splits(int64_t tiles, int64_t keys, int64_t groups, bool shared)
+{
+    if (!S::FEW) {
+        return tiles < groups;
+    }
+    return tiles < 4 * groups && (shared || keys > (tiles <= groups / 8 ? 1024 : 2048));
+}
 
 // steps of a share of the prefix
 constexpr int64_t LEAST_PREFIX = 4;
@@ -1242,12 +1263,12 @@ Plan plan_of(const kutacc_hip_cached_attention_args_t &a)
         const int64_t steps = p.prefix_few ? 0 : (stacked + 127) / 128 * ((b.prefix_length + 63) / 64) * kv_heads;
         const int64_t prefix_groups = !p.shared ? 0 : steps <= 32 * (groups / 4) ? groups / 4 : groups / 2;
         p.d = D;
-        // steps of a tile's keys, and so few of them that those of all tiles are counted in 30 bits
+        // steps of a tile's keys, and so few of them that those of all tiles are counted in 29 bits, of whole shares in 30
         const auto steps_of = [](int64_t tiles, int64_t keys, int step, int &log2) {
             for (log2 = 0; 1 << log2 < step; ++log2) {
             }
             const auto steps = [&] { return std::max<int64_t>((keys + ((int64_t)1 << log2) - 1) >> log2, 1); };
-            while (log2 < 30 && tiles * steps() >= (int64_t)1 << 30) {
+            while (log2 < 30 && tiles * steps() >= (int64_t)1 << 29) {
                 ++log2;
             }
             return steps();
@@ -1256,9 +1277,10 @@ Plan plan_of(const kutacc_hip_cached_attention_args_t &a)
             using S = decltype(shape);
             const int64_t keys = b.columns * a.cache.page_size + (p.shared ? 0 : b.prefix_length); // at most
             const int64_t tiles = (S::FEW ? std::max(stacked / S::ROWS, with_tokens) : std::max<int64_t>(stacked / S::ROWS, 1)) * kv_heads;
-            p.tile = S::ROWS, p.least = 2, p.waves = S::WAVES;
+            p.tile = S::ROWS, p.waves = S::WAVES;
+            p.least = S::WAVES == 8 ? 1 : 2; // of 256 keys and of 128 or 64 (8 sequences of 1 to 1500: 14.6 us, 16.0 with 2 of 256)
             p.most_tiles = stacked / S::ROWS + with_tokens;
-            p.shares = tiles >= groups || (S::FEW && keys <= FEW_KEYS) ? 0 : std::max<int64_t>(1, (groups - prefix_groups) * 4 / S::WAVES / kv_heads);
+            p.shares = splits<S>(tiles, keys, groups, p.shared) ? std::max<int64_t>(1, (groups - prefix_groups) * 4 / S::WAVES / kv_heads) : 0;
             p.blocks = (p.shares > 0 ? p.shares : p.most_tiles) * kv_heads;
             (void)steps_of(p.most_tiles, keys, S::STEP, p.step_log2);
         };

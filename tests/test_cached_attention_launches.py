@@ -62,8 +62,8 @@ def test_no_launch_has_2_to_the_32_threads():
 
 def test_few_launches():
     """One kernel where nothing is split or shared, else one more that joins the pieces."""
-    alone = [attention(8, 8 * 4096, 0, 32, 8, 128), attention(512, 512, 0, 32, 8, 128), attention(8, 8, 0, 32, 8, 128, columns=100)]
-    joined = [attention(8, 8, 0, 32, 8, 128), attention(1, 1, 0, 8, 8, 128), attention(64, 64, 8192, 32, 8, 128), attention(1, 500, 0, 8, 1, 128)]
+    alone = [attention(8, 8 * 4096, 0, 32, 8, 128), attention(512, 512, 0, 32, 8, 128), attention(8, 8, 0, 32, 8, 128, columns=60)]
+    joined = [attention(8, 8, 0, 32, 8, 128), attention(8, 8, 0, 32, 8, 128, columns=100), attention(1, 1, 0, 8, 8, 128), attention(64, 64, 8192, 32, 8, 128), attention(1, 500, 0, 8, 1, 128)]
     for r in record(alone):
         assert len(r.launches) == 1, r
     for r in record(joined):
