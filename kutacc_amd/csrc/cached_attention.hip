@@ -1074,7 +1074,8 @@ __global__ __launch_bounds__(OWN::THREADS, OWN::D <= 128 ? 2 : 1) void cached_at
     }
 }
 
-// The pieces of a row, those of the prefix in order, then its sequence's, WAVES of them side by side.
+// The pieces of a row, those of the prefix in order, then its sequence's: WAVES waves of a row's side by side, where there are few rows, or ROWS rows in a wave, as a row is one
+// read after the other, of its place, its sums, its results (3 sequences of 700 tokens, 67000 rows: 167 us with the products, 196 with a wave for each row).
 struct CombineParams {
     const float *prefix_partial, *partial;
     const float2 *prefix_sums, *sums;
@@ -1089,15 +1090,16 @@ struct CombineParams {
     float *lse;
 };
 
-template <int D, int WAVES>
+template <int D, int WAVES, int ROWS>
 __global__ __launch_bounds__(256) void combine_kernel(const CombineParams p)
 {
-    constexpr int PER_GROUP = 4 / WAVES, V = D / 64, AHEAD = 8;
+    static_assert(WAVES == 1 || (WAVES == 4 && ROWS == 1), "");
+    constexpr int PER_GROUP = 4 / WAVES * ROWS, LANES = 64 / ROWS, V = D / LANES, AHEAD = V > 8 ? 4 : 8, STORED = V < 8 ? V : 8;
     __shared__ float shared[WAVES > 1 ? WAVES * (D + 2) : 1];
-    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), part = WAVES > 1 ? wave : 0;
+    const int lane = (int)threadIdx.x & (LANES - 1), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), part = WAVES > 1 ? wave : 0;
     const int64_t count = (int64_t)p.tokens * p.heads;
     const int from = p.query_starts[0], to = p.query_starts[p.sequences];
-    for (int64_t index = (int64_t)blockIdx.x * PER_GROUP + (WAVES > 1 ? 0 : wave); index < count; index += (int64_t)gridDim.x * PER_GROUP) {
+    for (int64_t index = (int64_t)blockIdx.x * PER_GROUP + (WAVES > 1 ? 0 : (int)threadIdx.x / LANES); index < count; index += (int64_t)gridDim.x * PER_GROUP) {
         const int token = (int)(index / p.heads), head = (int)(index - (int64_t)token * p.heads);
         const int4 own = p.rows[index];
         if (token < from || token >= to) {
@@ -1194,13 +1196,16 @@ __global__ __launch_bounds__(256) void combine_kernel(const CombineParams p)
         }
         const float over = total == 0.f ? 0.f : 1.f / total;
         bf16_t *out = p.out + token * p.out_token + head * p.out_head;
-        if (V * lane < p.size) { // a multiple of 8
-            bf16_t r[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                r[e] = (bf16_t)(v[e] * over);
+        for (int at = 0; at < V; at += STORED) {
+            if (V * lane + at < p.size) { // a multiple of 8
+                bf16_t r[STORED];
+#pragma unroll
+                for (int e = 0; e < STORED; ++e) {
+                    r[e] = (bf16_t)(v[at + e] * over);
+                }
+                __builtin_memcpy(out + V * lane + at, r, sizeof(r));
             }
-            __builtin_memcpy(out + V * lane, r, sizeof(r));
         }
         if (p.lse != nullptr && lane == 0) {
             p.lse[index] = total > 0.f ? (most + __log2f(total)) * LN2 : total == 0.f ? -INFINITY : total;
@@ -1228,8 +1233,8 @@ struct Plan {
     int64_t prefix_partial, partial, prefix_sums, sums, rows, bytes; // offsets in the workspace, and its size
 };
 
-// Whether the keys of the sequences' tiles are split among workgroups.  Tiles of many rows: where there are fewer of them than the chip holds, as splitting them writes what a
-// 64th of a tile's products takes.  Tiles of few rows: where there are fewer than four times as many, as long sequences among short ones leave the chip to a few workgroups
+// Whether the keys of the sequences' tiles are split among workgroups.  Tiles of many rows: where there are fewer of them than the chip holds, as what balance gains goes
+// into the pieces (1088 tiles of 4000 entries, 512 workgroups at a time: 306 us split and 24 to join, 292 not).  Tiles of few rows: where there are fewer than four times as many, as long sequences among short ones leave the chip to a few workgroups
 // (64 sequences of 1 to 10000 entries, 8 kv heads: 242 us split, 298 not; all of 3000: 143 and 139), but not for few keys, whose pieces cost more to join than
 // they gain: of one CU's workgroups the keys come with 45 bytes a ns, a second kernel takes 3 us.  With an eighth of the chip's tiles 1024 keys (8 sequences: 700 entries 14.5 us
 // split, 14.1 not, 1 to 1500 14.6 and 18.5), with more 2048 (24 sequences of 1500: 40 and 34 us; of 1 to 3000: 41 and 48).  Behind a shared prefix pieces are joined anyway
@@ -1402,13 +1407,13 @@ int cached_attention(const kutacc_hip_cached_attention_args_t &a, hipStream_t st
                                 plan.tile, (int)plan.pieces, p.tokens, p.heads, p.size, p.sequences, p.group, p.by_prefix_per, p.query_starts, p.out, p.out_token, p.out_head, p.lse};
     const int64_t rows = b.tokens * a.q_heads;
     const bool side_by_side = rows <= 4 * kutacc_cu_count(); // four waves a row
-    const dim3 grid((unsigned)std::min<int64_t>(side_by_side ? rows : (rows + 3) / 4, 1 << 20));
+    const dim3 grid((unsigned)std::min<int64_t>(side_by_side ? rows : (rows + 15) / 16, 1 << 20));
     kutacc_prof::KernelTimer timer("combine_kernel", (double)rows * (double)c.head_size, stream);
     return by_size(c.head_size, [&](auto d) {
         if (side_by_side) {
-            combine_kernel<decltype(d)::value, 4><<<grid, 256, 0, stream>>>(join);
+            combine_kernel<decltype(d)::value, 4, 1><<<grid, 256, 0, stream>>>(join);
         } else {
-            combine_kernel<decltype(d)::value, 1><<<grid, 256, 0, stream>>>(join);
+            combine_kernel<decltype(d)::value, 1, 4><<<grid, 256, 0, stream>>>(join);
         }
         return kutacc_hip_status(hipGetLastError());
     });
