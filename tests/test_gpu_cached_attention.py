@@ -477,6 +477,25 @@ def test_append_saturates_and_keeps_what_is_no_number():
     assert float(got[2, 0]) == float((torch.tensor(1.0) / b.scales[1][0]).to(E4M3).float())
 
 
+def test_quotients_by_any_scale():
+    """Values go into an 8-bit cache as x / scale, rounded to 32 bits, then to the type: the same bytes for every scale, from subnormal ones to the largest."""
+    scales = torch.tensor([0.013, 1 / 3, 7.7, 2.0 ** -60, 2.0 ** -61 * 1.5, 2.0 ** 60, 2.0 ** 61, 2.0 ** -126, 2.0 ** -140, 1e38, 1.0, 0.0999])
+    heads, size, tokens = len(scales), 64, 50
+    g = torch.Generator().manual_seed(4)
+    v = torch.randn(tokens, heads, size, generator=g) * scales[:, None] * torch.exp2(torch.randint(-12, 11, (tokens, heads, size), generator=g).float())
+    v[0, :, :6] = torch.tensor([math.inf, -math.inf, math.nan, 0.0, -0.0, 1e38])
+    v = v.to(BF16)
+    ends = torch.tensor([0, tokens], dtype=INT32).cuda()
+    k_cache, v_cache = (torch.zeros(1, tokens, heads, size, dtype=E4M3, device="cuda") for _ in range(2))
+    batch = capi.CacheBatch(ends, ends[1:], torch.zeros(1, 1, dtype=INT32).cuda())
+    ok(capi.CacheAppend(capi.Cache(k_cache, v_cache, scales.cuda(), scales.cuda()), batch, v.cuda(), v.cuda()))
+    want = (v.float() / scales[:, None]).clamp(-448, 448).to(E4M3)
+    for got in (k_cache, v_cache):
+        got = got[0].cpu()
+        same = (got.view(torch.uint8) == want.view(torch.uint8)) | (got.float().isnan() & want.float().isnan())
+        assert bool(same.all()), [(float(v[t, h, c]), float(scales[h]), float(got[t, h, c]), float(want[t, h, c])) for t, h, c in (~same).nonzero()[:5].tolist()]
+
+
 def test_append_with_positions_of_its_own():
     b = Batch([(4, 10), (2, 2)], 0, 16, 2, 64)
     cache, batch = b.on_gpu()
