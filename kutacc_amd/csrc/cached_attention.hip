@@ -18,6 +18,9 @@
 // The work of a kv head, in steps of keys, is split into equal shares, one for each workgroup, as many as the chip holds at a time; a workgroup whose
 // share goes over the end of a tile goes on with the next one.  The lengths are on the device: every wave sums them up and finds its share by itself.  The pieces of a row
 // meet in a second kernel, in one order.  Where there are tiles enough, or few keys, a workgroup has a tile, and writes its results.
+//
+// 32 heads over 8 of 128, bf16: a token after 131071 entries 103 us, 5.2 TB/s (a large copy: 4.9); 8 after 1 to 1500 14.3 us; 64 after 1 to 1000 behind 8192 52 us (34 at the
+// copy's rate); 4500 tokens of three prompts behind 2000 235 us, 900 TFLOP/s (a large library product: 1200).  256 after 100 to 2000 behind 16384, e4m3: 186 us (119).
 #include <hip/hip_runtime.h>
 #include <math.h>
 
