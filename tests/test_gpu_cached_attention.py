@@ -346,6 +346,25 @@ def test_what_is_not_seen_may_be_anything(heads, queries, size, page):
     assert bool(torch.isfinite(rest).all())
 
 
+@pytest.mark.parametrize("size", [64, 128, 256])
+@pytest.mark.parametrize("heads,queries,length", [(2, 1, 150), (4, 1, 3000), (4, 40, 700)])
+def test_an_infinite_value_that_all_see_stays_one(size, heads, queries, length):
+    """Far in front of every token's end, with a weight that is not zero: infinite in its channel, and nothing changes in the others."""
+    b = Batch([(queries, length)] * 2, 0, 16, 1, size, seed=5)
+    q = randn(9, b.tokens, heads, size)
+    cache, batch = b.on_gpu()
+    clean, out = (torch.empty(b.tokens, heads, size, dtype=BF16, device="cuda") for _ in range(2))
+    ok(capi.CachedAttention(cache, batch, q.cuda(), clean))
+    for at, channel, value in ((3, 0, math.inf), (40, 5, -math.inf), (97, size - 1, math.inf)):
+        b.gpu[1][int(b.table[0, at // 16]), at % 16, 0, channel] = value
+    ok(capi.CachedAttention(cache, batch, q.cuda(), out))
+    got = out[:queries]
+    assert bool((got[..., 0] == math.inf).all()) and bool((got[..., 5] == -math.inf).all()) and bool((got[..., size - 1] == math.inf).all())
+    for t in (got, clean[:queries]):
+        t[..., [0, 5, size - 1]] = 0
+    assert torch.equal(out.view(torch.int16), clean.view(torch.int16))
+
+
 def test_large_logits_and_scales():
     """Logits that grow along the keys, so that the maximum has to be followed, and such that one key has all of the weight."""
     for size, heads, queries in ((64, 4, 1), (128, 4, 40)):
