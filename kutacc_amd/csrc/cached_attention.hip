@@ -702,7 +702,7 @@ __device__ __forceinline__ void attend_few(const AttentionParams &p, const Piece
         const int from_row = 4 * quarter + (row >> 2);
         uint32_t lane_at = (uint32_t)(from_row * S::PITCH + 16 * (((row & 3) >> 1) ^ S::value_swizzle(from_row)) + 8 * (row & 1));
         asm volatile("" : "+v"(lane_at)); // as above
-        // 16 bits of the weights: the second product is no cost here.  Both parts have the weight's sign, and the rest, 2^-20 of the weight larger than it is, is no zero where the
+        // 16 bits of the weights: the second product is no cost here.  Both parts have the weight's sign, and the rest, 2^-30 of the weight larger than it is, is no zero where the
         // weight is none: an infinite value stays one.
         bf16x8 w[KT / 32], rest[KT / 32];
 #pragma unroll
@@ -712,7 +712,7 @@ __device__ __forceinline__ void attend_few(const AttentionParams &p, const Piece
                 const float x = s[2 * t + e / 4][e & 3];
                 const float cut = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
                 w[t][e] = (bf16_t)cut;
-                rest[t][e] = (bf16_t)fmaf(x, 0x1p-20f, x - cut);
+                rest[t][e] = (bf16_t)fmaf(x, 0x1p-30f, x - cut);
             }
         }
         constexpr int OF_32 = D / 16, GROUP = 4, GROUPS = KT / 32 * OF_32 / GROUP;
