@@ -120,7 +120,8 @@ __global__ __launch_bounds__(THREADS) void rotary_kernel(const RotaryParams p)
 {
     constexpr bool CACHED = !std::is_same_v<CACHE, void>, FP8 = std::is_same_v<CACHE, uint8_t>;
     extern __shared__ float2 turns[]; // [per_group][rotated / 2]
-    __shared__ int place_page[MOST_TOKENS], place_slot[MOST_TOKENS], place_position[MOST_TOKENS];
+    __shared__ int place_page[MOST_TOKENS], place_slot[MOST_TOKENS];
+    __shared__ int64_t place_position[MOST_TOKENS]; // a length may be such that they pass 32 bits
     const int tid = (int)threadIdx.x, pairs = p.rotated / 2;
     for (int token0 = (int)blockIdx.x * p.per_group; token0 < p.tokens; token0 += (int)gridDim.x * p.per_group) {
         const int count = min(p.per_group, p.tokens - token0);
@@ -145,7 +146,7 @@ __global__ __launch_bounds__(THREADS) void rotary_kernel(const RotaryParams p)
                             page = (uint32_t)page < (uint32_t)p.pages ? page : NOWHERE;
                         }
                         place_page[t - token0] = page, place_slot[t - token0] = slot;
-                        place_position[t - token0] = (int)(p.prefix_length + at);
+                        place_position[t - token0] = p.prefix_length + at;
                     }
                 }
             }
@@ -153,7 +154,7 @@ __global__ __launch_bounds__(THREADS) void rotary_kernel(const RotaryParams p)
         }
         for (int i = tid; i < count * pairs; i += THREADS) {
             const int t = i / pairs, j = i - t * pairs;
-            const int position = p.positions != nullptr ? p.positions[token0 + t] : CACHED ? place_position[t] : token0 + t;
+            const int64_t position = p.positions != nullptr ? p.positions[token0 + t] : CACHED ? place_position[t] : token0 + t;
             double angle = (double)position * (double)p.inv_freq[j] * TURN;
             angle -= rint(angle);
             float s, c;
