@@ -724,7 +724,8 @@ kutacc_export int kutacc_hip_cache_append(const kutacc_hip_cache_append_args_t *
  * read once for all sequences where they have few tokens each.  bf16 queries and results; products accumulate, and the softmax is held, in fp32, its weights are rounded to
  * bf16 as an operand (16 bits of them are kept where few rows -- tokens times the q_heads / kv_heads that share a head -- take a kernel of
  * their own: up to 16 of a sequence on average, over the prefix up to 16 of the batch).  Sums
- * are taken in one order for given lengths and a GPU: the same bits every time.  Any strides and addresses of q and out.
+ * are taken in one order for given lengths and a GPU: the same bits every time.  Any strides and addresses of q and out; out may be q with the
+ * same strides, and must not overlap an input otherwise.
  * `workspace`: device memory, 256-byte aligned, of at least kutacc_hip_cached_attention_workspace(args) bytes, which reads the sizes alone: no pointer needs to be set.
  */
 typedef struct kutacc_hip_cached_attention_args {

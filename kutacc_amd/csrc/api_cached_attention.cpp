@@ -189,7 +189,7 @@ int kutacc_hip_cached_attention(const kutacc_hip_cached_attention_args_t *args, 
     if (a.batch.tokens == 0 || a.batch.sequences == 0) {
         return 0;
     }
-    if (!batch_of(a.batch) || !cache_of(a.cache) || !readable(a.q) || !writable(a.out, a.batch.tokens, a.q_heads, a.cache.head_size)) {
+    if (!batch_of(a.batch) || !cache_of(a.cache) || !mapped(a.q, a.out, a.batch.tokens, a.q_heads, a.cache.head_size)) {
         return KUTACC_HIP_EINVAL;
     }
     if (!cache_in_pieces(a.cache)) {

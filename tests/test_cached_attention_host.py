@@ -107,6 +107,12 @@ def test_heads_beyond_the_widest():
     assert append(**wide, q_out__head_stride=264, q_out__token_stride=4 * 264, k__head_stride=264, k__token_stride=528, v__head_stride=264, v__token_stride=528) == capi.EUNSUPPORTED
 
 
+def test_results_in_place_have_the_queries_strides():
+    same = dict(q__data=AT, out__data=AT)
+    assert attention(**same, out__token_stride=2048)[0] == capi.EINVAL
+    assert attention(**same, q__head_stride=128)[0] == capi.EINVAL
+
+
 def test_calls_that_do_nothing():
     assert append(batch__tokens=0) == append(batch__sequences=0) == 0
     assert attention(batch__tokens=0) == attention(batch__sequences=0) == (0, 0)

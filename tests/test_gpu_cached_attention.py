@@ -365,6 +365,34 @@ def test_an_infinite_value_that_all_see_stays_one(size, heads, queries, length):
     assert torch.equal(out.view(torch.int16), clean.view(torch.int16))
 
 
+@pytest.mark.parametrize("spans,prefix", [([(1, 300)] * 3, 0), ([(1, 3000)] * 2, 0), ([(1, 100), (3, 700)], 500), ([(60, 300), (40, 1200)], 0), ([(500, 900), (3, 3)], 40)])
+def test_results_in_place_of_the_queries(spans, prefix):
+    for heads, kv_heads, size in ((4, 2, 64), (32, 1, 128)):
+        b = Batch(spans, prefix, 16, kv_heads, size, seed=2)
+        cache, batch = b.on_gpu()
+        q = randn(9, b.tokens, heads, size).cuda()
+        out = torch.empty_like(q)
+        ok(capi.CachedAttention(cache, batch, q, out))
+        ok(capi.CachedAttention(cache, batch, q, q))
+        assert torch.equal(q.view(torch.int16), out.view(torch.int16))
+
+
+def test_positions_past_32_bits():
+    """Of a length that no page table holds: the entry is not kept, its query turned by its position all the same."""
+    b = Batch([(1, 5), (2, 40)], 100, 16, 1, 64)
+    b.lengths[0] = (1 << 31) - 1
+    cache, batch = b.on_gpu()
+    before = b.gpu[0].clone()
+    q, k = randn(1, 3, 2, 64), randn(2, 3, 1, 64)
+    inv_freq, q_out = capi.rotary_frequencies(64), torch.empty(3, 2, 64, dtype=BF16, device="cuda")
+    ok(capi.CacheAppend(cache, batch, k.cuda(), k.cuda(), inv_freq.cuda(), q=q.cuda(), q_out=q_out))
+    want, off = oracle.rotated(q, torch.tensor([100 + (1 << 31) - 2, 138, 139]), inv_freq)
+    off = off + 2.0 ** 31 * 2.0 ** -51 * (oracle.d(q).abs() + oracle.d(q).abs().roll(32, 2))  # the angle's two roundings in 64 bits, here and in the oracle
+    oracle.close(q_out, want, oracle.stored(want, off, BF16), "q")
+    changed = (before.view(torch.int16) != b.gpu[0].view(torch.int16)).any(3).any(2).nonzero().tolist()
+    assert sorted(changed) == sorted([int(b.table[1, at // 16]), at % 16] for at in (38, 39))
+
+
 def test_large_logits_and_scales():
     """Logits that grow along the keys, so that the maximum has to be followed, and such that one key has all of the weight."""
     for size, heads, queries in ((64, 4, 1), (128, 4, 40)):
