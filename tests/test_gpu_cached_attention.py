@@ -346,6 +346,18 @@ def test_what_is_not_seen_may_be_anything(heads, queries, size, page):
     assert bool(torch.isfinite(rest).all())
 
 
+@pytest.mark.parametrize("some,count", [(10, 200), (60, 64), (64, 65), (65, 65), (90, 150), (150, 150)])
+def test_many_sequences_whose_keys_are_split(some, count):
+    """More sequences than a wave has lanes, some of them without tokens, lengths around 2500 among short ones: shares that stay in a tile and such that go over its end."""
+    g = torch.Generator().manual_seed(some)
+    lengths = torch.where(torch.rand(count, generator=g) < 0.1, 2400 + torch.randint(0, 200, (count,), generator=g), torch.randint(1, 90, (count,), generator=g)).tolist()
+    lengths[-1] = lengths[0] = 2600
+    with_tokens = {0, count - 1, *torch.randperm(count, generator=g)[:some - 2].tolist()}
+    spans = [(int(i in with_tokens), n) for i, n in enumerate(lengths)]
+    for prefix in (0, 100):
+        Batch(spans, prefix, 16, 1, 64, seed=1).check(4, what=f"{some} of {count}, prefix {prefix}")
+
+
 @pytest.mark.parametrize("size", [64, 128, 256])
 @pytest.mark.parametrize("heads,queries,length", [(2, 1, 150), (4, 1, 3000), (4, 40, 700)])
 def test_an_infinite_value_that_all_see_stays_one(size, heads, queries, length):
