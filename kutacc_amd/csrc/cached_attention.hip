@@ -1239,19 +1239,21 @@ struct Plan {
     int64_t prefix_partial, partial, prefix_sums, sums, rows, bytes; // offsets in the workspace, and its size
 };
 
-// Whether the keys of the sequences' tiles are split among workgroups.  Tiles of many rows: where there are fewer of them than the chip holds, as what balance gains goes
-// into the pieces (1088 tiles of 4000 entries, 512 workgroups at a time: 306 us split and 24 to join, 292 not).  Tiles of few rows: where there are fewer than four times as many, as long sequences among short ones leave the chip to a few workgroups
-// (64 sequences of 1 to 10000 entries, 8 kv heads: 242 us split, 298 not; all of 3000: 143 and 139), but not for few keys, whose pieces cost more to join than
-// they gain: of one CU's workgroups the keys come with 45 bytes a ns, a second kernel takes 3 us.  With an eighth of the chip's tiles 1024 keys (8 sequences: 700 entries 14.5 us
-// split, 14.1 not, 1 to 1500 14.6 and 18.5), with more 2048 (24 sequences of 1500: 40 and 34 us; of 1 to 3000: 41 and 48).  Behind a shared prefix pieces are joined anyway
-// (32 sequences behind 8192 entries: 34 and 40 us).
+// Whether the keys of the sequences' tiles are split among workgroups: pieces cost a second kernel, 4 us, and their way through memory.  8 kv heads, 4 rows a token:
+// Tiles of many rows: where there are fewer of them than half of what the chip holds, and enough keys for as many; of 512 workgroups 14 keys for each tile (split and not, us: 48
+// tiles of 500 keys 22 and 22, of 700 24 and 27; 72 of 700 29 and 27, of 1000 31 and 32, of 2000 38 and 53; 144 of 1000 43 and 31, of 2000 53 and 53; 120 of 6000 79 split; 450 of 4000
+// 164 and 136), and more than 512 (8 of 500: 20 and 21, of 700: 19 and 24).
+// Tiles of few rows: where there are fewer than four times what the chip holds, as long sequences among short ones leave the chip to a few workgroups (64 of 1 to 10000 entries:
+// 242 us split, 298 not; all of 3000: 143 and 139), and more than 2048 keys (24 of 1500: 40 and 34; of 1 to 3000: 41 and 48).  With an eighth of the chip's tiles more than 1024
+// (8 of 700: 14.5 and 14.1; of 1 to 1500: 14.6 and 18.5: to one CU the keys come with 45 bytes a ns).  Behind a shared prefix, where pieces are joined anyway, more than 256, unless
+// there are more tiles than the chip holds (32 of 1 to 900: 35 and 37; 200 of 1 to 200: 84 and 71, of 1 to 900: 130 and 120).
 template <typename S>
 bool splits(int64_t tiles, int64_t keys, int64_t groups, bool shared)
 {
     if (!S::FEW) {
-        return tiles < groups;
+        return 2 * tiles < groups && keys > 512 && keys * groups > 14 * 512 * tiles;
     }
-    return tiles < 4 * groups && (shared || keys > (tiles <= groups / 8 ? 1024 : 2048));
+    return tiles < 4 * groups && keys > (shared && tiles < groups ? 256 : tiles <= groups / 8 ? 1024 : 2048);
 }
 
 // steps of a share of the prefix
