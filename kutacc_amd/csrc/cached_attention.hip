@@ -1271,10 +1271,12 @@ Plan plan_of(const kutacc_hip_cached_attention_args_t &a)
         constexpr int D = decltype(d)::value;
         const int64_t groups = (D <= 128 ? 2 : 1) * (int64_t)kutacc_cu_count(); // workgroups that are on the chip at a time
         // The prefix's workgroups and the sequences' share the CUs, the ones bound by the matrix cores, the others by memory: they are best done at the same time.  Few of the prefix
-        // leave room for the sequences' and have few pieces to join (64 sequences behind 8192 entries: 256 of them 63 us, 128 54, 64 67); where those would be long, every
-        // CU has one (256 behind 16384: 191, 207 and 369).
+        // leave room for the sequences' and have few pieces to join (64 sequences of 1 to 1000 behind 8192 entries: 256 of them 59 us, 128 53, 64 65); where those would be long, every
+        // CU has one (256 behind 16384, e4m3: 256 of them 191 us, 320 209), and where the sequences' tiles are short beside them, of 128 keys at most and what each costs anyway (64 of
+        // 1 to 200 behind 16000: 128 of them 61 us, 256 46, 512 53; 200 of 1 to 200 behind 3000, which is the other side: 52, 54 and 60).
         const int64_t steps = p.prefix_few ? 0 : (stacked + 127) / 128 * ((b.prefix_length + 63) / 64) * kv_heads;
-        const int64_t prefix_groups = !p.shared ? 0 : steps <= 32 * (groups / 4) ? groups / 4 : groups / 2;
+        const int64_t own_steps = std::max(stacked / (p.few ? 16 : 128), with_tokens) * kv_heads * (1 + (b.columns * a.cache.page_size + 127) / 128);
+        const int64_t prefix_groups = !p.shared ? 0 : steps <= 32 * (groups / 4) && 10 * steps <= 7 * own_steps ? groups / 4 : groups / 2;
         p.d = D;
         // steps of a tile's keys, and so few of them that those of all tiles are counted in 29 bits, of whole shares in 30
         const auto steps_of = [](int64_t tiles, int64_t keys, int step, int &log2) {
@@ -1293,8 +1295,8 @@ Plan plan_of(const kutacc_hip_cached_attention_args_t &a)
             p.tile = S::ROWS, p.waves = S::WAVES;
             p.least = S::WAVES == 8 ? 1 : 2; // of 256 keys and of 128 or 64 (8 sequences of 1 to 1500: 14.6 us, 16.0 with 2 of 256)
             p.most_tiles = stacked / S::ROWS + with_tokens;
-            p.shares = splits<S>(tiles, keys, groups, p.shared) ? std::max<int64_t>(1, (groups - prefix_groups) * 4 / S::WAVES / kv_heads) : 0;
-            p.blocks = (p.shares > 0 ? p.shares : p.most_tiles) * kv_heads;
+            p.shares = splits<S>(tiles, keys, groups, p.shared) ? std::max<int64_t>(1, (groups - p.prefix_shares * kv_heads) * 4 / S::WAVES / kv_heads) : 0;
+            p.blocks = (p.prefix_shares + (p.shares > 0 ? p.shares : p.most_tiles)) * kv_heads;
             (void)steps_of(p.most_tiles, keys, S::STEP, p.step_log2);
         };
         const auto prefix_of = [&](auto shape) {
@@ -1304,17 +1306,16 @@ Plan plan_of(const kutacc_hip_cached_attention_args_t &a)
             const int64_t all = p.prefix_tiles * p.prefix_steps, shares = std::max<int64_t>(1, prefix_groups / kv_heads);
             p.prefix_per = std::max<int64_t>((all + shares - 1) / shares, LEAST_PREFIX);
             p.prefix_shares = (all + p.prefix_per - 1) / p.prefix_per;
-            p.blocks += p.prefix_shares * kv_heads;
         };
+        if (p.shared) {
+            p.prefix_few ? prefix_of(FewRows<D, 4, false>{}) : prefix_of(ManyRows<D, false>{});
+        }
         if (!p.few) {
             tiles_of(ManyRows<D, false>{});
         } else if (D <= 128 && !p.shared && std::max(stacked / 16, with_tokens) * kv_heads <= groups / 2) { // a workgroup a CU: of eight waves
             tiles_of(FewRows<D, D <= 128 ? 8 : 4, false>{});
         } else {
             tiles_of(FewRows<D, 4, false>{});
-        }
-        if (p.shared) {
-            p.prefix_few ? prefix_of(FewRows<D, 4, false>{}) : prefix_of(ManyRows<D, false>{});
         }
         return 0;
     });
