@@ -721,7 +721,7 @@ kutacc_export int kutacc_hip_cache_append(const kutacc_hip_cache_append_args_t *
  * (causal 0) or those up to its own position (causal 1):
  *   out = sum_j softmax_j(scale q k_j) v_j,   lse = ln sum_j exp(scale q k_j)
  * A token that sees nothing gets zeros, and -inf as lse.  Entries that a token does not see may hold anything, infinities and NaN included.  The prefix is
- * read once for all sequences where they have few tokens each.  bf16 queries and results; products accumulate, and the softmax is held, in fp32, its weights are rounded to
+ * read once for all sequences where they have few tokens each and it is long, or they are many.  bf16 queries and results; products accumulate, and the softmax is held, in fp32, its weights are rounded to
  * bf16 as an operand (16 bits of them are kept where few rows -- tokens times the q_heads / kv_heads that share a head -- take a kernel of
  * their own: up to 16 of a sequence on average, over the prefix up to 16 of the batch).  Sums
  * are taken in one order for given lengths and a GPU: the same bits every time.  Any strides and addresses of q and out; out may be q with the

@@ -1266,16 +1266,19 @@ Plan plan_of(const kutacc_hip_cached_attention_args_t &a)
     const int64_t with_tokens = std::min(b.sequences, b.tokens), average = (b.tokens * group + with_tokens - 1) / with_tokens, stacked = b.tokens * group;
     Plan p = {};
     p.few = average <= 16, p.prefix_few = stacked <= 16;
-    p.shared = b.prefix_length > 0 && b.sequences > 1 && average <= 64;
     by_size(a.cache.head_size, [&](auto d) {
         constexpr int D = decltype(d)::value;
         const int64_t groups = (D <= 128 ? 2 : 1) * (int64_t)kutacc_cu_count(); // workgroups that are on the chip at a time
+        const int64_t own_tiles = std::max(stacked / (p.few ? 16 : 128), with_tokens) * kv_heads;
+        // A prefix that each sequence's tiles walk by themselves needs no second kernel (short sequences, 8 kv heads, us shared and by themselves: 16 behind 512 entries 14.5 and
+        // 11.9, behind 1024 15.0 and 16.5; 64 behind 256 16.7 and 13.0, behind 512 17.0 and 18.1; 248 behind 16 35 and 29, behind 256 34 and 44)
+        p.shared = b.sequences > 1 && average <= 64 && (b.prefix_length > 768 || b.prefix_length * own_tiles > 500 * groups);
         // The prefix's workgroups and the sequences' share the CUs, the ones bound by the matrix cores, the others by memory: they are best done at the same time.  Few of the prefix
         // leave room for the sequences' and have few pieces to join (64 sequences of 1 to 1000 behind 8192 entries: 256 of them 59 us, 128 53, 64 65); where those would be long, every
         // CU has one (256 behind 16384, e4m3: 256 of them 191 us, 320 209), and where the sequences' tiles are short beside them, of 128 keys at most and what each costs anyway (64 of
         // 1 to 200 behind 16000: 128 of them 61 us, 256 46, 512 53; 200 of 1 to 200 behind 3000, which is the other side: 52, 54 and 60).
         const int64_t steps = p.prefix_few ? 0 : (stacked + 127) / 128 * ((b.prefix_length + 63) / 64) * kv_heads;
-        const int64_t own_steps = std::max(stacked / (p.few ? 16 : 128), with_tokens) * kv_heads * (1 + (b.columns * a.cache.page_size + 127) / 128);
+        const int64_t own_steps = own_tiles * (1 + (b.columns * a.cache.page_size + 127) / 128);
         const int64_t prefix_groups = !p.shared ? 0 : steps <= 32 * (groups / 4) && 10 * steps <= 7 * own_steps ? groups / 4 : groups / 2;
         p.d = D;
         // steps of a tile's keys, and so few of them that those of all tiles are counted in 29 bits, of whole shares in 30

@@ -294,6 +294,18 @@ def test_prefix_lengths_around_every_border(queries):
         b.check(4, what=f"{queries} {prefix}")
 
 
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+@pytest.mark.parametrize("size", [64, 96, 128, 256])
+@pytest.mark.parametrize("page", [16, 6])
+def test_prefixes_that_are_read_once(page, size, cache):
+    """Long ones, and short ones of many sequences: a batch of 16 rows and less, and more, of each sequence up to 16 and more; a page of the prefix that is not there."""
+    for prefix, spans, heads, kv_heads in ((769, [(1, 50), (1, 1)], 8, 1), (800, [(1, 300), (0, 9), (3, 41), (1, 700)], 4, 2), (1030, [(8, 20), (16, 300), (5, 5)], 4, 1),
+                                           (77, [(1, 1 + i % 90) for i in range(3500)], 1, 1)):
+        b = Batch(spans, prefix, page, kv_heads, size, cache, seed=prefix)
+        b.prefix_pages[prefix // page // 2] = -1
+        b.check(heads, what=f"{prefix} {len(spans)}")
+
+
 @pytest.mark.parametrize("queries,prefix", [(1, 0), (1, 70), (30, 0), (30, 70), (200, 70)])
 def test_pages_that_are_not_there(queries, prefix):
     """Their entries are not seen, whatever number stands for them."""
