@@ -89,7 +89,8 @@ def test_append_refuses(over):
 
 @pytest.mark.parametrize("over", BOTH + [
     dict(q_heads=0), dict(q_heads=3), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.inf), dict(scale=math.nan), dict(causal=2), dict(q__data=None), dict(out__data=None),
-    dict(out__token_stride=255), dict(out__head_stride=0), dict(q__head_stride=-1), dict(workspace=None), dict(workspace=AT + 128), dict(workspace_bytes=256)])
+    dict(out__token_stride=255), dict(out__head_stride=0), dict(q__head_stride=-1), dict(workspace=None, batch__prefix_length=1000),
+    dict(workspace=AT + 128, batch__prefix_length=1000), dict(workspace_bytes=256, batch__prefix_length=1000)])  # a prefix that is shared: results meet there
 def test_attention_refuses(over):
     assert attention(**over)[0] == capi.EINVAL
 
