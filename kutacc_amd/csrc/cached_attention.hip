@@ -1,9 +1,10 @@
 // Attention over a cache of keys and values in pages, behind a prefix that the sequences share.
 //
-//   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q k_j - m),  m close to max_j scale q k_j
+//   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^-8 exp(scale q k_j - m),  m close to max_j scale q k_j
 //
-// m is the largest logit of the first keys, and follows the larger ones of later keys only when they leave it behind by more than 8 powers of two: nothing comes
-// near the ends of fp32 before, and the results are multiplied with exp(m - m') for few tiles instead of most.
+// m is the largest logit of the first keys, and follows the larger ones of later keys only when they leave it behind by more than 8 powers of two: the results are
+// multiplied with exp(m - m') for few tiles instead of most.  With the 2^-8 no weight is above one all the same, and sums of weighted values leave fp32 only where those of a softmax
+// with the exact maximum do.
 //
 // A row is one token's query head; the rows of a tile share a kv head: the tokens of one sequence times the heads of its group, or, over the shared prefix, all of the
 // batch's.  A pass over the keys holds m, the sum and a wave's results in registers, by the transposed products of the matrix instructions: K Q^T leaves a row's
@@ -391,6 +392,13 @@ __device__ __forceinline__ uint4 load16(Buffer from, uint32_t at, uint32_t furth
 }
 constexpr uint32_t PAST_BLOCKS = 1u << 30; // no block is as long
 
+// Powers of two by which m may stay behind the largest logit.  Weights are 2^-BEHIND of what they are to m, at most one, and so are the sums that a piece leaves.
+constexpr float BEHIND = 8.f;
+__device__ __forceinline__ float lse_of(float most, float total) // most in powers of two
+{
+    return total > 0.f ? (most + __log2f(total * 0x1p8f)) * LN2 : total == 0.f ? -INFINITY : total;
+}
+
 // results of a piece's rows: to where they belong, or as a share of them into the workspace
 template <typename S>
 struct Results {
@@ -417,7 +425,7 @@ struct Results {
         place_of(row, token, query_head);
         if (direct) {
             if (p.lse != nullptr) {
-                p.lse[(int64_t)token * p.heads + query_head] = total > 0.f ? (most + __log2f(total)) * LN2 : total == 0.f ? -INFINITY : total;
+                p.lse[(int64_t)token * p.heads + query_head] = lse_of(most, total);
             }
         } else {
             (shared_prefix ? p.prefix_sums : p.sums)[(int64_t)u.at * S::ROWS + row] = make_float2(most, total);
@@ -455,8 +463,6 @@ struct Results {
         }
     }
 };
-
-constexpr float BEHIND = 8.f; // powers of two by which m may stay behind the largest logit
 
 // COUNT groups of N operands, each read from the LDS while the products of the one before it are formed.  Left to itself the compiler reads one operand, waits, and goes on
 // with its product.
@@ -662,7 +668,7 @@ __device__ __forceinline__ void attend_few(const AttentionParams &p, const Piece
                 o[d] *= keep;
             }
         }
-        const float base = (m == -INFINITY ? 0.f : m) * factor; // nothing seen yet: weights of zero
+        const float base = fmaf(m == -INFINITY ? 0.f : m, factor, BEHIND); // nothing seen yet: weights of zero
 #pragma unroll
         for (int b = 0; b < BLOCKS; ++b) {
 #pragma unroll
@@ -953,7 +959,7 @@ __device__ __forceinline__ void attend_many(const AttentionParams &p, const Piec
                 }
             }
         }
-        const float base = (m == -INFINITY ? 0.f : m) * factor; // nothing seen yet: weights of zero
+        const float base = fmaf(m == -INFINITY ? 0.f : m, factor, BEHIND); // nothing seen yet: weights of zero
         bf16x8 w[KT / 16];
 #pragma unroll
         for (int i = 0; i < KT / 16; ++i) {
@@ -1214,7 +1220,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const CombineParams p)
             }
         }
         if (p.lse != nullptr && lane == 0) {
-            p.lse[index] = total > 0.f ? (most + __log2f(total)) * LN2 : total == 0.f ? -INFINITY : total;
+            p.lse[index] = lse_of(most, total);
         }
     }
 }
