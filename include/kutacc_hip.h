@@ -626,7 +626,8 @@ typedef struct kutacc_hip_rotation {
  *   KUTACC_HIP_ROTARY_LINEAR      over `factor`
  *   KUTACC_HIP_ROTARY_BASE        of the base times factor^(rotated / (rotated - 2)): the lowest frequency over `factor`, the highest as it is
  *   KUTACC_HIP_ROTARY_BY_PAIRS    as they are for pairs that turn at least `fast` times over original_length, over `factor` for those that turn at most `slow` times,
- *                                 and mixed linearly in the pair's number between (from the last whole pair at or before the one to the first whole one at or after the other)
+ *                                 and mixed linearly in the pair's number between (from the last whole pair at or before the one, number 0 at the least, to the first whole
+ *                                 one at or after the other, number rotated - 1 at the most)
  *   KUTACC_HIP_ROTARY_BY_TURNS    the same, mixed linearly in the number of turns
  * base > 1, factor >= 1; fast > slow > 0 and original_length > 0 where they are used.
  */

@@ -119,7 +119,7 @@ int kutacc_hip_rotary_frequencies(float *inv_freq, int32_t rotated, int32_t scal
         double stretched = scaling == KUTACC_HIP_ROTARY_LINEAR ? 1.0 : 0.0; // the share of f / factor
         if (scaling == KUTACC_HIP_ROTARY_BY_PAIRS) {
             const double from = std::fmax(std::floor(pair_of(fast)), 0.0), to = std::fmin(std::ceil(pair_of(slow)), rotated - 1.0);
-            stretched = (j - from) / std::fmax(to - from, 0.001);
+            stretched = from < to ? (j - from) / (to - from) : j >= pair_of(slow) ? 1.0 : 0.0; // to <= 0: all pairs are slow; from >= rotated - 1: all are fast
         } else if (scaling == KUTACC_HIP_ROTARY_BY_TURNS) {
             stretched = (fast - original_length * f / two_pi) / (fast - slow);
         }
