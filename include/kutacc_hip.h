@@ -765,7 +765,8 @@ kutacc_export int64_t kutacc_hip_release_staging(void);
 /* Per-kernel timing for benchmarks.  While enabled, each kernel launched by this library is
  * bracketed by hipEvents on its stream.  kutacc_hip_profile_read(i, ...) waits for the recorded
  * events and returns entry i (0 on success, -1 past the last entry): kernel name, summed
- * milliseconds, number of launches and the algorithmic flops of one launch.  Enabling clears the
+ * milliseconds, number of launches and the algorithmic flops of one launch (0: none that count, or not
+ * known to the host, as those of cached attention, whose lengths are on the device).  Enabling clears the
  * previous totals. */
 kutacc_export void kutacc_hip_profile_enable(int on);
 kutacc_export int kutacc_hip_profile_read(int index, char *name, int name_len, double *total_ms, int64_t *launches,

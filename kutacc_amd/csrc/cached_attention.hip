@@ -1346,7 +1346,7 @@ Plan plan_of(const kutacc_hip_cached_attention_args_t &a)
 }
 
 template <typename OWN, typename PREFIX, bool PAGED_BLOCKS>
-int launch_kernel(const AttentionParams &p, int64_t blocks, double flops, hipStream_t stream)
+int launch_kernel(const AttentionParams &p, int64_t blocks, hipStream_t stream)
 {
     constexpr int LDS = OWN::LDS > PREFIX::LDS ? OWN::LDS : PREFIX::LDS;
     const auto kernel = cached_attention_kernel<OWN, PREFIX, PAGED_BLOCKS>;
@@ -1354,14 +1354,14 @@ int launch_kernel(const AttentionParams &p, int64_t blocks, double flops, hipStr
     if (const hipError_t e = kutacc_opt_in_lds((const void *)kernel, LDS, opted)) {
         return kutacc_hip_status(e);
     }
-    kutacc_prof::KernelTimer timer("cached_attention_kernel", flops, stream);
+    kutacc_prof::KernelTimer timer("cached_attention_kernel", 0.0, stream); // how many keys there are is known on the device alone
     kernel<<<dim3((unsigned)blocks), OWN::THREADS, LDS, stream>>>(p);
     return kutacc_hip_status(hipGetLastError());
 }
 template <typename OWN, typename PREFIX>
-int launch(const AttentionParams &p, bool paged_blocks, int64_t blocks, double flops, hipStream_t stream)
+int launch(const AttentionParams &p, bool paged_blocks, int64_t blocks, hipStream_t stream)
 {
-    return paged_blocks ? launch_kernel<OWN, PREFIX, true>(p, blocks, flops, stream) : launch_kernel<OWN, PREFIX, false>(p, blocks, flops, stream);
+    return paged_blocks ? launch_kernel<OWN, PREFIX, true>(p, blocks, stream) : launch_kernel<OWN, PREFIX, false>(p, blocks, stream);
 }
 
 } // namespace
@@ -1404,17 +1404,16 @@ int cached_attention(const kutacc_hip_cached_attention_args_t &a, hipStream_t st
             p.prefix_sums = (float2 *)(workspace + plan.prefix_sums), p.prefix_partial = (float *)(workspace + plan.prefix_partial);
         }
     }
-    const double flops = 4.0 * (double)c.head_size * (double)a.q_heads * (double)b.tokens * (double)std::max<int64_t>(b.prefix_length, 1);
     const int rc = by_size(c.head_size, [&](auto d) {
         constexpr int D = decltype(d)::value;
         const auto of_type = [&](auto fp8) {
             using Few = FewRows<D, 4, decltype(fp8)::value>;
             using Wide = FewRows<D, D <= 128 ? 8 : 4, decltype(fp8)::value>;
             using Many = ManyRows<D, decltype(fp8)::value>;
-            return !plan.few                           ? launch<Many, Many>(p, paged_blocks, plan.blocks, flops, stream)
-                   : plan.shared && !plan.prefix_few ? launch<Few, Many>(p, paged_blocks, plan.blocks, flops, stream)
-                   : plan.waves == 8                 ? launch<Wide, Wide>(p, paged_blocks, plan.blocks, flops, stream)
-                                                     : launch<Few, Few>(p, paged_blocks, plan.blocks, flops, stream);
+            return !plan.few                           ? launch<Many, Many>(p, paged_blocks, plan.blocks, stream)
+                   : plan.shared && !plan.prefix_few ? launch<Few, Many>(p, paged_blocks, plan.blocks, stream)
+                   : plan.waves == 8                 ? launch<Wide, Wide>(p, paged_blocks, plan.blocks, stream)
+                                                     : launch<Few, Few>(p, paged_blocks, plan.blocks, stream);
         };
         return c.dtype == KUTACC_DTYPE_E4M3 ? of_type(std::true_type{}) : of_type(std::false_type{});
     });
@@ -1426,7 +1425,7 @@ int cached_attention(const kutacc_hip_cached_attention_args_t &a, hipStream_t st
     const int64_t rows = b.tokens * a.q_heads;
     const bool side_by_side = rows <= 4 * kutacc_cu_count(); // four waves a row
     const dim3 grid((unsigned)std::min<int64_t>(side_by_side ? rows : (rows + 15) / 16, 1 << 20));
-    kutacc_prof::KernelTimer timer("combine_kernel", (double)rows * (double)c.head_size, stream);
+    kutacc_prof::KernelTimer timer("combine_kernel", 0.0, stream); // nor how many pieces
     return by_size(c.head_size, [&](auto d) {
         if (side_by_side) {
             combine_kernel<decltype(d)::value, 4, 1><<<grid, 256, 0, stream>>>(join);
