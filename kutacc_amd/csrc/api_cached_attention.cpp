@@ -135,14 +135,13 @@ int kutacc_hip_rotary(const kutacc_hip_rotary_args_t *args, void *stream)
         return KUTACC_HIP_EINVAL;
     }
     const kutacc_hip_rotary_args_t &a = *args;
-    if (a.tokens < 0 || a.tokens > MAX_INDEX || !extent(a.head_size) || (a.dtype != KUTACC_DTYPE_BF16 && a.dtype != KUTACC_DTYPE_FP32) || !rotation_of(a.rotation, a.head_size) ||
-        (a.q.data == nullptr && a.k.data == nullptr)) {
+    if (a.tokens < 0 || a.tokens > MAX_INDEX || !extent(a.head_size) || (a.dtype != KUTACC_DTYPE_BF16 && a.dtype != KUTACC_DTYPE_FP32) || !rotation_of(a.rotation, a.head_size)) {
         return KUTACC_HIP_EINVAL;
     }
-    if (a.tokens == 0) {
+    if (a.tokens == 0) { // tensors of no element may have no address
         return 0;
     }
-    if ((a.q.data != nullptr && !mapped(a.q, a.q_out, a.tokens, a.q_heads, a.head_size)) || (a.k.data != nullptr && !mapped(a.k, a.k_out, a.tokens, a.k_heads, a.head_size))) {
+    if ((a.q.data == nullptr && a.k.data == nullptr) || (a.q.data != nullptr && !mapped(a.q, a.q_out, a.tokens, a.q_heads, a.head_size)) || (a.k.data != nullptr && !mapped(a.k, a.k_out, a.tokens, a.k_heads, a.head_size))) {
         return KUTACC_HIP_EINVAL;
     }
     return kutacc_launch::rotary(a, kutacc_api::stream_or_default(stream));
