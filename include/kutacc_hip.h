@@ -606,8 +606,8 @@ typedef struct kutacc_hip_heads {
  * Rotary positions.  The channels first .. first + rotated - 1 of a head are rotated / 2 pairs; pair j of a token at position t is turned by the angle
  * t inv_freq[j]:
  *   a' = magnitude (a cos - b sin),  b' = magnitude (b cos + a sin)      (inverse: by the negative angle)
- * (a, b) are channels (first + j, first + rotated / 2 + j), or with `interleaved` (first + 2 j, first + 2 j + 1).  The angle is the exact product of the
- * position and the fp32 frequency, reduced in 64 bits; its sine and cosine and the turn are fp32.  rotated == 0: nothing is turned.
+ * (a, b) are channels (first + j, first + rotated / 2 + j), or with `interleaved` (first + 2 j, first + 2 j + 1).  The angle is the product of the
+ * position and the fp32 frequency in 64 bits, reduced there; its sine and cosine, their products with the magnitude and the turn are fp32.  rotated == 0: nothing is turned.
  */
 typedef struct kutacc_hip_rotation {
     const float *inv_freq; /* [rotated / 2] */
@@ -722,10 +722,11 @@ kutacc_export int kutacc_hip_cache_append(const kutacc_hip_cache_append_args_t *
  * (causal 0) or those up to its own position (causal 1):
  *   out = sum_j softmax_j(scale q k_j) v_j,   lse = ln sum_j exp(scale q k_j)
  * A token that sees nothing gets zeros, and -inf as lse.  Entries that a token does not see may hold anything, infinities and NaN included.  The prefix is
- * read once for all sequences where they have few tokens each and it is long, or they are many.  bf16 queries and results; products accumulate, and the softmax is held, in fp32, its weights are rounded to
+ * read once for all sequences where they have few tokens each and it is long, or they are many.  Logits before their scale, and sums of values with weights of at most one, have to lie in fp32's range.  bf16 queries and results; products accumulate, and the softmax is held, in fp32, its weights are rounded to
  * bf16 as an operand (16 bits of them are kept where few rows -- tokens times the q_heads / kv_heads that share a head -- take a kernel of
- * their own: up to 16 of a sequence on average, over the prefix up to 16 of the batch).  Sums
- * are taken in one order for given lengths and a GPU: the same bits every time.  Any strides and addresses of q and out; out may be q with the
+ * their own: up to 16 of a sequence on average, over a prefix that is read once up to 16 of the batch).  Sums
+ * are taken in one order for given lengths, sizes and a GPU: the same bits every time.  Whether a sequence's keys are split among workgroups goes by batch.columns, as the lengths are on the device: a
+ * page table much longer than its sequences costs short ones some time.  Fastest with pages, and a prefix, of a multiple of 16 entries.  Any strides and addresses of q and out; out may be q with the
  * same strides, and must not overlap an input otherwise.
  * `workspace`: device memory, 256-byte aligned, of at least kutacc_hip_cached_attention_workspace(args) bytes, which reads the sizes alone: no pointer needs to be set.
  */

@@ -21,7 +21,7 @@
 // meet in a second kernel, in one order.  Where there are tiles enough, or few keys, a workgroup has a tile, and writes its results.
 //
 // 32 heads over 8 of 128, bf16: a token after 131071 entries 103 us, 5.2 TB/s (a large copy: 4.9); 8 after 1 to 1500 14.3 us; 64 after 1 to 1000 behind 8192 52 us (34 at the
-// copy's rate); 4500 tokens of three prompts behind 2000 235 us, 900 TFLOP/s (a large library product: 1200).  256 after 100 to 2000 behind 16384, e4m3: 186 us (119).
+// copy's rate); 4500 tokens of three prompts behind 2000 239 us, 890 TFLOP/s (a large library product: 1200).  256 after 100 to 2000 behind 16384, e4m3: 187 us (119).
 #include <hip/hip_runtime.h>
 #include <math.h>
 
@@ -1262,7 +1262,8 @@ bool splits(int64_t tiles, int64_t keys, int64_t groups, bool shared)
     return tiles < 4 * groups && keys > (shared && tiles < groups ? 256 : tiles <= groups / 8 ? 1024 : 2048);
 }
 
-// steps of a share of the prefix
+// Steps of a share of the prefix, of 64 keys or 128: fewer are more pieces to join, more are a longer wait for one (us with 2, 4, 8: 64 sequences of 1 to 200 behind 1024 entries 24.2, 20.0, 23.5;
+// 2 of 1 to 300 behind 800 12.6, 13.7, 16.4; 8 of 1 to 900 behind 2000 14.9, 15.0, 18.7; 5 x 4 behind 1000, heads of 64, 14.9, 14.8, 15.2; with 1 19.8)
 constexpr int64_t LEAST_PREFIX = 4;
 
 Plan plan_of(const kutacc_hip_cached_attention_args_t &a)
@@ -1277,7 +1278,9 @@ Plan plan_of(const kutacc_hip_cached_attention_args_t &a)
         const int64_t groups = (D <= 128 ? 2 : 1) * (int64_t)kutacc_cu_count(); // workgroups that are on the chip at a time
         const int64_t own_tiles = std::max(stacked / (p.few ? 16 : 128), with_tokens) * kv_heads;
         // A prefix that each sequence's tiles walk by themselves needs no second kernel (short sequences, 8 kv heads, us shared and by themselves: 16 behind 512 entries 14.5 and
-        // 11.9, behind 1024 15.0 and 16.5; 64 behind 256 16.7 and 13.0, behind 512 17.0 and 18.1; 248 behind 16 35 and 29, behind 256 34 and 44)
+        // 11.9, behind 1024 15.0 and 16.5; 64 behind 256 16.7 and 13.0, behind 512 17.0 and 18.1; 248 behind 16 35 and 29, behind 256 34 and 44).  A length that is no multiple of 16,
+        // which those tiles read entry by entry, moves the border by little (1 to 200 of their own: 64 behind 300 21 and 17, behind 500 19 and 21; 248 behind 33 42 and 41, behind 100 42 and
+        // 46, behind 200 42 and 52).
         p.shared = b.sequences > 1 && average <= 64 && (b.prefix_length > 768 || b.prefix_length * own_tiles > 500 * groups);
         // The prefix's workgroups and the sequences' share the CUs, the ones bound by the matrix cores, the others by memory: they are best done at the same time.  Few of the prefix
         // leave room for the sequences' and have few pieces to join (64 sequences of 1 to 1000 behind 8192 entries: 256 of them 59 us, 128 53, 64 65); where those would be long, every
@@ -1390,6 +1393,8 @@ int cached_attention(const kutacc_hip_cached_attention_args_t &a, hipStream_t st
     p.pages = (int)c.pages, p.own_limit = (int)(b.columns * c.page_size), p.prefix_length = (int)b.prefix_length;
     p.joined = b.prefix_length > 0 && !plan.shared;
     const auto near = [](int64_t stride) { return stride < 1 << 26; }; // 16 entries within 2^30 bytes
+    // Entry by entry otherwise, with a shuffle and an address for each load: prompts behind 2001 entries 299 us, behind 2000 248; 64 single tokens of 1 to 200 behind 500 21, behind 496 20; pages of
+    // one entry 72, of 16 66 (64 of 100 to 2000)
     const bool paged_blocks = c.page_size % 16 == 0 && (!p.joined || b.prefix_length % 16 == 0) && near(p.k_token) && near(p.v_token);
     p.causal = a.causal, p.scale_log2 = a.scale * LOG2E;
     p.page_size = Divisor::of((uint32_t)c.page_size), p.group = Divisor::of((uint32_t)(a.q_heads / c.kv_heads));
